@@ -21,6 +21,31 @@
 #include <string>
 
 #include "stencil_tma.cuh"
+#include "train.hpp"
+
+namespace commux_ops {
+
+std::atomic<std::int64_t> g_launches{0};
+
+// host-mapped status word of the kernels with bounded waits (nonzero: one gave up)
+unsigned* status_word(unsigned** dev) {
+  struct Word {
+    unsigned *host = nullptr, *device = nullptr;
+  };
+  static const Word w = [] {  // made once, whichever thread comes first
+    Word v;
+    C10_CUDA_CHECK(cudaHostAlloc(reinterpret_cast<void**>(&v.host), 64, cudaHostAllocMapped | cudaHostAllocPortable));
+    *v.host = 0;
+    C10_CUDA_CHECK(cudaHostGetDevicePointer(reinterpret_cast<void**>(&v.device), v.host, 0));
+    return v;
+  }();
+  *dev = w.device;
+  return w.host;
+}
+
+}  // namespace commux_ops
+
+void bind_train(pybind11::module& m);  // train.cpp
 
 namespace {
 
@@ -28,7 +53,8 @@ constexpr int kTX = 32;
 constexpr int kTY = 8;
 constexpr int kZB = 16;  // planes per CTA
 
-std::atomic<std::int64_t> g_launches{0};
+using commux_ops::g_launches;
+using commux_ops::status_word;
 
 template <typename T>
 __global__ void __launch_bounds__(kTX* kTY)
@@ -152,19 +178,6 @@ bool use_simple() {
     return e != nullptr && std::string(e) == "simple";
   }();
   return v;
-}
-
-// host-mapped status word of the TMA kernel (nonzero: a bounded wait gave up)
-unsigned* status_word(unsigned** dev) {
-  static unsigned* host = nullptr;
-  static unsigned* device = nullptr;
-  if (host == nullptr) {
-    C10_CUDA_CHECK(cudaHostAlloc(reinterpret_cast<void**>(&host), 64, cudaHostAllocMapped | cudaHostAllocPortable));
-    *host = 0;
-    C10_CUDA_CHECK(cudaHostGetDevicePointer(reinterpret_cast<void**>(&device), host, 0));
-  }
-  *dev = device;
-  return host;
 }
 
 // cuTensorMapEncodeTiled, resolved through the runtime at first use: the
@@ -310,5 +323,6 @@ PYBIND11_MODULE(_ops, m) {
   m.def("jacobi7", &jacobi7, py::arg("u"), py::arg("v"), py::arg("halo"), py::arg("residual") = py::none(),
         py::arg("part") = 0);
   m.def("launches", &launches);
+  bind_train(m);
   m.def("kernel_status", &kernel_status, py::arg("reset") = false);
 }

@@ -1,5 +1,6 @@
 """Compute kernels of the workloads (sm_100a, in commux_b200._ops) and their
-plain-PyTorch references used by the numerics tests."""
+plain-PyTorch references used by the numerics tests: the Jacobi update of the
+halo workload, and the operators of a training step (``ops.train``)."""
 
 from __future__ import annotations
 
@@ -51,3 +52,10 @@ def jacobi7_reference(u: torch.Tensor, v: torch.Tensor, halo: int) -> float:
     new = s / 6
     v[h:-h, h:-h, h:-h] = new
     return float(((new.double() - c.double()) ** 2).sum())
+
+
+from .train import (Act8, cross_entropy, gelu8, layer_norm, linear8, pack8,  # noqa: E402
+                    weight_grad8)
+
+__all__ = ["jacobi7", "jacobi7_reference", "launches", "Act8", "cross_entropy", "gelu8", "layer_norm", "linear8",
+           "pack8", "weight_grad8"]

@@ -7,6 +7,8 @@ random init (seeded), synthetic uniform token ids; DDP with 25 MB gradient
 buckets, all-reduced by the backend on its collective stream while backward
 runs. ``--backend nccl`` runs the same step on NCCL (the comparator: the
 reference backend cannot run DDP at all -- no allgather, no getFuture).
+``--act8`` runs the same model through the training operators with 8-bit
+activation checkpoints (``commux_b200.ops``).
 
     torchrun --nproc-per-node N benchmarks/ddp_gpt.py --backend ucx
 """
@@ -30,6 +32,7 @@ def main():
     ap.add_argument("--micro-batch", type=int, default=8)
     ap.add_argument("--bucket-mb", type=float, default=25.0)
     ap.add_argument("--layers", type=int, default=12)
+    ap.add_argument("--act8", action="store_true", help="training operators with 8-bit activation checkpoints")
     args = ap.parse_args()
 
     import torch
@@ -49,7 +52,7 @@ def main():
     dist.init_process_group(args.backend, rank=rank, world_size=world,
                             timeout=datetime.timedelta(seconds=600))
     torch.manual_seed(0)
-    cfg = GPTConfig(n_layer=args.layers)
+    cfg = GPTConfig(n_layer=args.layers, act8=args.act8)
     model = GPT(cfg).cuda()
     ddp = DDP(model, device_ids=[local], bucket_cap_mb=args.bucket_mb, gradient_as_bucket_view=True)
     opt = torch.optim.AdamW(model.parameters(), lr=3e-4, fused=True)
@@ -87,7 +90,8 @@ def main():
         print(json.dumps({"metric": "DDP GPT-12L tokens/s", "backend": args.backend, "n_gpus": world,
                           "value": round(toks, 1), "ms_per_step": round(ms, 3), "loss": float(loss),
                           "params_M": round(sum(p.numel() for p in model.parameters()) / 1e6, 2),
-                          "micro_batch": B, "seq_len": T, "bucket_mb": args.bucket_mb}), flush=True)
+                          "micro_batch": B, "seq_len": T, "bucket_mb": args.bucket_mb, "act8": args.act8,
+                          "peak_GB": round(torch.cuda.max_memory_allocated() / 1e9, 3)}), flush=True)
     dist.barrier()
     dist.destroy_process_group()
 

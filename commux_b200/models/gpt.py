@@ -5,6 +5,12 @@ autocast with fp32 master weights under torch DDP on the commux backend.
 Plain library kernels (cuBLAS GEMMs, flash SDPA) do the math; the backend's
 job here is the gradient all-reduce of DDP's buckets, overlapped with the
 backward pass on the collective stream.
+
+With ``GPTConfig(act8=True)`` the same weights run through ``commux_b200.ops``
+(CUDA only): the residual sums inside the norms, every linear layer's input
+but the attention's (which flash SDPA keeps anyway) held in 8 bits for its
+weight's gradient, the norms' and GELU's backward passes from those same
+checkpoints, and the loss with its gradient in one pass over the logits.
 """
 
 from __future__ import annotations
@@ -16,6 +22,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .. import ops
+
 
 @dataclass
 class GPTConfig:
@@ -25,6 +33,7 @@ class GPTConfig:
     d_ff: int = 3072
     vocab: int = 32000
     seq_len: int = 1024
+    act8: bool = False  # training operators with 8-bit activation checkpoints
 
 
 class Block(nn.Module):
@@ -39,15 +48,36 @@ class Block(nn.Module):
         self.n_head = c.n_head
 
     def forward(self, x):
-        B, T, C = x.shape
-        q, k, v = self.qkv(self.ln1(x)).split(C, dim=2)
+        x = x + self.proj(self._attend(self.qkv(self.ln1(x))))
+        return x + self.out(F.gelu(self.fc(self.ln2(x)), approximate="tanh"))
+
+    def forward8(self, x, r):
+        """The block on the stream ``x`` and what is still to be added to it
+        (None before the first block); returns the same pair."""
+        x, y, kept = _norm8(self.ln1, x, r)
+        r = self.proj(self._attend(ops.linear8(y, self.qkv.weight, self.qkv.bias, act8=kept)))
+        x, y, kept = _norm8(self.ln2, x, r)
+        a, kept = ops.gelu8(ops.linear8(y, self.fc.weight, self.fc.bias, act8=kept), pack=True)
+        return x, ops.linear8(a, self.out.weight, self.out.bias, act8=kept)
+
+    def _attend(self, qkv):
+        B, T, C = qkv.shape[0], qkv.shape[1], qkv.shape[2] // 3
+        q, k, v = qkv.split(C, dim=2)
         h = self.n_head
         q = q.view(B, T, h, C // h).transpose(1, 2)
         k = k.view(B, T, h, C // h).transpose(1, 2)
         v = v.view(B, T, h, C // h).transpose(1, 2)
         y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
-        x = x + self.proj(y.transpose(1, 2).reshape(B, T, C))
-        return x + self.out(F.gelu(self.fc(self.ln2(x)), approximate="tanh"))
+        return y.transpose(1, 2).reshape(B, T, C)
+
+
+def _norm8(ln, x, r):
+    """(s, y, y's checkpoint) of ``s = x + r`` (s is x when r is None)."""
+    if r is None:
+        y, kept = ops.layer_norm(x, ln.weight, ln.bias, ln.eps, pack=True)
+        return x, y, kept
+    y, s, kept = ops.layer_norm(x, ln.weight, ln.bias, ln.eps, residual=r, pack=True)
+    return s, y, kept
 
 
 class GPT(nn.Module):
@@ -77,9 +107,21 @@ class GPT(nn.Module):
     def forward(self, idx, targets=None):
         B, T = idx.shape
         x = self.tok(idx) + self.pos(torch.arange(T, device=idx.device))
+        if self.c.act8:
+            return self._forward8(x, targets)
         for b in self.blocks:
             x = b(x)
         logits = self.head(self.ln(x))
         if targets is None:
             return logits
         return F.cross_entropy(logits.float().view(-1, logits.size(-1)), targets.view(-1))
+
+    def _forward8(self, x, targets):
+        r = None
+        for b in self.blocks:
+            x, r = b.forward8(x, r)
+        _, y, kept = _norm8(self.ln, x, r)
+        logits = ops.linear8(y, self.head.weight, act8=kept)
+        if targets is None:
+            return logits
+        return ops.cross_entropy(logits, targets)

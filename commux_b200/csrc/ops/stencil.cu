@@ -43,6 +43,14 @@ unsigned* status_word(unsigned** dev) {
   return w.host;
 }
 
+std::uint64_t wait_limit_ns() {
+  static const std::uint64_t v = [] {
+    const char* e = std::getenv("COMMUX_KERNEL_WAIT_MS");
+    return static_cast<std::uint64_t>(e ? std::atoll(e) : 2000) * 1000000ull;
+  }();
+  return v;
+}
+
 }  // namespace commux_ops
 
 void bind_train(pybind11::module& m);  // train.cpp
@@ -223,10 +231,7 @@ void launch_tma(const at::Tensor& u, at::Tensor& v, int nz, int ny, int nx, int 
   }
   unsigned* st_dev = nullptr;
   status_word(&st_dev);
-  static const std::uint64_t limit_ns = [] {
-    const char* e = std::getenv("COMMUX_KERNEL_WAIT_MS");
-    return static_cast<std::uint64_t>(e ? std::atoll(e) : 2000) * 1000000ull;
-  }();
+  const std::uint64_t limit_ns = commux_ops::wait_limit_ns();
   dim3 grid((sb.ex + stencil::kTX - 1) / stencil::kTX, (sb.ey + stencil::kTY - 1) / stencil::kTY,
             (sb.ez + stencil::kZB - 1) / stencil::kZB);
   stencil::jacobi7_tma_kernel<T><<<grid, stencil::kThreads, B::kSmem, stream>>>(

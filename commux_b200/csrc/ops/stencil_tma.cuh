@@ -22,6 +22,8 @@
 
 #include <cstdint>
 
+#include "async.cuh"
+
 namespace stencil {
 
 constexpr int kTX = 64;      // interior points per CTA along x
@@ -40,54 +42,11 @@ struct Box {
   static constexpr int kSmem = kStages * kStride + kStages * 8;
 };
 
-__device__ __forceinline__ std::uint32_t smem_u32(const void* p) {
-  return static_cast<std::uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ std::uint64_t gtimer() {
-  std::uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-__device__ __forceinline__ void mbar_init(std::uint64_t* bar, unsigned count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(std::uint64_t* bar, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-               : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(std::uint64_t* bar, unsigned parity) {
-  unsigned done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      " selp.b32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
-// Bounded wait; false if it gave up.
-__device__ __forceinline__ bool mbar_wait(std::uint64_t* bar, unsigned parity, std::uint64_t limit_ns) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const std::uint64_t t0 = gtimer();
-  while (!mbar_try_wait(bar, parity)) {
-    if (gtimer() - t0 > limit_ns) return false;
-  }
-  return true;
-}
-
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
-                                            std::uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<std::uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
+using async::gtimer;
+using async::mbar_expect_tx;
+using async::mbar_init;
+using async::mbar_wait;
+using async::tma_load_3d;
 
 // x origin of the box for tile bx (rounded down to 16 bytes) and the shift of
 // the tile's first halo column inside the box.

@@ -2,8 +2,8 @@
 
 // Training operators (sm_100a): what the bindings (train.cpp) hand to the
 // kernels. No torch types here, so the kernels compile without ATen; every
-// launch function enqueues on the given stream, throws nothing and returns
-// the first CUDA error.
+// launch function enqueues on the given stream, and returns the first
+// CUDA error.
 //
 // Matrices are rows of `cols` adjacent elements; `ld*` is the distance
 // between rows in elements. Outputs without an ld are contiguous.
@@ -151,5 +151,6 @@ extern std::atomic<std::int64_t> g_launches;  // kernels this extension launched
 // Host-mapped status word (nonzero after a bounded wait in a kernel gave up)
 // and its device address.
 unsigned* status_word(unsigned** dev);
+std::uint64_t wait_limit_ns();  // bound of every wait in a kernel (COMMUX_KERNEL_WAIT_MS)
 
 }  // namespace commux_ops

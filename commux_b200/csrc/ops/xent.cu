@@ -6,17 +6,43 @@
 // row of the type's lowest value), and x_j - m comes before the product with
 // log2(e), which such a value would overflow. A row of only -inf has no
 // softmax: its loss and gradient are NaN, as is every row with NaN or +inf.
+//
+// A row is read once and lives in the registers of its threads, 32 elements
+// each, from the maximum to the gradient. Rows up to 16 K elements have a block
+// of their own and many blocks an SM, so that some load while others compute.
+// Longer rows fill an SM's registers; there one block of 1024 threads walks
+// over rows, whose elements come through shared memory by bulk copies that run
+// ahead of it, and up to 8 blocks (a cluster) share a row that is longer still
+// or one of few.
 
+#include <cooperative_groups.h>
+
+#include "async.cuh"
 #include "train_utils.cuh"
 
 namespace train {
 
 namespace {
 
-constexpr int kThreads = 512;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kEach = 32;      // elements of a thread
+constexpr int kSweep = 512;
 
+__device__ __forceinline__ float nan_value() { return __int_as_float(0x7fffffff); }
 __device__ __forceinline__ bool bad_target(const Xent& a, std::int64_t t) { return t < 0 || t >= a.cols; }
+
+// exp2; results under 2^-126 become 0, which no sum or gradient here can tell
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float larger(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 
 // work[0] = number of rows that count
 __global__ void __launch_bounds__(1024) count_rows(const Xent a) {
@@ -28,51 +54,6 @@ __global__ void __launch_bounds__(1024) count_rows(const Xent a) {
   if (threadIdx.x == 0) a.work[0] = sum;
 }
 
-// dx of a row from its maximum, its sum and the factor of its gradient
-__device__ __forceinline__ void write_row(const Xent& a, std::int64_t row, float m, float s, std::int64_t target,
-                                          float f, bool counts) {
-  const float inv = 1.0f / s;
-  const bool bad = counts && bad_target(a, target);
-  for (std::int64_t i = threadIdx.x; i < a.cols; i += blockDim.x) {
-    float d = 0.0f;
-    if (counts) {
-      d = exp2f((load(a.x.p, a.x.t, row * a.x.ld + i) - m) * kLog2e) * inv;
-      if (i == target) d -= 1.0f;
-      d = bad ? __int_as_float(0x7fffffff) : d * f;
-    }
-    store(a.dx, a.x.t, row * a.cols + i, d);
-  }
-}
-
-__global__ void __launch_bounds__(kThreads) xent_sweep(const Xent a) {
-  __shared__ float slots[32];
-  const float count = a.reduction == 1 ? a.work[0] : 1.0f;
-  float* losses = a.reduction == 0 ? a.loss : a.work + 1;
-  for (std::int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const std::int64_t target = a.target[row];
-    const bool counts = target != a.ignore;
-    float m = -INFINITY, s = 0.0f, loss = 0.0f;
-    if (counts) {
-      for (std::int64_t i = threadIdx.x; i < a.cols; i += kThreads) {
-        const float v = load(a.x.p, a.x.t, row * a.x.ld + i);
-        m = v > m || v != v ? v : m;
-      }
-      m = block_max(m, slots);
-      for (std::int64_t i = threadIdx.x; i < a.cols; i += kThreads)
-        s += exp2f((load(a.x.p, a.x.t, row * a.x.ld + i) - m) * kLog2e);
-      s = block_sum(s, slots);
-      loss = bad_target(a, target) ? __int_as_float(0x7fffffff)
-                                   : logf(s) + (m - load(a.x.p, a.x.t, row * a.x.ld + target));
-    }
-    if (threadIdx.x == 0) {
-      losses[row] = loss;
-      a.stats[row] = m;
-      a.stats[a.rows + row] = s;
-    }
-    if (a.dx != nullptr) write_row(a, row, m, s, target, 1.0f / count, counts);
-  }
-}
-
 // mean or sum of the rows' losses, in a fixed order
 __global__ void __launch_bounds__(1024) join_losses(const Xent a) {
   __shared__ float slots[32];
@@ -82,7 +63,329 @@ __global__ void __launch_bounds__(1024) join_losses(const Xent a) {
   if (threadIdx.x == 0) *a.loss = a.reduction == 1 ? v / a.work[0] : v;
 }
 
-__global__ void __launch_bounds__(kThreads) xent_again(const Xent a, const float* gout, bool have_unit) {
+// The target's logit; NaN where the target names none.
+__device__ __forceinline__ float target_logit(const Xent& a, std::int64_t row, std::int64_t target) {
+  return bad_target(a, target) ? nan_value() : load(a.x.p, a.x.t, row * a.x.ld + target);
+}
+
+// What is known of a row once its maximum and sum are (one thread).
+__device__ __forceinline__ void finish_row(const Xent& a, std::int64_t row, std::int64_t target, float logit, float m,
+                                           float s) {
+  const float loss = target != a.ignore ? logf(s) + (m - logit) : 0.0f;
+  (a.reduction == 0 ? a.loss : a.work + 1)[row] = loss;
+  a.stats[row] = m;
+  a.stats[a.rows + row] = s;
+}
+
+// A row's elements in registers: each thread has kEach / E vectors of E = 16
+// bytes' worth, `threads` vectors apart. Vectors start on 16-byte boundaries: a
+// row that does not begins `shift` elements into its first one. The 16 bytes
+// around a row's first and last element belong to its allocation (which starts
+// and ends on such a boundary), and what is not the row's is masked.
+template <typename T>
+struct Row {
+  static constexpr int E = 16 / sizeof(T), kVectors = kEach / E;
+  float v[kEach];
+
+  static __device__ __forceinline__ void widen(uint4 w, float* to) {
+    if constexpr (sizeof(T) == 4) {
+      to[0] = __uint_as_float(w.x), to[1] = __uint_as_float(w.y), to[2] = __uint_as_float(w.z),
+      to[3] = __uint_as_float(w.w);
+    } else {
+      const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = Elem<T>::get2(u[i]);
+        to[2 * i] = f.x;
+        to[2 * i + 1] = f.y;
+      }
+    }
+  }
+
+  static __device__ __forceinline__ uint4 narrow(const float* v) {
+    if constexpr (sizeof(T) == 4)
+      return uint4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    else
+      return uint4{Elem<T>::put2(v[0], v[1]), Elem<T>::put2(v[2], v[3]), Elem<T>::put2(v[4], v[5]),
+                   Elem<T>::put2(v[6], v[7])};
+  }
+
+  // elements [from, to) of vector k's E are the row's; the others do not count
+  __device__ __forceinline__ void mask(int k, int from, int to) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < from || i >= to) v[k * E + i] = -INFINITY;
+  }
+
+  __device__ __forceinline__ float max() const {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < kEach; ++i) m = larger(m, v[i]);
+    return m;
+  }
+
+  __device__ __forceinline__ float exponentials(float m) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      v[i] = exp2_fast((v[i] - m) * kLog2e);
+      s += v[i];
+    }
+    return s;
+  }
+};
+
+// Vector `at` of a row part of `cols` elements that starts `shift` elements
+// into vector 0: which of its elements are the part's.
+template <int E>
+__device__ __forceinline__ void part_of(int at, int shift, int cols, int& from, int& to) {
+  from = at == 0 ? shift : 0;
+  to = min(E, shift + cols - at * E);
+}
+
+// Gradient of a row part: columns [first, first + cols), `shift` as it is in dx.
+// Where dx has the logits' shift its vectors are those of the registers.
+template <typename T>
+__device__ __forceinline__ void write_part(const Xent& a, Row<T>& r, std::int64_t row, int first, int cols, int shift,
+                                           bool aligned, int threads, int t, std::int64_t target, float f, float inv) {
+  constexpr int E = Row<T>::E;
+  T* dx = static_cast<T*>(a.dx) + row * a.cols + first;
+  const bool counts = target != a.ignore;
+  const float scale = !counts ? 0.0f : bad_target(a, target) ? nan_value() : f * inv;
+  const std::int64_t mine = target - first + shift;  // in elements of the vectors
+#pragma unroll
+  for (int k = 0; k < Row<T>::kVectors; ++k) {
+    const int at = k * threads + t;
+    if (at * E >= shift + cols) break;
+    float* v = r.v + k * E;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      v[i] = counts ? v[i] * scale : 0.0f;
+      if (counts && at * E + i == mine) v[i] -= f;
+    }
+    int from, to;
+    part_of<E>(at, shift, cols, from, to);
+    if (aligned && from == 0 && to == E) {
+      *reinterpret_cast<uint4*>(dx + at * E - shift) = Row<T>::narrow(v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (i >= from && i < to) dx[at * E - shift + i] = Elem<T>::put(v[i]);
+    }
+  }
+}
+
+__device__ __forceinline__ int shift_of(const void* p, int size) {
+  return static_cast<int>(reinterpret_cast<std::uintptr_t>(p) % 16) / size;
+}
+
+// --- rows up to kEach * 512: a block (or a warp of one) to a row ---
+
+template <typename T>
+__global__ void __launch_bounds__(512) xent_rows(const Xent a, const int group) {
+  __shared__ float slots[2][32];
+  constexpr int E = Row<T>::E;
+  const int id = threadIdx.x / group, t = threadIdx.x - id * group, warps = group >> 5, lane = t & 31;
+  const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * (blockDim.x / group) + id;
+  if (row >= a.rows) return;  // whole warps; a row of more than one has the block alone
+  const int cols = static_cast<int>(a.cols);
+  const T* x = static_cast<const T*>(a.x.p) + row * a.x.ld;
+  const int shift = shift_of(x, sizeof(T));
+  const std::int64_t target = a.target[row];
+  const float logit = t == 0 ? target_logit(a, row, target) : 0.0f;  // on its way early
+  Row<T> r;
+  uint4 w[Row<T>::kVectors];
+#pragma unroll
+  for (int k = 0; k < Row<T>::kVectors; ++k) {
+    const int at = k * group + t;
+    if (at * E < shift + cols) w[k] = *reinterpret_cast<const uint4*>(x - shift + at * E);
+  }
+#pragma unroll
+  for (int k = 0; k < Row<T>::kVectors; ++k) {
+    Row<T>::widen(w[k], r.v + k * E);
+    int from, to;
+    part_of<E>(k * group + t, shift, cols, from, to);
+    r.mask(k, from, to);
+  }
+  float m = warp_max(r.max());
+  if (warps > 1) {
+    if (lane == 0) slots[0][t >> 5] = m;
+    __syncthreads();
+    m = warp_max(lane < warps ? slots[0][lane] : -INFINITY);
+  }
+  float s = warp_sum(r.exponentials(m));
+  if (warps > 1) {
+    if (lane == 0) slots[1][t >> 5] = s;
+    __syncthreads();
+    s = warp_sum(lane < warps ? slots[1][lane] : 0.0f);
+  }
+  if (t == 0) finish_row(a, row, target, logit, m, s);
+  if (a.dx != nullptr) {
+    const bool aligned = shift_of(static_cast<T*>(a.dx) + row * a.cols, sizeof(T)) == shift;
+    write_part<T>(a, r, row, 0, cols, shift, aligned, group, t, target,
+                  1.0f / (a.reduction == 1 ? a.work[0] : 1.0f), 1.0f / s);
+  }
+}
+
+// --- longer rows: blocks of 1024 threads, clusters of `kC` to a row ---
+
+constexpr int kLong = 1024;
+constexpr int kPiece = kLong * 16;           // bytes of one vector a thread, one bulk copy
+constexpr int kRing = 12;                    // pieces in shared memory
+constexpr int kRingBytes = kRing * kPiece;
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, std::uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          async::smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(async::smem_u32(bar))
+      : "memory");
+}
+
+template <typename T, int kC>
+__global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* status, std::uint64_t limit_ns) {
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ std::uint64_t full[kRing];
+  __shared__ float slots[2][32], ranks[2][2][8];
+  __shared__ int gave_up;
+  constexpr int E = Row<T>::E, kV = Row<T>::kVectors;
+  namespace cg = cooperative_groups;
+  const int t = threadIdx.x, lane = t & 31;
+  int rank = 0;
+  if constexpr (kC > 1) rank = cg::this_cluster().block_rank();
+  const std::int64_t clusters = gridDim.x / kC, mine = blockIdx.x / kC;
+  // this block's part of every row; parts begin on whole vectors of the columns
+  const std::int64_t share = ((a.cols + kC - 1) / kC + E - 1) / E * E;
+  const int first = static_cast<int>(share * rank);
+  const int cols = static_cast<int>(a.cols - first < share ? (a.cols > first ? a.cols - first : 0) : share);
+  if (t == 0) {
+    for (int i = 0; i < kRing; ++i) async::mbar_init(&full[i], 1);
+    gave_up = 0;
+    async::fence_async();
+  }
+  __syncthreads();
+  if constexpr (kC > 1) cg::this_cluster().sync();  // every block has started: its shared memory can be written
+  const async::Bound bound{&gave_up, status, limit_ns};
+  auto part = [&](std::int64_t row) { return static_cast<const T*>(a.x.p) + row * a.x.ld + first; };
+  // Pieces are numbered through the rows; piece n goes to slot n % kRing. Every
+  // row of this block has the same pieces but for one that a shift may add.
+  auto vectors = [&](std::int64_t row) {
+    return cols == 0 ? 0 : (shift_of(part(row), sizeof(T)) + cols + E - 1) / E;
+  };
+  auto pieces = [&](std::int64_t row) { return (vectors(row) + kLong - 1) / kLong; };
+  unsigned issued = 0, used = 0;
+  std::int64_t ahead = mine;  // the row, and its piece, to ask for next
+  int piece = 0;
+  auto request = [&] {  // thread 0: pieces while they find room
+    while (ahead < a.rows) {
+      const T* x = part(ahead);
+      const char* from = reinterpret_cast<const char*>(x - shift_of(x, sizeof(T)));
+      const int n = pieces(ahead), bytes = vectors(ahead) * 16;
+      for (; piece < n; ++piece, ++issued) {
+        if (issued == used + kRing) return;
+        const unsigned slot = issued % kRing;
+        const unsigned size = min(kPiece, bytes - piece * kPiece);
+        async::mbar_expect_tx(&full[slot], size);
+        bulk_load(ring + slot * kPiece, from + piece * kPiece, size, &full[slot]);
+      }
+      ahead += clusters;
+      piece = 0;
+    }
+  };
+  if (t == 0) request();
+  const float f = 1.0f / (a.reduction == 1 ? a.work[0] : 1.0f);
+  unsigned turn = 0;
+  for (std::int64_t row = mine; row < a.rows; row += clusters, turn ^= 1u) {
+    const int n = pieces(row), shift = shift_of(part(row), sizeof(T));
+    const std::int64_t target = a.target[row];
+    const float logit = t == 0 && rank == 0 ? target_logit(a, row, target) : 0.0f;  // on its way early
+    Row<T> r;
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+      uint4 w = {0, 0, 0, 0};
+      if (k < n) {
+        const unsigned slot = (used + k) % kRing;
+        async::bounded_wait(&full[slot], (used + k) / kRing & 1u, bound);
+        w = *reinterpret_cast<const uint4*>(ring + slot * kPiece + t * 16);
+      }
+      Row<T>::widen(w, r.v + k * E);
+      int from, to;
+      part_of<E>(k * kLong + t, shift, cols, from, to);
+      r.mask(k, from, to);
+    }
+    used += n;
+    float m = warp_max(r.max());
+    if (lane == 0) slots[0][t >> 5] = m;
+    __syncthreads();  // and every thread has its elements: their pieces are free
+    if (t == 0) {
+      async::fence_async();
+      request();
+    }
+    m = warp_max(slots[0][lane]);
+    if constexpr (kC > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      if (t < kC) *cluster.map_shared_rank(&ranks[turn][0][rank], t) = m;
+      cluster.sync();
+      m = warp_max(lane < kC ? ranks[turn][0][lane] : -INFINITY);
+    }
+    float s = warp_sum(r.exponentials(m));
+    if (lane == 0) slots[1][t >> 5] = s;
+    __syncthreads();
+    s = warp_sum(slots[1][lane]);
+    if constexpr (kC > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      if (t < kC) *cluster.map_shared_rank(&ranks[turn][1][rank], t) = s;
+      cluster.sync();
+      s = warp_sum(lane < kC ? ranks[turn][1][lane] : 0.0f);
+    }
+    if (t == 0 && rank == 0) finish_row(a, row, target, logit, m, s);
+    if (a.dx != nullptr) {
+      const bool aligned = shift_of(static_cast<T*>(a.dx) + row * a.cols + first, sizeof(T)) == shift;
+      write_part<T>(a, r, row, first, cols, shift, aligned, kLong, t, target, f, 1.0f / s);
+    }
+  }
+  // shared memory outlives the copies also where a wait gave up
+  if (t == 0 && gave_up != 0)
+    for (unsigned n = used; n < issued; ++n) async::mbar_wait(&full[n % kRing], n / kRing & 1u, limit_ns);
+}
+
+// --- rows longer than a cluster's registers, and gradients formed again ---
+
+// dx of a row from its maximum, its sum and the factor of its gradient
+__device__ __forceinline__ void write_row(const Xent& a, std::int64_t row, float m, float s, std::int64_t target,
+                                          float f, bool counts) {
+  const float inv = 1.0f / s;
+  const bool bad = counts && bad_target(a, target);
+  for (std::int64_t i = threadIdx.x; i < a.cols; i += blockDim.x) {
+    float d = 0.0f;
+    if (counts) {
+      d = exp2_fast((load(a.x.p, a.x.t, row * a.x.ld + i) - m) * kLog2e) * inv;
+      if (i == target) d -= 1.0f;
+      d = bad ? nan_value() : d * f;
+    }
+    store(a.dx, a.x.t, row * a.cols + i, d);
+  }
+}
+
+__global__ void __launch_bounds__(kSweep) xent_sweep(const Xent a) {
+  __shared__ float slots[32];
+  const float count = a.reduction == 1 ? a.work[0] : 1.0f;
+  for (std::int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const std::int64_t target = a.target[row];
+    float m = -INFINITY, s = 0.0f;
+    if (target != a.ignore) {
+      for (std::int64_t i = threadIdx.x; i < a.cols; i += kSweep) m = larger(m, load(a.x.p, a.x.t, row * a.x.ld + i));
+      m = block_max(m, slots);
+      for (std::int64_t i = threadIdx.x; i < a.cols; i += kSweep)
+        s += exp2_fast((load(a.x.p, a.x.t, row * a.x.ld + i) - m) * kLog2e);
+      s = block_sum(s, slots);
+    }
+    if (threadIdx.x == 0) finish_row(a, row, target, target_logit(a, row, target), m, s);
+    if (a.dx != nullptr) write_row(a, row, m, s, target, 1.0f / count, target != a.ignore);
+  }
+}
+
+__global__ void __launch_bounds__(kSweep) xent_again(const Xent a, const float* gout, bool have_unit) {
   if (have_unit && *gout == 1.0f) return;
   const float count = a.reduction == 1 ? a.work[0] : 1.0f;
   for (std::int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -97,20 +400,67 @@ unsigned grid_of(std::int64_t rows) {
   return static_cast<unsigned>(rows < 1 ? 1 : rows < most ? rows : most);
 }
 
+template <typename T, int kC>
+cudaError_t launch_long(const Xent& a, cudaStream_t stream) {
+  cudaError_t rc = cudaFuncSetAttribute(xent_long<T, kC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  if (rc != cudaSuccess) return rc;
+  const std::int64_t most = sm_count() / kC;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((a.rows < most ? a.rows : most) * kC));
+  cfg.blockDim = dim3(kLong);
+  cfg.dynamicSmemBytes = kRingBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kC;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  unsigned* status = nullptr;
+  commux_ops::status_word(&status);
+  return cudaLaunchKernelEx(&cfg, xent_long<T, kC>, a, status, commux_ops::wait_limit_ns());
+}
+
+template <typename T>
+cudaError_t launch_rows(const Xent& a, cudaStream_t stream) {
+  constexpr int E = Row<T>::E;
+  const std::int64_t need = a.cols + E - 1;  // with the longest shift
+  if (need <= kEach * 512) {
+    const int group = static_cast<int>((need + kEach * 32 - 1) / (kEach * 32)) * 32;
+    const int ids = group == 32 ? 4 : 1;
+    xent_rows<T><<<static_cast<unsigned>((a.rows + ids - 1) / ids), group * ids, 0, stream>>>(a, group);
+    return cudaSuccess;
+  }
+  // the fewest blocks that hold a row, and more where the rows leave SMs idle
+  int c = 1;
+  const int most = kEach * kLong - E;
+  while (c < 8 && ((a.cols + c - 1) / c + E > most || a.rows * c * 2 <= sm_count())) c *= 2;
+  if ((a.cols + c - 1) / c + E > most) {
+    xent_sweep<<<grid_of(a.rows), kSweep, 0, stream>>>(a);
+    return cudaSuccess;
+  }
+  return c == 1 ? launch_long<T, 1>(a, stream)
+                : c == 2 ? launch_long<T, 2>(a, stream) : c == 4 ? launch_long<T, 4>(a, stream) : launch_long<T, 8>(a, stream);
+}
+
 }  // namespace
 
 std::int64_t xent_work(std::int64_t rows) { return 1 + rows; }
 
 cudaError_t xent_forward(const Xent& a, cudaStream_t stream) {
   if (a.reduction == 1) count_rows<<<1, 1024, 0, stream>>>(a), commux_ops::g_launches++;
-  xent_sweep<<<grid_of(a.rows), kThreads, 0, stream>>>(a);
-  commux_ops::g_launches++;
+  if (a.rows > 0) {
+    cudaError_t rc = cudaSuccess;
+    with_type(a.x.t, [&](auto e) { rc = launch_rows<decltype(e)>(a, stream); });
+    if (rc != cudaSuccess) return rc;
+    commux_ops::g_launches++;
+  }
   if (a.reduction != 0) join_losses<<<1, 1024, 0, stream>>>(a), commux_ops::g_launches++;
   return cudaGetLastError();
 }
 
 cudaError_t xent_backward(const Xent& a, const float* gout, bool have_unit, cudaStream_t stream) {
-  xent_again<<<grid_of(a.rows), kThreads, 0, stream>>>(a, gout, have_unit);
+  xent_again<<<grid_of(a.rows), kSweep, 0, stream>>>(a, gout, have_unit);
   commux_ops::g_launches++;
   return cudaGetLastError();
 }

@@ -14,223 +14,191 @@ namespace train {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // independent loads of a thread
 
 // tanh form: x (1 + tanh u) / 2 = x / (1 + exp(-2u)), 2u = k (x + c x^3). The
-// quotient keeps its relative accuracy where the sum 1 + tanh u cancels.
+// quotient keeps its relative accuracy where the sum 1 + tanh u cancels. exp(-2u)
+// is infinite only where x < -6, and x / inf is the limit 0. The constants carry
+// the log2(e) of the exponential.
 constexpr float kK = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kC = 0.044715f;
+constexpr float kE = 1.4426950408889634f;
 
-template <bool kTanh>
-__device__ __forceinline__ float gelu(float x) {
-  if (kTanh) {
-    // exp(-2u) is infinite only where x < -6, and x / inf is the limit 0
-    return __fdividef(x, 1.0f + __expf(-kK * (x + kC * x * x * x)));
-  }
-  return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+__device__ __forceinline__ float2 sigmoid2(float2 x, float2 sq) {  // 1 / (1 + exp(-k x (1 + c x^2)))
+  const float2 z = mul2(x, fma2(sq, both(-kK * kC * kE), both(-kK * kE)));
+  const float2 d = add2(float2{exp2_fast(z.x), exp2_fast(z.y)}, both(1.0f));
+  return {inverse_fast(d.x), inverse_fast(d.y)};
 }
 
 template <bool kTanh>
-__device__ __forceinline__ float gelu_slope(float x) {
-  if (kTanh) {
-    // the slope is 0 or 1 to every bit beyond +-20; the clamp keeps x^2 finite, and a NaN
-    x = x > 20.0f ? 20.0f : x < -20.0f ? -20.0f : x;
-    const float sig = __fdividef(1.0f, 1.0f + __expf(-kK * (x + kC * x * x * x)));
-    return sig + x * sig * (1.0f - sig) * kK * (1.0f + 3.0f * kC * x * x);
-  }
-  return 0.5f * (1.0f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * __expf(-0.5f * x * x);
+__device__ __forceinline__ float2 gelu(float2 x) {
+  if constexpr (kTanh) return mul2(x, sigmoid2(x, mul2(x, x)));
+  const float2 z = mul2(x, both(0.70710678118654752f));
+  return mul2(mul2(x, both(0.5f)), add2(float2{erff(z.x), erff(z.y)}, both(1.0f)));
 }
 
-// What a pass does with values: the four passes differ in that alone, and each
-// runs in the two arrangements below. `In` and `Out` are the element types of
-// its tensors; a pass reads a tensor (kReads) or an 8-bit form (kHeld) or both.
+template <bool kTanh>
+__device__ __forceinline__ float2 gelu_slope(float2 x) {
+  if constexpr (kTanh) {
+    // beyond +-20 the slope is 0 or 1 to every bit; the bound keeps x^2 finite
+    float2 sq = mul2(x, x);
+    sq = float2{fminf(sq.x, 400.0f), fminf(sq.y, 400.0f)};
+    const float2 sig = sigmoid2(x, sq);
+    const float2 rest = fma2(sig, both(-1.0f), both(1.0f));
+    return fma2(mul2(x, sig), mul2(rest, fma2(sq, both(3.0f * kC * kK), both(kK))), sig);
+  }
+  const float2 z = mul2(x, both(0.70710678118654752f)), p = mul2(mul2(x, x), both(-0.5f * kE));
+  const float2 cdf = fma2(float2{erff(z.x), erff(z.y)}, both(0.5f), both(0.5f));
+  return fma2(mul2(x, both(0.39894228040143268f)), float2{exp2_fast(p.x), exp2_fast(p.y)}, cdf);
+}
+
+// What a pass does with its values; the passes differ in that alone. A pass
+// reads a tensor x (kReads), an 8-bit form h (kHeld) or both, writes a tensor y
+// (kWrites) and the 8-bit forms of x and y that it is asked for.
 struct Args {
-  Rows x;                                        // kReads
-  const std::int8_t* q;                          // kHeld
+  Rows x;
+  const std::int8_t* q;
   const std::uint8_t* scale;
-  void* y;                                       // unless null
-  std::int8_t *q1, *q2;                          // forms to write, unless null
-  std::uint8_t *scale1, *scale2;
-  const void *w, *b;                             // unpack: the norm's
+  void* y;
+  std::int8_t *xq, *yq;
+  std::uint8_t *xscale, *yscale;
+  const void *w, *b;  // unpack: the norm's weight and bias
   Type wt;
   std::int64_t rows, cols;
 };
 
 struct Pack {
-  static constexpr bool kReads = true, kHeld = false;
+  static constexpr bool kReads = true, kHeld = false, kWrites = false;
   template <typename T>
-  static __device__ __forceinline__ void apply(const Args&, std::int64_t, float x, float, float& y, float& f1, float&) {
-    y = 0.0f;
-    f1 = x;
-  }
+  static __device__ __forceinline__ void apply(const Args&, int, const float2 (&)[4], const float2 (&)[4],
+                                               float2 (&)[4]) {}
 };
 
+template <bool kAffine>
 struct Unpack {
-  static constexpr bool kReads = false, kHeld = true;
+  static constexpr bool kReads = false, kHeld = true, kWrites = true;
   template <typename T>
-  static __device__ __forceinline__ void apply(const Args& a, std::int64_t col, float, float h, float& y, float&,
-                                               float&) {
-    // 65504 may be held as 2^16, which float16 has no finite value for
-    if (Elem<T>::kType == Type::f16 && a.w == nullptr && fabsf(h) == 65536.0f) h = copysignf(65504.0f, h);
-    if (a.w != nullptr && col < a.cols) h *= load(a.w, a.wt, col);
-    if (a.b != nullptr && col < a.cols) h += load(a.b, a.wt, col);
-    y = h;
+  static __device__ __forceinline__ void apply(const Args& a, int c, const float2 (&)[4], const float2 (&h)[4],
+                                               float2 (&y)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[i] = h[i];
+      if constexpr (kAffine) {
+        const int at = c + 2 * i;
+        const bool one = at < a.cols, two = at + 1 < a.cols;
+        y[i] = mul2(y[i], float2{one ? train::load(a.w, a.wt, at) : 0.0f, two ? train::load(a.w, a.wt, at + 1) : 0.0f});
+        if (a.b != nullptr)
+          y[i] = add2(y[i],
+                      float2{one ? train::load(a.b, a.wt, at) : 0.0f, two ? train::load(a.b, a.wt, at + 1) : 0.0f});
+      } else if constexpr (Elem<T>::kType == Type::f16) {
+        // 65504 may be held as 2^16, which float16 has no finite value for
+        if (fabsf(y[i].x) == 65536.0f) y[i].x = copysignf(65504.0f, y[i].x);
+        if (fabsf(y[i].y) == 65536.0f) y[i].y = copysignf(65504.0f, y[i].y);
+      }
+    }
   }
 };
 
 template <bool kTanh>
 struct GeluForward {
-  static constexpr bool kReads = true, kHeld = false;
+  static constexpr bool kReads = true, kHeld = false, kWrites = true;
   template <typename T>
-  static __device__ __forceinline__ void apply(const Args&, std::int64_t, float x, float, float& y, float& f1,
-                                               float& f2) {
-    y = gelu<kTanh>(x);  // 0 at 0, so the padding of a row's last group stays 0
-    f1 = x;
-    f2 = y;
+  static __device__ __forceinline__ void apply(const Args&, int, const float2 (&x)[4], const float2 (&)[4],
+                                               float2 (&y)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = gelu<kTanh>(x[i]);  // 0 at 0, as past a row's end
   }
 };
 
 template <bool kTanh>
 struct GeluBackward {
-  static constexpr bool kReads = true, kHeld = true;
+  static constexpr bool kReads = true, kHeld = true, kWrites = true;
   template <typename T>
-  static __device__ __forceinline__ void apply(const Args&, std::int64_t, float x, float h, float& y, float&, float&) {
-    y = x * gelu_slope<kTanh>(h);
+  static __device__ __forceinline__ void apply(const Args&, int, const float2 (&x)[4], const float2 (&h)[4],
+                                               float2 (&y)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = mul2(x[i], gelu_slope<kTanh>(h[i]));
   }
 };
 
-// Rows that can be read by eight: a thread takes 8 neighbours, four threads a
-// group. kFlat: the rows follow each other without a gap or a partial group,
-// so the matrix is one row.
-template <typename T, typename Pass, bool kFlat>
-__global__ void __launch_bounds__(kThreads) by_vectors(const Args a) {
-  const std::int64_t ng = (a.cols + kGroup - 1) / kGroup, total = a.rows * ng * 4;
-  const std::int64_t first = static_cast<std::int64_t>(blockIdx.x) * (kThreads * kUnroll) + threadIdx.x;
-  Eight<T> in[kUnroll];
-  uint2 held[kUnroll];
-  unsigned e[kUnroll];
-  std::int64_t xo[kUnroll], yo[kUnroll], col[kUnroll];
-  bool some[kUnroll];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const std::int64_t v = first + u * kThreads;
-    std::int64_t row = 0;
-    if (!kFlat) row = total < (1ll << 31) ? static_cast<unsigned>(v) / static_cast<unsigned>(ng * 4) : v / (ng * 4);
-    col[u] = (v - row * ng * 4) * 8;
-    xo[u] = row * a.x.ld + col[u];
-    yo[u] = row * a.cols + col[u];
-    some[u] = v < total && col[u] < a.cols;
-    in[u].zero();
-    held[u] = uint2{0, 0};
-    e[u] = 1;
-    if (Pass::kReads && some[u]) in[u].load(static_cast<const T*>(a.x.p) + xo[u]);
-    if (Pass::kHeld && some[u]) {
-      held[u] = *reinterpret_cast<const uint2*>(a.q + v * 8);
-      e[u] = a.scale[v >> 2];
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const std::int64_t v = first + u * kThreads;
-    float x[8], h[8], y[8], f1[8], f2[8];
-    if (Pass::kReads) in[u].get(x);
-    if (Pass::kHeld) unpack_eight(held[u], e[u], h);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) Pass::template apply<T>(a, col[u] + i, x[i], h[i], y[i], f1[i], f2[i]);
-    if (a.y != nullptr && some[u]) {
-      Eight<T> out;
-      out.put(y);
-      out.store(static_cast<T*>(a.y) + yo[u]);
-    }
-    if (a.q1 != nullptr) {
-      uint2 q;
-      const unsigned s = pack_eight(f1, q);
-      if (v < total) {
-        *reinterpret_cast<uint2*>(a.q1 + v * 8) = q;
-        if ((threadIdx.x & 3) == 0) a.scale1[v >> 2] = static_cast<std::uint8_t>(s);
-      }
-    }
-    if (a.q2 != nullptr) {
-      uint2 q;
-      const unsigned s = pack_eight(f2, q);
-      if (v < total) {
-        *reinterpret_cast<uint2*>(a.q2 + v * 8) = q;
-        if ((threadIdx.x & 3) == 0) a.scale2[v >> 2] = static_cast<std::uint8_t>(s);
-      }
-    }
-  }
+__device__ __forceinline__ void pack_part(const float2 (&v)[4], std::int8_t* q, std::uint8_t* scale, std::int64_t part,
+                                          bool in) {
+  uint2 bytes;
+  const unsigned e = pack_eight(v, bytes);
+  if (!in) return;
+  *reinterpret_cast<uint2*>(q + part * 8) = bytes;
+  if ((threadIdx.x & 3) == 0) scale[part >> 2] = static_cast<std::uint8_t>(e);
 }
 
-// Any rows: a warp takes kUnroll groups that follow each other, a lane an
-// element of each. Index (32 bits where the counts allow) divides once a warp.
-template <typename T, typename Pass, typename Index>
-__global__ void __launch_bounds__(kThreads) by_lanes(const Args a) {
-  const int lane = threadIdx.x & 31;
-  const Index ng = static_cast<Index>((a.cols + kGroup - 1) / kGroup), total = static_cast<Index>(a.rows) * ng;
-  const Index first = (static_cast<Index>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5)) * kUnroll;
-  if (first >= total) return;
-  Index row = first / ng, at = first - row * ng;
-  T in[kUnroll] = {};
-  std::int8_t held[kUnroll];
+// A thread takes a few parts of 8 elements; four threads hold a group. kFlat:
+// the rows are whole groups without gaps, so the matrix is one long row (and
+// no index is divided); otherwise Index counts parts through the rows.
+constexpr int unroll_of(bool aligned) { return aligned ? 4 : 2; }  // independent loads, as the registers allow
+
+template <typename T, typename Pass, bool kFlat, bool kAligned, typename Index>
+__global__ void __launch_bounds__(kThreads) eights(const Args a) {
+  constexpr int kUnroll = unroll_of(kAligned);
+  const Index per = static_cast<Index>((a.cols + kGroup - 1) / kGroup * 4);  // parts of a row
+  const Index total = static_cast<Index>(a.rows) * per;
+  const Index first = static_cast<Index>(blockIdx.x) * (kThreads * kUnroll) + threadIdx.x;
+  const int cols = kFlat ? 8 : static_cast<int>(a.cols);  // flat: a part is a row of its own
+  Part<T, kAligned> in[Pass::kReads ? kUnroll : 1];
+  uint2 held[kUnroll];
   unsigned e[kUnroll];
-  std::int64_t yo[kUnroll], col[kUnroll];
-  bool some[kUnroll];
+  Index row[kUnroll];
+  int col[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    col[u] = static_cast<std::int64_t>(at) * kGroup + lane;
-    yo[u] = static_cast<std::int64_t>(row) * a.cols + col[u];
-    some[u] = first + u < total && col[u] < a.cols;
-    held[u] = 0;
-    e[u] = 1;
-    if (Pass::kReads && some[u]) in[u] = static_cast<const T*>(a.x.p)[static_cast<std::int64_t>(row) * a.x.ld + col[u]];
-    if (Pass::kHeld && some[u]) {
-      held[u] = a.q[static_cast<std::int64_t>(first + u) * kGroup + lane];
-      e[u] = a.scale[first + u];
+    const Index part = first + u * kThreads;
+    const bool some = part < total;
+    row[u] = kFlat ? part : part / per;
+    col[u] = kFlat ? 0 : static_cast<int>(part - row[u] * per) * 8;
+    if (!some) col[u] = cols;  // past the end: reads 0, writes nothing
+    if (Pass::kReads) {
+      const std::int64_t at = some ? (kFlat ? static_cast<std::int64_t>(part) * 8 : row[u] * a.x.ld) : 0;
+      in[u].load(static_cast<const T*>(a.x.p) + at, col[u], cols);
     }
-    if (++at == ng) at = 0, ++row;
+    if (Pass::kHeld) {
+      held[u] = uint2{0, 0};
+      e[u] = 1;
+      if (some) {
+        held[u] = *reinterpret_cast<const uint2*>(a.q + static_cast<std::int64_t>(part) * 8);
+        e[u] = a.scale[part >> 2];
+      }
+    }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    if (first + u >= total) break;  // the same for a warp
-    float y = 0.0f, f1 = 0.0f, f2 = 0.0f;
-    Pass::template apply<T>(a, col[u], some[u] ? Elem<T>::get(in[u]) : 0.0f,
-                            static_cast<float>(held[u]) * step_of(e[u]), y, f1, f2);
-    if (a.y != nullptr && some[u]) static_cast<T*>(a.y)[yo[u]] = Elem<T>::put(y);
-    const std::int64_t g = first + u;
-    if (a.q1 != nullptr) {
-      const unsigned s = warp_scale(f1);
-      a.q1[g * kGroup + lane] = static_cast<std::int8_t>(quantised(f1, s));
-      if (lane == 0) a.scale1[g] = static_cast<std::uint8_t>(s);
+    const Index part = first + u * kThreads;
+    float2 x[4], h[4], y[4];
+    if (Pass::kReads) in[u].get(x);
+    if (Pass::kHeld) unpack_eight(held[u], e[u], h);
+    Pass::template apply<T>(a, col[u], x, h, y);
+    if (Pass::kWrites) {
+      const bool some = part < total;
+      T* to = static_cast<T*>(a.y) + (some ? (kFlat ? static_cast<std::int64_t>(part) * 8 : row[u] * a.cols) : 0);
+      const int lane = threadIdx.x & 31;
+      Part<T, kAligned>::store(to, col[u], cols, y, lane > 0 && col[u] > 0 && some,
+                               some && (lane == 31 || part + 1 == total || col[u] + 8 >= static_cast<int>(per) * 8));
     }
-    if (a.q2 != nullptr) {
-      const unsigned s = warp_scale(f2);
-      a.q2[g * kGroup + lane] = static_cast<std::int8_t>(quantised(f2, s));
-      if (lane == 0) a.scale2[g] = static_cast<std::uint8_t>(s);
-    }
+    if (Pass::kReads && a.xq != nullptr) pack_part(x, a.xq, a.xscale, part, part < total);
+    if (Pass::kReads && a.yq != nullptr) pack_part(y, a.yq, a.yscale, part, part < total);
   }
 }
 
 template <typename T, typename Pass>
 cudaError_t launch(const Args& a, cudaStream_t stream) {
-  const std::int64_t total = a.rows * groups(a.cols);
-  const auto blocks = [](std::int64_t work, std::int64_t each) { return static_cast<unsigned>((work + each - 1) / each); };
-  if (by_eight(a.x.p, a.x.ld, a.cols)) {
-    const unsigned n = blocks(total * 4, kThreads * kUnroll);
-    if (a.cols % kGroup == 0 && (a.x.ld == a.cols || a.rows == 1) && a.w == nullptr) {
-      Args one = a;
-      one.rows = 1;
-      one.cols = a.rows * a.cols;
-      by_vectors<T, Pass, true><<<n, kThreads, 0, stream>>>(one);
-    } else {
-      by_vectors<T, Pass, false><<<n, kThreads, 0, stream>>>(a);
-    }
-  } else {
-    const unsigned n = blocks(total, kThreads / 32 * kUnroll);
-    if (total < (1ll << 30))
-      by_lanes<T, Pass, unsigned><<<n, kThreads, 0, stream>>>(a);
-    else
-      by_lanes<T, Pass, std::int64_t><<<n, kThreads, 0, stream>>>(a);
-  }
+  const std::int64_t parts = a.rows * groups(a.cols) * 4;
+  const bool small = parts < (1ll << 30), aligned = aligned_rows(a.x.p, a.x.ld, a.cols) && small;
+  const std::int64_t each = kThreads * unroll_of(aligned);
+  const unsigned blocks = static_cast<unsigned>((parts + each - 1) / each);
+  if (aligned && a.cols % kGroup == 0 && (a.x.ld == a.cols || a.rows == 1) && a.w == nullptr)
+    eights<T, Pass, true, true, unsigned><<<blocks, kThreads, 0, stream>>>(a);
+  else if (aligned)
+    eights<T, Pass, false, true, unsigned><<<blocks, kThreads, 0, stream>>>(a);
+  else if (small)
+    eights<T, Pass, false, false, unsigned><<<blocks, kThreads, 0, stream>>>(a);
+  else
+    eights<T, Pass, false, false, std::int64_t><<<blocks, kThreads, 0, stream>>>(a);
   commux_ops::g_launches++;
   return cudaGetLastError();
 }
@@ -248,8 +216,8 @@ cudaError_t pack8(Rows x, std::int8_t* q, std::uint8_t* scale, std::int64_t rows
                   cudaStream_t stream) {
   Args a{};
   a.x = x;
-  a.q1 = q;
-  a.scale1 = scale;
+  a.xq = q;
+  a.xscale = scale;
   a.rows = rows;
   a.cols = cols;
   return launch<Pack>(a, x.t, stream);
@@ -267,17 +235,17 @@ cudaError_t unpack8(const std::int8_t* q, const std::uint8_t* scale, const void*
   a.wt = wt;
   a.rows = rows;
   a.cols = cols;
-  return launch<Unpack>(a, t, stream);
+  return w != nullptr ? launch<Unpack<true>>(a, t, stream) : launch<Unpack<false>>(a, t, stream);
 }
 
 cudaError_t gelu8_forward(const GeluFwd& g, cudaStream_t stream) {
   Args a{};
   a.x = g.x;
   a.y = g.y;
-  a.q1 = g.q;
-  a.scale1 = g.scale;
-  a.q2 = g.yq;
-  a.scale2 = g.yscale;
+  a.xq = g.q;
+  a.xscale = g.scale;
+  a.yq = g.yq;
+  a.yscale = g.yscale;
   a.rows = g.rows;
   a.cols = g.cols;
   return g.tanh_form ? launch<GeluForward<true>>(a, g.x.t, stream) : launch<GeluForward<false>>(a, g.x.t, stream);

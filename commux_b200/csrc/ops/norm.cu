@@ -12,90 +12,42 @@ namespace train {
 
 namespace {
 
-// Both passes hold a row in registers, 8 elements of it to a chunk and a few
-// chunks to a thread, so a row is read once; `group` threads (whole warps) share
-// it. Where the rows allow it a chunk is 8 neighbours (wide loads and stores),
-// else 8 elements `group` apart (a warp's lanes on 32 neighbours), so that any
-// length, stride and alignment keeps whole cache lines. A warp holds whole groups
-// of the 8-bit form in both.
+// Both passes hold a row in registers, so it is read once: `group` threads (whole
+// warps) share it, each with a few parts of 8 neighbours. Sums, products and the
+// 8-bit form work on pairs of elements: a third of the instructions of a first
+// version with one element at a time, which they bound.
 constexpr int kMaxGroup = 512;
 
 __host__ __device__ inline std::int64_t held_groups(std::int64_t cols) { return (cols + kGroup - 1) / kGroup; }
 
-template <typename T, bool kVec>
-struct Chunk {
-  Eight<T> w;
-  __device__ __forceinline__ void load(const T* row, int c, int, int cols) {
-    if (c < cols)
-      w.load(row + c);
-    else
-      w.zero();
-  }
-  __device__ __forceinline__ void get(float (&v)[8]) const { w.get(v); }
-  static __device__ __forceinline__ void store(T* row, int c, int, int cols, const float (&v)[8]) {
-    if (c >= cols) return;
-    Eight<T> o;
-    o.put(v);
-    o.store(row + c);
-  }
-};
-template <typename T>
-struct Chunk<T, false> {
-  T w[8];
-  __device__ __forceinline__ void load(const T* row, int c, int apart, int cols) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = c + i * apart < cols ? row[c + i * apart] : Elem<T>::put(0.0f);
-  }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::get(w[i]);
-  }
-  static __device__ __forceinline__ void store(T* row, int c, int apart, int cols, const float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i * apart < cols) row[c + i * apart] = Elem<T>::put(v[i]);
-  }
-};
-
-// A chunk of a tensor whose type is known at run time alone (the weights, the
+// A part of a tensor whose type is known at run time alone (the weights, the
 // residual: their branches are the same for the whole grid).
-template <bool kVec>
-__device__ __forceinline__ void load_any(const void* p, Type t, std::int64_t at, int c, int apart, int cols,
-                                         float (&v)[8]) {
+template <bool kAligned>
+__device__ __forceinline__ void load_any(const void* p, Type t, std::int64_t at, int c, int cols, float2 (&v)[4]) {
   if (t == Type::f32) {
-    Chunk<float, kVec> k;
-    k.load(static_cast<const float*>(p) + at, c, apart, cols);
+    Part<float, kAligned> k;
+    k.load(static_cast<const float*>(p) + at, c, cols);
     k.get(v);
   } else if (t == Type::bf16) {
-    Chunk<__nv_bfloat16, kVec> k;
-    k.load(static_cast<const __nv_bfloat16*>(p) + at, c, apart, cols);
+    Part<__nv_bfloat16, kAligned> k;
+    k.load(static_cast<const __nv_bfloat16*>(p) + at, c, cols);
     k.get(v);
   } else {
-    Chunk<__half, kVec> k;
-    k.load(static_cast<const __half*>(p) + at, c, apart, cols);
+    Part<__half, kAligned> k;
+    k.load(static_cast<const __half*>(p) + at, c, cols);
     k.get(v);
   }
 }
 
-template <bool kVec>
-__device__ __forceinline__ void store_any(void* p, Type t, std::int64_t at, int c, int apart, int cols,
-                                          const float (&v)[8]) {
+template <bool kAligned>
+__device__ __forceinline__ void store_any(void* p, Type t, std::int64_t at, int c, int cols, const float2 (&v)[4],
+                                          bool joined, bool last) {
   if (t == Type::f32)
-    Chunk<float, kVec>::store(static_cast<float*>(p) + at, c, apart, cols, v);
+    Part<float, kAligned>::store(static_cast<float*>(p) + at, c, cols, v, joined, last);
   else if (t == Type::bf16)
-    Chunk<__nv_bfloat16, kVec>::store(static_cast<__nv_bfloat16*>(p) + at, c, apart, cols, v);
+    Part<__nv_bfloat16, kAligned>::store(static_cast<__nv_bfloat16*>(p) + at, c, cols, v, joined, last);
   else
-    Chunk<__half, kVec>::store(static_cast<__half*>(p) + at, c, apart, cols, v);
-}
-
-// First element of this thread's chunk n, and whether element i is in the row.
-template <bool kVec>
-__device__ __forceinline__ int chunk_at(int n, int group, int t) {
-  return kVec ? (n * group + t) * 8 : n * 8 * group + t;
-}
-template <bool kVec>
-__device__ __forceinline__ bool in_row(int c, int i, int apart, int cols) {
-  return kVec ? c < cols : c + i * apart < cols;
+    Part<__half, kAligned>::store(static_cast<__half*>(p) + at, c, cols, v, joined, last);
 }
 
 __device__ __forceinline__ void sync_group(int id, int threads) {
@@ -105,109 +57,104 @@ __device__ __forceinline__ void sync_group(int id, int threads) {
 
 // Sums of two values over a row's threads, in a fixed order. `slots` (one for
 // each warp) may be used again after another sum with other slots.
-__device__ __forceinline__ float2 group_sum(float a, float b, int group, int id, float2* slots) {
-  a = warp_sum(a);
-  b = warp_sum(b);
-  if (group == 32) return {a, b};
-  const int lane = threadIdx.x & 31, warps = group >> 5;
-  if (lane == 0) slots[(threadIdx.x >> 5) % warps] = float2{a, b};
-  sync_group(id, group);
-  const float2 v = lane < warps ? slots[lane] : float2{0.0f, 0.0f};
-  return {warp_sum(v.x), warp_sum(v.y)};
-}
-
-// A chunk's 8-bit form at its place in the row.
-template <bool kVec>
-__device__ __forceinline__ void pack_chunk(const float (&h)[8], std::int8_t* q, std::uint8_t* scale, int c, int apart,
-                                           int padded) {
-  if (kVec) {
-    uint2 v;
-    const unsigned e = pack_eight(h, v);
-    if (c < padded) {
-      *reinterpret_cast<uint2*>(q + c) = v;
-      if ((threadIdx.x & 3) == 0) scale[c / kGroup] = static_cast<std::uint8_t>(e);
-    }
-  } else {
+__device__ __forceinline__ float2 group_sum(float2 v, int group, int id, float2* slots) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned e = warp_scale(h[i]);
-      const int at = c + i * apart;
-      if (at < padded) {
-        q[at] = static_cast<std::int8_t>(quantised(h[i], e));
-        if ((threadIdx.x & 31) == 0) scale[at / kGroup] = static_cast<std::uint8_t>(e);
-      }
-    }
-  }
+  for (int o = 16; o > 0; o >>= 1)
+    v = add2(v, float2{__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)});
+  if (group == 32) return v;
+  const int lane = threadIdx.x & 31, warps = group >> 5;
+  if (lane == 0) slots[(threadIdx.x >> 5) % warps] = v;
+  sync_group(id, group);
+  v = lane < warps ? slots[lane] : float2{0.0f, 0.0f};
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1)  // 16 warps at most
+    v = add2(v, float2{__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)});
+  return {__shfl_sync(0xffffffffu, v.x, 0), __shfl_sync(0xffffffffu, v.y, 0)};
 }
 
 // --- forward: one row to a group of threads, 256 threads or one row a block ---
 
-constexpr int kFwdChunks = 4;
+constexpr int kFwdParts = 4;
 
-template <typename X, typename Y, bool kVec>
+template <typename X, typename Y, bool kAligned>
 __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int group) {
   __shared__ float2 slots[2][32];
-  const int id = threadIdx.x / group, t = threadIdx.x - id * group;
+  const int id = threadIdx.x / group, t = threadIdx.x - id * group, lane = threadIdx.x & 31;
   const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * (blockDim.x / group) + id;
   if (row >= a.rows) return;  // a whole group
-  const int cols = static_cast<int>(a.cols), apart = group;
+  const int cols = static_cast<int>(a.cols);
   const std::int64_t out = row * a.cols;
   const X* x = static_cast<const X*>(a.x.p) + row * a.x.ld;
-  float v[kFwdChunks][8];
+  float2 v[kFwdParts][4];
   {
-    Chunk<X, kVec> k[kFwdChunks];
+    Part<X, kAligned> k[kFwdParts];
 #pragma unroll
-    for (int n = 0; n < kFwdChunks; ++n) k[n].load(x, chunk_at<kVec>(n, group, t), apart, cols);
+    for (int n = 0; n < kFwdParts; ++n) k[n].load(x, (n * group + t) * 8, cols);
 #pragma unroll
-    for (int n = 0; n < kFwdChunks; ++n) k[n].get(v[n]);
+    for (int n = 0; n < kFwdParts; ++n) k[n].get(v[n]);
   }
+  const bool joined = lane > 0, last = lane == 31;
   if (a.r.p != nullptr) {
 #pragma unroll
-    for (int n = 0; n < kFwdChunks; ++n) {
-      const int c = chunk_at<kVec>(n, group, t);
-      float r[8];
-      load_any<kVec>(a.r.p, a.r.t, row * a.r.ld, c, apart, cols, r);
+    for (int n = 0; n < kFwdParts; ++n) {
+      if (n * group * 8 >= cols) break;
+      const int c = (n * group + t) * 8;
+      float2 r[4];
+      load_any<kAligned>(a.r.p, a.r.t, row * a.r.ld, c, cols, r);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[n][i] = Elem<X>::get(Elem<X>::put(v[n][i] + r[i]));
-      Chunk<X, kVec>::store(static_cast<X*>(a.s) + out, c, apart, cols, v[n]);
+      for (int i = 0; i < 4; ++i) v[n][i] = Elem<X>::rounded2(add2(v[n][i], r[i]));
+      Part<X, kAligned>::store(static_cast<X*>(a.s) + out, c, cols, v[n], joined, last);
     }
   }
-  float sum = 0.0f, sq = 0.0f;
+  float2 sum = {0.0f, 0.0f}, sq = {0.0f, 0.0f};
 #pragma unroll
-  for (int n = 0; n < kFwdChunks; ++n)
+  for (int n = 0; n < kFwdParts; ++n)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += v[n][i];  // 0 past the row's end
+    for (int i = 0; i < 4; ++i) sum = add2(sum, v[n][i]);  // 0 past the row's end
   const float inv = 1.0f / static_cast<float>(cols);
-  const float mean = group_sum(sum, 0.0f, group, id, slots[0] + id * (group >> 5)).x * inv;
+  sum = group_sum(sum, group, id, slots[0] + id * (group >> 5));
+  const float mean = (sum.x + sum.y) * inv;
 #pragma unroll
-  for (int n = 0; n < kFwdChunks; ++n) {
-    const int c = chunk_at<kVec>(n, group, t);
+  for (int n = 0; n < kFwdParts; ++n) {
+    const int left = cols - (n * group + t) * 8;
+    if (left >= 8) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[n][i] = in_row<kVec>(c, i, apart, cols) ? v[n][i] - mean : 0.0f;
-      sq += v[n][i] * v[n][i];
+      for (int i = 0; i < 4; ++i) v[n][i] = add2(v[n][i], both(-mean));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[n][i] = float2{2 * i < left ? v[n][i].x - mean : 0.0f, 2 * i + 1 < left ? v[n][i].y - mean : 0.0f};
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sq = fma2(v[n][i], v[n][i], sq);
   }
-  const float rstd = rsqrtf(group_sum(sq, 0.0f, group, id, slots[1] + id * (group >> 5)).x * inv + a.eps);
+  sq = group_sum(sq, group, id, slots[1] + id * (group >> 5));
+  const float rstd = rsqrtf((sq.x + sq.y) * inv + a.eps);
   if (t == 0) {
     if (a.mean != nullptr) a.mean[row] = mean;
     if (a.rstd != nullptr) a.rstd[row] = rstd;
   }
-  const int padded = static_cast<int>(held_groups(a.cols)) * kGroup;
+  const int ng = static_cast<int>(held_groups(a.cols));
 #pragma unroll
-  for (int n = 0; n < kFwdChunks; ++n) {
-    const int c = chunk_at<kVec>(n, group, t);
-    if (n > 0 && chunk_at<kVec>(n, group, 0) >= cols) break;
+  for (int n = 0; n < kFwdParts; ++n) {
+    if (n * group * 8 >= cols) break;
+    const int c = (n * group + t) * 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[n][i] *= rstd;
-    if (a.q != nullptr)
-      pack_chunk<kVec>(v[n], a.q + row * padded, a.scale + row * (padded / kGroup), c, apart, padded);
-    float w[8], b[8] = {};
-    load_any<kVec>(a.w, a.wt, 0, c, apart, cols, w);
-    if (a.b != nullptr) load_any<kVec>(a.b, a.wt, 0, c, apart, cols, b);
+    for (int i = 0; i < 4; ++i) v[n][i] = mul2(v[n][i], both(rstd));
+    if (a.q != nullptr) {
+      uint2 q;
+      const unsigned e = pack_eight(v[n], q);
+      if (c < ng * kGroup) {
+        *reinterpret_cast<uint2*>(a.q + row * ng * kGroup + c) = q;
+        if ((threadIdx.x & 3) == 0) a.scale[row * ng + c / kGroup] = static_cast<std::uint8_t>(e);
+      }
+    }
+    float2 w[4], b[4] = {};
+    load_any<kAligned>(a.w, a.wt, 0, c, cols, w);
+    if (a.b != nullptr) load_any<kAligned>(a.b, a.wt, 0, c, cols, b);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[n][i] = v[n][i] * w[i] + b[i];
-    Chunk<Y, kVec>::store(static_cast<Y*>(a.y) + out, c, apart, cols, v[n]);
+    for (int i = 0; i < 4; ++i) v[n][i] = fma2(v[n][i], w[i], b[i]);
+    Part<Y, kAligned>::store(static_cast<Y*>(a.y) + out, c, cols, v[n], joined, last);
   }
 }
 
@@ -218,124 +165,100 @@ __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int
 // one partial sum of each column, and norm_join adds those. The next row is on
 // its way while one is worked on.
 
-template <typename X, typename Y, bool kVec, bool kHeld, int kChunks>
+template <typename X, typename Y, bool kAligned, bool kHeld, int kParts>
 struct BwdRow {
-  Chunk<Y, kVec> dy[kChunks];
-  Chunk<X, kVec> s[kHeld ? 1 : kChunks];
-  uint2 q[kHeld ? kChunks : 1];  // 8 held values
-  unsigned e[kHeld ? kChunks : 1][kVec ? 1 : 8];
+  Part<Y, kAligned> dy[kParts];
+  Part<X, kAligned> s[kHeld ? 1 : kParts];
+  uint2 q[kHeld ? kParts : 1];  // 8 held values
+  unsigned e[kHeld ? kParts : 1];
   float mean, rstd;
 
   __device__ __forceinline__ void load(const NormBwd& a, std::int64_t row, int group, int t) {
     const int cols = static_cast<int>(a.cols);
     const Y* from = static_cast<const Y*>(a.dy.p) + row * a.dy.ld;
 #pragma unroll
-    for (int n = 0; n < kChunks; ++n) dy[n].load(from, chunk_at<kVec>(n, group, t), group, cols);
+    for (int n = 0; n < kParts; ++n) dy[n].load(from, (n * group + t) * 8, cols);
     rstd = a.rstd[row];
     if constexpr (!kHeld) {
       mean = a.mean[row];
       const X* x = static_cast<const X*>(a.s.p) + row * a.s.ld;
 #pragma unroll
-      for (int n = 0; n < kChunks; ++n) s[n].load(x, chunk_at<kVec>(n, group, t), group, cols);
+      for (int n = 0; n < kParts; ++n) s[n].load(x, (n * group + t) * 8, cols);
     } else {
       const int ng = static_cast<int>(held_groups(a.cols));
-      const std::int8_t* held = a.q + row * ng * kGroup;
-      const std::uint8_t* scale = a.scale + row * ng;
 #pragma unroll
-      for (int n = 0; n < kChunks; ++n) {
-        const int c = chunk_at<kVec>(n, group, t);
+      for (int n = 0; n < kParts; ++n) {
+        const int c = (n * group + t) * 8;
         q[n] = uint2{0, 0};
-        if constexpr (kVec) {
-          e[n][0] = 1;
-          if (c < cols) {
-            q[n] = *reinterpret_cast<const uint2*>(held + c);
-            e[n][0] = scale[c / kGroup];
-          }
-        } else {
-          unsigned b[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int at = c + i * group;
-            b[i] = 0;
-            e[n][i] = 1;
-            if (at < cols) {
-              b[i] = static_cast<std::uint8_t>(held[at]);
-              e[n][i] = scale[at / kGroup];
-            }
-          }
-          q[n] = uint2{low_bytes(b[0], b[1], b[2], b[3]), low_bytes(b[4], b[5], b[6], b[7])};
+        e[n] = 1;
+        if (c < cols) {
+          q[n] = *reinterpret_cast<const uint2*>(a.q + row * ng * kGroup + c);
+          e[n] = a.scale[row * ng + c / kGroup];
         }
       }
     }
   }
 
-  __device__ __forceinline__ void normalised(const NormBwd& a, int n, int c, int group, float (&h)[8]) const {
-    if constexpr (!kHeld) {
+  // past the row's end 0 (packed) or -mean * rstd, which meets a dy of 0
+  __device__ __forceinline__ void normalised(int n, float2 (&h)[4]) const {
+    if constexpr (kHeld) {
+      unpack_eight(q[n], e[n], h);
+    } else {
       s[n].get(h);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        h[i] = in_row<kVec>(c, i, group, static_cast<int>(a.cols)) ? (h[i] - mean) * rstd : 0.0f;
-    } else if constexpr (kVec) {
-      unpack_eight(q[n], e[n][0], h);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        h[i] = static_cast<float>(static_cast<std::int8_t>((i < 4 ? q[n].x : q[n].y) >> (8 * (i & 3)))) *
-               step_of(e[n][i]);
+      for (int i = 0; i < 4; ++i) h[i] = mul2(add2(h[i], both(-mean)), both(rstd));
     }
   }
 };
 
-template <typename X, typename Y, bool kVec, bool kHeld, int kChunks>
+template <typename X, typename Y, bool kAligned, bool kHeld, int kParts>
 __global__ void __launch_bounds__(kMaxGroup) norm_bwd(const NormBwd a, const int group, float* part) {
   extern __shared__ float sums[];  // [2][cols], where a block has more than one group
   __shared__ float2 slots[2][32];
-  const int id = threadIdx.x / group, t = threadIdx.x - id * group, ids = blockDim.x / group;
+  const int id = threadIdx.x / group, t = threadIdx.x - id * group, ids = blockDim.x / group, lane = threadIdx.x & 31;
   const int cols = static_cast<int>(a.cols);
   const float inv = 1.0f / static_cast<float>(cols);
-  float dw[kChunks][8] = {}, db[kChunks][8] = {}, w[kChunks][8];
+  float2 dw[kParts][4] = {}, db[kParts][4] = {}, w[kParts][4];
 #pragma unroll
-  for (int n = 0; n < kChunks; ++n) load_any<kVec>(a.w, a.wt, 0, chunk_at<kVec>(n, group, t), group, cols, w[n]);
+  for (int n = 0; n < kParts; ++n) load_any<kAligned>(a.w, a.wt, 0, (n * group + t) * 8, cols, w[n]);
   const std::int64_t stride = static_cast<std::int64_t>(gridDim.x) * ids;
   std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * ids + id;
-  BwdRow<X, Y, kVec, kHeld, kChunks> next;
+  BwdRow<X, Y, kAligned, kHeld, kParts> next;
   if (row < a.rows) next.load(a, row, group, t);
   for (unsigned turn = 0; row < a.rows; row += stride, turn ^= 1u) {
-    const BwdRow<X, Y, kVec, kHeld, kChunks> now = next;
+    const BwdRow<X, Y, kAligned, kHeld, kParts> now = next;
     if (row + stride < a.rows) next.load(a, row + stride, group, t);
-    float g[kChunks][8], h[kChunks][8], c1 = 0.0f, c2 = 0.0f;
+    float2 g[kParts][4], h[kParts][4], c1 = {0.0f, 0.0f}, c2 = {0.0f, 0.0f};
 #pragma unroll
-    for (int n = 0; n < kChunks; ++n) {
-      const int c = chunk_at<kVec>(n, group, t);
-      now.normalised(a, n, c, group, h[n]);
+    for (int n = 0; n < kParts; ++n) {
+      now.normalised(n, h[n]);
       now.dy[n].get(g[n]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dw[n][i] += g[n][i] * h[n][i];
-        db[n][i] += g[n][i];
-        g[n][i] *= w[n][i];  // 0 past the row's end, and so is h
-        c1 += g[n][i];
-        c2 += g[n][i] * h[n][i];
+      for (int i = 0; i < 4; ++i) {
+        dw[n][i] = fma2(g[n][i], h[n][i], dw[n][i]);
+        db[n][i] = add2(db[n][i], g[n][i]);
+        g[n][i] = mul2(g[n][i], w[n][i]);  // 0 past the row's end
+        c1 = add2(c1, g[n][i]);
+        c2 = fma2(g[n][i], h[n][i], c2);
       }
     }
-    const float2 c = group_sum(c1, c2, group, id, slots[turn] + id * (group >> 5));
-    c1 = c.x * inv;
-    c2 = c.y * inv;
+    const float2 c = group_sum(float2{c1.x + c1.y, c2.x + c2.y}, group, id, slots[turn] + id * (group >> 5));
+    const float2 k0 = both(-c.x * inv), k1 = both(-c.y * inv), r = both(now.rstd);
 #pragma unroll
-    for (int n = 0; n < kChunks; ++n) {
-      const int at = chunk_at<kVec>(n, group, t);
+    for (int n = 0; n < kParts; ++n) {
+      const int at = (n * group + t) * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[n][i] = now.rstd * (g[n][i] - c1 - h[n][i] * c2);
+      for (int i = 0; i < 4; ++i) g[n][i] = mul2(fma2(h[n][i], k1, add2(g[n][i], k0)), r);
       if (a.ds.p != nullptr) {
-        Chunk<X, kVec> k;
-        float ds[8];
-        k.load(static_cast<const X*>(a.ds.p) + row * a.ds.ld, at, group, cols);
+        Part<X, kAligned> k;
+        float2 ds[4];
+        k.load(static_cast<const X*>(a.ds.p) + row * a.ds.ld, at, cols);
         k.get(ds);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[n][i] += ds[i];
+        for (int i = 0; i < 4; ++i) g[n][i] = add2(g[n][i], ds[i]);
       }
-      Chunk<X, kVec>::store(static_cast<X*>(a.dx) + row * a.cols, at, group, cols, g[n]);
-      if (a.dr != nullptr) store_any<kVec>(a.dr, a.rt, row * a.cols, at, group, cols, g[n]);
+      Part<X, kAligned>::store(static_cast<X*>(a.dx) + row * a.cols, at, cols, g[n], lane > 0, lane == 31);
+      if (a.dr != nullptr) store_any<kAligned>(a.dr, a.rt, row * a.cols, at, cols, g[n], lane > 0, lane == 31);
     }
   }
   if (part == nullptr) return;
@@ -343,15 +266,14 @@ __global__ void __launch_bounds__(kMaxGroup) norm_bwd(const NormBwd a, const int
   for (int k = 0; k < ids; ++k) {  // group after group
     if (id == k) {
 #pragma unroll
-      for (int n = 0; n < kChunks; ++n) {
-        const int c = chunk_at<kVec>(n, group, t);
+      for (int n = 0; n < kParts; ++n) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int at = kVec ? c + i : c + i * group;
+          const int at = (n * group + t) * 8 + i;
           if (at >= cols) continue;
-          const float w = (k > 0 ? sums[at] : 0.0f) + dw[n][i], b = (k > 0 ? sums[cols + at] : 0.0f) + db[n][i];
-          (k + 1 < ids ? sums : to)[at] = w;
-          (k + 1 < ids ? sums : to)[cols + at] = b;
+          const float dwi = i & 1 ? dw[n][i / 2].y : dw[n][i / 2].x, dbi = i & 1 ? db[n][i / 2].y : db[n][i / 2].x;
+          (k + 1 < ids ? sums : to)[at] = (k > 0 ? sums[at] : 0.0f) + dwi;
+          (k + 1 < ids ? sums : to)[cols + at] = (k > 0 ? sums[cols + at] : 0.0f) + dbi;
         }
       }
     }
@@ -500,32 +422,32 @@ void with_pair(Type x, Type y, F f) {
 
 // How the backward pass is laid out.
 struct BwdPlan {
-  bool vec;
-  int chunks, group, ids, blocks;  // chunks 0: sweeps, with `blocks` row shares
+  bool aligned;
+  int parts, group, ids, blocks;  // parts 0: sweeps, with `blocks` row shares
 };
 
-bool by_chunks(const Rows& r, std::int64_t cols) { return r.p == nullptr || by_eight(r.p, r.ld, cols); }
+bool aligned(const void* p, std::int64_t ld, std::int64_t cols) { return p == nullptr || aligned_rows(p, ld, cols); }
 
-// Threads of a group that hold `cols` in up to `chunks` chunks each.
-int group_of(std::int64_t cols, int chunks) {
-  return static_cast<int>((cols + 8 * chunks * 32 - 1) / (8 * chunks * 32)) * 32;
+// Threads of a group that hold `cols` in up to `parts` parts each.
+int group_of(std::int64_t cols, int parts) {
+  return static_cast<int>((cols + 8 * parts * 32 - 1) / (8 * parts * 32)) * 32;
 }
 
 BwdPlan plan_of(const NormBwd& a) {
   BwdPlan p{};
-  p.vec = by_chunks(a.dy, a.cols) && by_chunks(a.ds, a.cols) && by_chunks(a.s, a.cols) &&
-          by_eight(a.w, a.cols, a.cols);
-  // One chunk a thread keeps the registers (two sums and two values for each
-  // element) near 80 and the loads of many rows in flight; long rows take more.
-  p.chunks = a.cols <= 8 * kMaxGroup ? 1 : a.cols <= 16 * kMaxGroup ? 2 : 0;
-  if (!paired(a.xt, a.dy.t)) p.chunks = 0;
+  p.aligned = aligned(a.dy.p, a.dy.ld, a.cols) && aligned(a.ds.p, a.ds.ld, a.cols) && aligned(a.s.p, a.s.ld, a.cols) &&
+              aligned(a.w, a.cols, a.cols);
+  // One part a thread keeps the registers (two sums and two values for each
+  // element) near 80 and the loads of many rows in flight; long rows take two.
+  p.parts = a.cols <= 8 * kMaxGroup ? 1 : a.cols <= 16 * kMaxGroup ? 2 : 0;
+  if (!paired(a.xt, a.dy.t)) p.parts = 0;
   const int sms = sm_count();
-  if (p.chunks == 0) {
+  if (p.parts == 0) {
     const std::int64_t blocks = (a.cols + 31) / 32, want = (8ll * sms + blocks - 1) / blocks, most = (a.rows + 63) / 64;
     p.blocks = static_cast<int>(want < most ? want : most);
     return p;
   }
-  p.group = group_of(a.cols, p.chunks);
+  p.group = group_of(a.cols, p.parts);
   p.ids = p.group < 384 ? 384 / p.group : 1;
   // two blocks an SM, or fewer where a group would have under four rows
   const std::int64_t want = (a.rows + 4ll * p.ids - 1) / (4ll * p.ids);
@@ -533,31 +455,31 @@ BwdPlan plan_of(const NormBwd& a) {
   return p;
 }
 
-template <typename X, typename Y, bool kVec, bool kHeld>
+template <typename X, typename Y, bool kAligned, bool kHeld>
 void launch_bwd(const NormBwd& a, const BwdPlan& p, float* part, cudaStream_t stream) {
   const int threads = p.group * p.ids;
   const std::size_t smem = p.ids > 1 ? 2 * sizeof(float) * a.cols : 0;
-  if (p.chunks == 1)
-    norm_bwd<X, Y, kVec, kHeld, 1><<<p.blocks, threads, smem, stream>>>(a, p.group, part);
+  if (p.parts == 1)
+    norm_bwd<X, Y, kAligned, kHeld, 1><<<p.blocks, threads, smem, stream>>>(a, p.group, part);
   else
-    norm_bwd<X, Y, kVec, kHeld, 2><<<p.blocks, threads, smem, stream>>>(a, p.group, part);
+    norm_bwd<X, Y, kAligned, kHeld, 2><<<p.blocks, threads, smem, stream>>>(a, p.group, part);
 }
 
 }  // namespace
 
 cudaError_t norm_forward(const NormFwd& a, cudaStream_t stream) {
-  if (a.cols > 8 * kFwdChunks * kMaxGroup || !paired(a.x.t, a.yt)) {
+  if (a.cols > 8 * kFwdParts * kMaxGroup || !paired(a.x.t, a.yt)) {
     const std::int64_t most = 32ll * sm_count();
     norm_fwd_sweep<<<static_cast<unsigned>(a.rows < most ? a.rows : most), kSweep, 0, stream>>>(a);
   } else {
-    const bool vec = by_chunks(a.x, a.cols) && by_chunks(a.r, a.cols) && by_eight(a.w, a.cols, a.cols) &&
-                     by_chunks(Rows{a.b, a.cols, a.wt}, a.cols);
-    const int group = group_of(a.cols, kFwdChunks), ids = group < 256 ? 256 / group : 1;
+    const bool all = aligned(a.x.p, a.x.ld, a.cols) && aligned(a.r.p, a.r.ld, a.cols) &&
+                     aligned(a.w, a.cols, a.cols) && aligned(a.b, a.cols, a.cols);
+    const int group = group_of(a.cols, kFwdParts), ids = group < 256 ? 256 / group : 1;
     const unsigned blocks = static_cast<unsigned>((a.rows + ids - 1) / ids);
     with_pair(a.x.t, a.yt, [&](auto x, auto y) {
       using X = decltype(x);
       using Y = decltype(y);
-      if (vec)
+      if (all)
         norm_fwd<X, Y, true><<<blocks, group * ids, 0, stream>>>(a, group);
       else
         norm_fwd<X, Y, false><<<blocks, group * ids, 0, stream>>>(a, group);
@@ -572,7 +494,7 @@ std::int64_t norm_backward_work(const NormBwd& a) { return 2ll * plan_of(a).bloc
 cudaError_t norm_backward(const NormBwd& a, cudaStream_t stream) {
   const BwdPlan p = plan_of(a);
   const bool columns = a.dw != nullptr || a.db != nullptr;
-  if (p.chunks == 0) {
+  if (p.parts == 0) {
     const std::int64_t most = 32ll * sm_count();
     norm_bwd_sweep<<<static_cast<unsigned>(a.rows < most ? a.rows : most), kSweep, 0, stream>>>(a);
     commux_ops::g_launches++;
@@ -586,9 +508,9 @@ cudaError_t norm_backward(const NormBwd& a, cudaStream_t stream) {
       using X = decltype(x);
       using Y = decltype(y);
       float* part = columns ? a.work : nullptr;
-      if (p.vec && a.q != nullptr)
+      if (p.aligned && a.q != nullptr)
         launch_bwd<X, Y, true, true>(a, p, part, stream);
-      else if (p.vec)
+      else if (p.aligned)
         launch_bwd<X, Y, true, false>(a, p, part, stream);
       else if (a.q != nullptr)
         launch_bwd<X, Y, false, true>(a, p, part, stream);

@@ -416,27 +416,65 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Tiles whose steps several CTAs shared: their parts in the order of the steps.
+// A block takes kJoinRows rows of a tile, a thread four neighbours of a few rows.
 constexpr int kJoinRows = 16;
-__global__ void __launch_bounds__(kN) wgrad_join(const Plan p, const Out out) {
-  const int tile = blockIdx.x;
-  const std::int64_t lo = static_cast<std::int64_t>(tile) * p.steps, hi = lo + p.steps;
-  const std::int64_t total = static_cast<std::int64_t>(p.tiles) * p.steps;
-  int first = static_cast<int>(lo * p.ctas / total);
-  while (p.begin(first + 1) <= lo) ++first;  // the quotient rounds down twice
-  if (p.begin(first) <= lo && p.begin(first + 1) >= hi) return;
-  const std::int64_t m0 = static_cast<std::int64_t>(tile / p.tiles_n) * kM, n0 = tile % p.tiles_n * kN;
-  const std::int64_t i = n0 + threadIdx.x;
-  const bool columns = out.b != nullptr || (out.db != nullptr && n0 == 0);
-  for (int r = blockIdx.y * kJoinRows; r < (blockIdx.y + 1) * kJoinRows; ++r) {
-    if (m0 + r >= p.outs) break;
-    float v = 0.0f, db = 0.0f;
-    for (int c = first; c < p.ctas && p.begin(c) < hi; ++c) {
-      const float* slot = out.slots + (2 * static_cast<std::int64_t>(c) + (p.begin(c) >= lo ? 0 : 1)) * kSlot;
-      if (i < p.cols) v += slot[r * kN + threadIdx.x];
-      if (columns) db += slot[kM * kN + r];
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) wgrad_join(const Plan p, const Out out) {
+  __shared__ int parts, first_slot;
+  __shared__ float column[kJoinRows];
+  const int tile = blockIdx.x, m0 = tile / p.tiles_n * kM, n0 = tile % p.tiles_n * kN, r0 = blockIdx.y * kJoinRows;
+  if (m0 + r0 >= p.outs) return;
+  if (threadIdx.x == 0) {
+    const std::int64_t lo = static_cast<std::int64_t>(tile) * p.steps, hi = lo + p.steps;
+    int c = static_cast<int>(lo * p.ctas / (static_cast<std::int64_t>(p.tiles) * p.steps));
+    while (p.begin(c + 1) <= lo) ++c;  // the quotient rounds down twice
+    // the first part is a CTA's last one unless the CTA begins with it; every
+    // later part is its CTA's first
+    first_slot = 2 * c + (p.begin(c) >= lo ? 0 : 1);
+    int n = 1;
+    while (p.begin(c + n) < hi && c + n < p.ctas) ++n;
+    parts = n;
+  }
+  __syncthreads();
+  const int n = parts, s0 = first_slot;
+  if (n == 1) return;
+  auto slot = [&](int k) { return out.slots + static_cast<std::int64_t>(k == 0 ? s0 : (s0 / 2 + k) * 2) * kSlot; };
+  if (out.b != nullptr || (out.db != nullptr && n0 == 0)) {
+    if (threadIdx.x < kJoinRows) {
+      const int r = r0 + threadIdx.x;
+      float db = 0.0f;
+      for (int k = 0; k < n; ++k) db += slot(k)[kM * kN + r];
+      column[threadIdx.x] = db;
+      if (n0 == 0 && out.db != nullptr && m0 + r < p.outs) store(out.db, out.dwt, m0 + r, db);
     }
-    if (i < p.cols) write_dw(p, out, m0 + r, i, v, db);
-    if (n0 == 0 && out.db != nullptr && threadIdx.x == 0) store(out.db, out.dwt, m0 + r, db);
+    __syncthreads();
+  }
+  constexpr int kPass = kJoinThreads * 4 / kN;  // rows that the block reads at once
+  const int col = threadIdx.x % (kN / 4) * 4, row = r0 + threadIdx.x / (kN / 4);
+  float4 v[kJoinRows / kPass] = {};
+#pragma unroll 2
+  for (int k = 0; k < n; ++k) {
+    const float* from = slot(k) + row * kN + col;
+#pragma unroll
+    for (int j = 0; j < kJoinRows / kPass; ++j) {
+      const float4 w = *reinterpret_cast<const float4*>(from + j * kPass * kN);
+      v[j].x += w.x, v[j].y += w.y, v[j].z += w.z, v[j].w += w.w;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kJoinRows / kPass; ++j) {
+    const int r = row + j * kPass;
+    const std::int64_t o = m0 + r, i = n0 + col;
+    if (o >= p.outs || i >= p.cols) continue;
+    const float db = out.b != nullptr ? column[r - r0] : 0.0f;
+    if (out.dwt == Type::f32 && out.w == nullptr && p.cols % 4 == 0) {
+      *reinterpret_cast<float4*>(static_cast<float*>(out.dw) + o * p.cols + i) = v[j];
+      continue;
+    }
+    write_dw(p, out, o, i, v[j].x, db);
+    if (i + 1 < p.cols) write_dw(p, out, o, i + 1, v[j].y, db);
+    if (i + 2 < p.cols) write_dw(p, out, o, i + 2, v[j].z, db);
+    if (i + 3 < p.cols) write_dw(p, out, o, i + 3, v[j].w, db);
   }
 }
 
@@ -494,11 +532,13 @@ Plan plan_of(const Wgrad8& a) {
   p.steps = static_cast<int>((a.rows + kK - 1) / kK);
   // One CTA an SM. Where whole shares of the tiles fill nearly all of them,
   // every CTA has one part of one tile; otherwise parts may cross tiles. No
-  // CTA takes under 4 steps, which cost about what its start and end do.
+  // tile is cut into parts under 4 steps, which cost about what a CTA's start
+  // and end do.
   const int sms = sm_count();
   const std::int64_t total = static_cast<std::int64_t>(p.tiles) * p.steps;
   std::int64_t n = p.tiles <= sms && sms / p.tiles * p.tiles * 10 >= sms * 9 ? sms / p.tiles * p.tiles : sms;
-  if (n > (total + 3) / 4) n = (total + 3) / 4;
+  const std::int64_t most = (total + 3) / 4 > p.tiles ? (total + 3) / 4 : p.tiles;
+  if (n > most) n = most;
   p.ctas = static_cast<int>(n);
   return p;
 }
@@ -554,7 +594,7 @@ cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
   bool joined = false;
   for (int c = 1; c < p.ctas && !joined; ++c) joined = p.begin(c) % p.steps != 0;
   if (joined) {
-    wgrad_join<<<dim3(p.tiles, kM / kJoinRows), kN, 0, stream>>>(p, out);
+    wgrad_join<<<dim3(p.tiles, kM / kJoinRows), kJoinThreads, 0, stream>>>(p, out);
     commux_ops::g_launches++;
   }
   return cudaGetLastError();

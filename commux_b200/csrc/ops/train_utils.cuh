@@ -33,28 +33,10 @@ __device__ __forceinline__ float rounded(float v, Type t) {
 }
 
 // Two fp32 operations in one instruction.
-__device__ __forceinline__ unsigned long long bits2(float2 v) {
-  return static_cast<unsigned long long>(__float_as_uint(v.y)) << 32 | __float_as_uint(v.x);
-}
-__device__ __forceinline__ float2 float2_of(unsigned long long w) {
-  return {__uint_as_float(static_cast<unsigned>(w)), __uint_as_float(static_cast<unsigned>(w >> 32))};
-}
 __device__ __forceinline__ float2 both(float v) { return {v, v}; }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
-  return float2_of(d);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  unsigned long long d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
-  return float2_of(d);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
-  return float2_of(d);
-}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 
 // 2^x and 1/x to about two units of the last place; results (and arguments)
 // under 2^-126 become 0.

@@ -60,21 +60,15 @@ __device__ __forceinline__ void write_dw(const Plan& p, const Out& out, std::int
   store(out.dw, out.dwt, o * p.cols + i, v);
 }
 
-__device__ __forceinline__ unsigned long long pair(unsigned lo, unsigned hi) {
-  return static_cast<unsigned long long>(hi) << 32 | lo;
-}
-
 // Two neighbouring bytes (of u = q + 128) times the step, as two bf16. A byte
 // in the low bits of 2^23's mantissa is 2^23 + u; less 2^23 + 128 that is q,
 // and q s has its low 16 bits clear, so its upper half is the bf16.
-__device__ __forceinline__ unsigned widen2(unsigned word, int at, unsigned long long step) {
+__device__ __forceinline__ unsigned widen2(unsigned word, int at, float2 step) {
   const unsigned sel = 0x7540u + static_cast<unsigned>(at);
-  const unsigned lo = __byte_perm(word, 0x4b000000u, sel), hi = __byte_perm(word, 0x4b000000u, sel + 1);
-  unsigned long long v = pair(lo, hi);
-  const unsigned long long base = pair(0xcb000080u, 0xcb000080u);  // -(2^23 + 128)
-  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(base));
-  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(step));
-  return __byte_perm(static_cast<unsigned>(v), static_cast<unsigned>(v >> 32), 0x7632);
+  const float2 u = {__uint_as_float(__byte_perm(word, 0x4b000000u, sel)),
+                    __uint_as_float(__byte_perm(word, 0x4b000000u, sel + 1))};
+  const float2 v = mul2(add2(u, both(-8388736.0f)), step);
+  return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
 }
 
 // Both operands have their M or N elements adjacent: blocks of 64 elements
@@ -297,8 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int r = j * 16 + row0;
             uint4 v = *reinterpret_cast<const uint4*>(from + r * kN + unit * 16);
             v.x ^= 0x80808080u, v.y ^= 0x80808080u, v.z ^= 0x80808080u, v.w ^= 0x80808080u;
-            const unsigned sbits = __float_as_uint(step_of(e[j]));
-            const unsigned long long step = pair(sbits, sbits);
+            const float2 step = both(step_of(e[j]));
             const uint4 lo = {widen2(v.x, 0, step), widen2(v.x, 2, step), widen2(v.y, 0, step), widen2(v.y, 2, step)};
             const uint4 hi = {widen2(v.z, 0, step), widen2(v.z, 2, step), widen2(v.w, 0, step), widen2(v.w, 2, step)};
             // odd blocks write their halves the other way round: the 8 lanes of

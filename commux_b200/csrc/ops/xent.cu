@@ -246,10 +246,23 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned b
       : "memory");
 }
 
+// Leaves v in the shared memory of block `rank` of the cluster, at its copy of
+// `to`, and counts its 4 bytes on that block's copy of `bar`. Unlike a cluster
+// barrier it does not wait for this thread's stores of gradients to arrive
+// (which cost 8 us a row).
+__device__ __forceinline__ void send(float* to, std::uint64_t* bar, int rank, float v) {
+  std::uint32_t at, there;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(async::smem_u32(to)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(async::smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(at),
+               "r"(__float_as_uint(v)), "r"(there)
+               : "memory");
+}
+
 template <typename T, int kC>
 __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* status, std::uint64_t limit_ns) {
   extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ std::uint64_t full[kRing];
+  __shared__ std::uint64_t full[kRing], joined[2][2];
   __shared__ float slots[2][32], ranks[2][2][8];
   __shared__ int gave_up;
   constexpr int E = Row<T>::E, kV = Row<T>::kVectors;
@@ -264,6 +277,8 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
   const int cols = static_cast<int>(a.cols - first < share ? (a.cols > first ? a.cols - first : 0) : share);
   if (t == 0) {
     for (int i = 0; i < kRing; ++i) async::mbar_init(&full[i], 1);
+    if constexpr (kC > 1)
+      for (int i = 0; i < 4; ++i) async::mbar_init(&joined[i >> 1][i & 1], 1);
     gave_up = 0;
     async::fence_async();
   }
@@ -298,8 +313,18 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
   };
   if (t == 0) request();
   const float f = 1.0f / (a.reduction == 1 ? a.work[0] : 1.0f);
-  unsigned turn = 0;
-  for (std::int64_t row = mine; row < a.rows; row += clusters, turn ^= 1u) {
+  // A value of each of the cluster's blocks to all of them. Slots and barriers
+  // come in two sets: a block that is a row ahead writes to the other one, and
+  // it cannot be two ahead.
+  unsigned round = 0;
+  auto exchange = [&](int which, float v) {
+    const unsigned set = round & 1u;
+    if (t == 0) async::mbar_expect_tx(&joined[set][which], kC * 4);
+    if (t < kC) send(&ranks[set][which][rank], &joined[set][which], t, v);
+    async::bounded_wait(&joined[set][which], round >> 1 & 1u, bound);
+    return ranks[set][which][lane & (kC - 1)];
+  };
+  for (std::int64_t row = mine; row < a.rows; row += clusters, ++round) {
     const int n = pieces(row), shift = shift_of(part(row), sizeof(T));
     const std::int64_t target = a.target[row];
     const float logit = t == 0 && rank == 0 ? target_logit(a, row, target) : 0.0f;  // on its way early
@@ -325,21 +350,14 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
       request();
     }
     m = warp_max(slots[0][lane]);
-    if constexpr (kC > 1) {
-      cg::cluster_group cluster = cg::this_cluster();
-      if (t < kC) *cluster.map_shared_rank(&ranks[turn][0][rank], t) = m;
-      cluster.sync();
-      m = warp_max(lane < kC ? ranks[turn][0][lane] : -INFINITY);
-    }
+    if constexpr (kC > 1) m = warp_max(exchange(0, m));
     float s = warp_sum(r.exponentials(m));
     if (lane == 0) slots[1][t >> 5] = s;
     __syncthreads();
     s = warp_sum(slots[1][lane]);
     if constexpr (kC > 1) {
-      cg::cluster_group cluster = cg::this_cluster();
-      if (t < kC) *cluster.map_shared_rank(&ranks[turn][1][rank], t) = s;
-      cluster.sync();
-      s = warp_sum(lane < kC ? ranks[turn][1][lane] : 0.0f);
+      const float part = exchange(1, s);
+      s = warp_sum(lane < kC ? part : 0.0f);
     }
     if (t == 0 && rank == 0) finish_row(a, row, target, logit, m, s);
     if (a.dx != nullptr) {
@@ -347,9 +365,10 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
       write_row_part<T>(a, r, row, first, cols, shift, aligned, kLong, t, target, f, 1.0f / s);
     }
   }
-  // shared memory outlives the copies also where a wait gave up
+  // shared memory outlives the copies, and what other blocks send, also where a wait gave up
   if (t == 0 && gave_up != 0)
     for (unsigned n = used; n < issued; ++n) async::mbar_wait(&full[n % kRing], n / kRing & 1u, limit_ns);
+  if constexpr (kC > 1) cg::this_cluster().sync();
 }
 
 // --- rows longer than a cluster's registers, and gradients formed again ---

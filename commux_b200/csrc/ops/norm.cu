@@ -6,6 +6,8 @@
 // not a difference of moments, so a large mean costs no accuracy.
 // HBM-bound: about 10 operations an element.
 
+#include <type_traits>
+
 #include "train_utils.cuh"
 
 namespace train {
@@ -13,177 +15,206 @@ namespace train {
 namespace {
 
 // Both passes hold a row in registers, so it is read once: `group` threads (whole
-// warps) share it, each with a few parts of 8 neighbours. Sums, products and the
-// 8-bit form work on pairs of elements: a third of the instructions of a first
-// version with one element at a time, which they bound.
+// warps) share it, each with one or two parts of 8 neighbours, and groups walk
+// over rows. A thread keeps its columns from row to row, so the weights, and the
+// backward pass's sums of dw and db, stay in registers, and the next row is on its
+// way while one is worked on. Arithmetic is on pairs of elements. What bounds
+// both is half the memory and half the instructions: converting 16-bit values,
+// the group's reductions and the 8-bit form cost as many as the norm itself.
 constexpr int kMaxGroup = 512;
+constexpr int kBlock = 256;  // threads of a block of several groups, about
 
 __host__ __device__ inline std::int64_t held_groups(std::int64_t cols) { return (cols + kGroup - 1) / kGroup; }
 
-// A part of a tensor whose type is known at run time alone (the weights, the
-// residual: their branches are the same for the whole grid).
+// A part of a vector over the columns, of a type known at run time.
 template <bool kAligned>
-__device__ __forceinline__ void load_any(const void* p, Type t, std::int64_t at, int c, int cols, float2 (&v)[4]) {
+__device__ __forceinline__ void load_any(const void* p, Type t, int c, int cols, float2 (&v)[4]) {
   if (t == Type::f32) {
     Part<float, kAligned> k;
-    k.load(static_cast<const float*>(p) + at, c, cols);
+    k.load(static_cast<const float*>(p), c, cols);
     k.get(v);
   } else if (t == Type::bf16) {
     Part<__nv_bfloat16, kAligned> k;
-    k.load(static_cast<const __nv_bfloat16*>(p) + at, c, cols);
+    k.load(static_cast<const __nv_bfloat16*>(p), c, cols);
     k.get(v);
   } else {
     Part<__half, kAligned> k;
-    k.load(static_cast<const __half*>(p) + at, c, cols);
+    k.load(static_cast<const __half*>(p), c, cols);
     k.get(v);
   }
 }
 
-template <bool kAligned>
-__device__ __forceinline__ void store_any(void* p, Type t, std::int64_t at, int c, int cols, const float2 (&v)[4],
-                                          bool joined, bool last) {
-  if (t == Type::f32)
-    Part<float, kAligned>::store(static_cast<float*>(p) + at, c, cols, v, joined, last);
-  else if (t == Type::bf16)
-    Part<__nv_bfloat16, kAligned>::store(static_cast<__nv_bfloat16*>(p) + at, c, cols, v, joined, last);
-  else
-    Part<__half, kAligned>::store(static_cast<__half*>(p) + at, c, cols, v, joined, last);
-}
-
 __device__ __forceinline__ void sync_group(int id, int threads) {
-  if (threads > 32)
-    asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
 }
 
-// Sums of two values over a row's threads, in a fixed order. `slots` (one for
-// each warp) may be used again after another sum with other slots.
-__device__ __forceinline__ float2 group_sum(float2 v, int group, int id, float2* slots) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    v = add2(v, float2{__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)});
+// The sum of a value over a row's threads, in a fixed order, to all of them.
+// `slots` (one for each of the group's warps) may be used again after another
+// sum with other slots.
+__device__ __forceinline__ float group_sum(float v, int group, int id, float* slots) {
+  v = warp_sum(v);
   if (group == 32) return v;
   const int lane = threadIdx.x & 31, warps = group >> 5;
-  if (lane == 0) slots[(threadIdx.x >> 5) % warps] = v;
+  if (lane == 0) slots[(threadIdx.x >> 5) - id * warps] = v;
   sync_group(id, group);
-  v = lane < warps ? slots[lane] : float2{0.0f, 0.0f};
+  v = lane < warps ? slots[lane] : 0.0f;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1)  // 16 warps at most
-    v = add2(v, float2{__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)});
-  return {__shfl_sync(0xffffffffu, v.x, 0), __shfl_sync(0xffffffffu, v.y, 0)};
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);  // 16 warps at most
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// --- forward: one row to a group of threads, 256 threads or one row a block ---
+// The same of two values at the price of little more than one: after a first
+// exchange the lower half of a warp sums one of them and the upper half the other.
+__device__ __forceinline__ float2 group_sum2(float2 v, int group, int id, float* slots /* 32 */) {
+  const int lane = threadIdx.x & 31, warps = group >> 5;
+  const bool upper = lane >= 16;
+  float mine = upper ? v.y : v.x;
+  mine += __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (group > 32) {
+    if ((lane & 15) == 0) slots[lane + (threadIdx.x >> 5) - id * warps] = mine;
+    sync_group(id, group);
+    mine = (lane & 15) < warps ? slots[lane] : 0.0f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  }
+  return {__shfl_sync(0xffffffffu, mine, 0), __shfl_sync(0xffffffffu, mine, 16)};
+}
 
-constexpr int kFwdParts = 4;
+struct None {};
 
-template <typename X, typename Y, bool kAligned>
+// The tensors of a row as they are loaded. S: the residual's type, or None.
+template <typename X, typename S, bool kAligned, int kParts>
+struct FwdRow {
+  Part<X, kAligned> x[kParts];
+  Part<S, kAligned> r[kParts];
+  __device__ __forceinline__ void load(const NormFwd& a, std::int64_t row, int group, int t) {
+    const int cols = static_cast<int>(a.cols);
+#pragma unroll
+    for (int n = 0; n < kParts; ++n)
+      x[n].load(static_cast<const X*>(a.x.p) + row * a.x.ld, (n * group + t) * 8, cols);
+#pragma unroll
+    for (int n = 0; n < kParts; ++n)
+      r[n].load(static_cast<const S*>(a.r.p) + row * a.r.ld, (n * group + t) * 8, cols);
+  }
+};
+template <typename X, bool kAligned, int kParts>
+struct FwdRow<X, None, kAligned, kParts> {
+  Part<X, kAligned> x[kParts];
+  __device__ __forceinline__ void load(const NormFwd& a, std::int64_t row, int group, int t) {
+#pragma unroll
+    for (int n = 0; n < kParts; ++n)
+      x[n].load(static_cast<const X*>(a.x.p) + row * a.x.ld, (n * group + t) * 8, static_cast<int>(a.cols));
+  }
+};
+
+template <typename X, typename Y, typename S, bool kAligned, int kParts>
 __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int group) {
-  __shared__ float2 slots[2][32];
-  const int id = threadIdx.x / group, t = threadIdx.x - id * group, lane = threadIdx.x & 31;
-  const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * (blockDim.x / group) + id;
-  if (row >= a.rows) return;  // a whole group
-  const int cols = static_cast<int>(a.cols);
-  const std::int64_t out = row * a.cols;
-  const X* x = static_cast<const X*>(a.x.p) + row * a.x.ld;
-  float2 v[kFwdParts][4];
-  {
-    Part<X, kAligned> k[kFwdParts];
-#pragma unroll
-    for (int n = 0; n < kFwdParts; ++n) k[n].load(x, (n * group + t) * 8, cols);
-#pragma unroll
-    for (int n = 0; n < kFwdParts; ++n) k[n].get(v[n]);
-  }
-  const bool joined = lane > 0, last = lane == 31;
-  if (a.r.p != nullptr) {
-#pragma unroll
-    for (int n = 0; n < kFwdParts; ++n) {
-      if (n * group * 8 >= cols) break;
-      const int c = (n * group + t) * 8;
-      float2 r[4];
-      load_any<kAligned>(a.r.p, a.r.t, row * a.r.ld, c, cols, r);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[n][i] = Elem<X>::rounded2(add2(v[n][i], r[i]));
-      Part<X, kAligned>::store(static_cast<X*>(a.s) + out, c, cols, v[n], joined, last);
-    }
-  }
-  float2 sum = {0.0f, 0.0f}, sq = {0.0f, 0.0f};
-#pragma unroll
-  for (int n = 0; n < kFwdParts; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum = add2(sum, v[n][i]);  // 0 past the row's end
+  __shared__ float slots[2][kMaxGroup / 32];
+  const int id = threadIdx.x / group, t = threadIdx.x - id * group, ids = blockDim.x / group, lane = threadIdx.x & 31;
+  const int cols = static_cast<int>(a.cols), ng = static_cast<int>(held_groups(a.cols));
   const float inv = 1.0f / static_cast<float>(cols);
-  sum = group_sum(sum, group, id, slots[0] + id * (group >> 5));
-  const float mean = (sum.x + sum.y) * inv;
+  const bool joined = lane > 0, last = lane == 31;
+  const std::int64_t stride = static_cast<std::int64_t>(gridDim.x) * ids;
+  std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * ids + id;
+  FwdRow<X, S, kAligned, kParts> in;
+  if (row < a.rows) in.load(a, row, group, t);
+  float2 w[kParts][4], b[kParts][4] = {};
 #pragma unroll
-  for (int n = 0; n < kFwdParts; ++n) {
-    const int left = cols - (n * group + t) * 8;
-    if (left >= 8) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[n][i] = add2(v[n][i], both(-mean));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[n][i] = float2{2 * i < left ? v[n][i].x - mean : 0.0f, 2 * i + 1 < left ? v[n][i].y - mean : 0.0f};
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sq = fma2(v[n][i], v[n][i], sq);
+  for (int n = 0; n < kParts; ++n) {
+    load_any<kAligned>(a.w, a.wt, (n * group + t) * 8, cols, w[n]);
+    if (a.b != nullptr) load_any<kAligned>(a.b, a.wt, (n * group + t) * 8, cols, b[n]);
   }
-  sq = group_sum(sq, group, id, slots[1] + id * (group >> 5));
-  const float rstd = rsqrtf((sq.x + sq.y) * inv + a.eps);
-  if (t == 0) {
-    if (a.mean != nullptr) a.mean[row] = mean;
-    if (a.rstd != nullptr) a.rstd[row] = rstd;
-  }
-  const int ng = static_cast<int>(held_groups(a.cols));
+  for (; row < a.rows; row += stride) {
+    float2 v[kParts][4];
 #pragma unroll
-  for (int n = 0; n < kFwdParts; ++n) {
-    if (n * group * 8 >= cols) break;
-    const int c = (n * group + t) * 8;
+    for (int n = 0; n < kParts; ++n) {
+      in.x[n].get(v[n]);
+      if constexpr (!std::is_same<S, None>::value) {
+        float2 r[4];
+        in.r[n].get(r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[n][i] = mul2(v[n][i], both(rstd));
-    if (a.q != nullptr) {
-      uint2 q;
-      const unsigned e = pack_eight(v[n], q);
-      if (c < ng * kGroup) {
-        *reinterpret_cast<uint2*>(a.q + row * ng * kGroup + c) = q;
-        if ((threadIdx.x & 3) == 0) a.scale[row * ng + c / kGroup] = static_cast<std::uint8_t>(e);
+        for (int i = 0; i < 4; ++i) v[n][i] = Elem<X>::rounded2(add2(v[n][i], r[i]));
       }
     }
-    float2 w[4], b[4] = {};
-    load_any<kAligned>(a.w, a.wt, 0, c, cols, w);
-    if (a.b != nullptr) load_any<kAligned>(a.b, a.wt, 0, c, cols, b);
+    if (row + stride < a.rows) in.load(a, row + stride, group, t);
+    float2 sum = {0.0f, 0.0f}, sq = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[n][i] = fma2(v[n][i], w[i], b[i]);
-    Part<Y, kAligned>::store(static_cast<Y*>(a.y) + out, c, cols, v[n], joined, last);
+    for (int n = 0; n < kParts; ++n) {
+      if constexpr (!std::is_same<S, None>::value)
+        Part<X, kAligned>::store(static_cast<X*>(a.s) + row * a.cols, (n * group + t) * 8, cols, v[n], joined, last);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = add2(sum, v[n][i]);  // 0 past the row's end
+    }
+    const float mean = group_sum(sum.x + sum.y, group, id, slots[0] + id * (group >> 5)) * inv;
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) {
+      const int left = cols - (n * group + t) * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[n][i] = add2(v[n][i], both(-mean));
+      if (left < 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (2 * i >= left) v[n][i].x = 0.0f;
+          if (2 * i + 1 >= left) v[n][i].y = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sq = fma2(v[n][i], v[n][i], sq);
+    }
+    const float var = group_sum(sq.x + sq.y, group, id, slots[1] + id * (group >> 5)) * inv;
+    const float rstd = rsqrtf(var + a.eps);
+    if (t == 0 && a.rstd != nullptr) {
+      a.rstd[row] = rstd;
+      if (a.mean != nullptr) a.mean[row] = mean;
+    }
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) {
+      const int c = (n * group + t) * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[n][i] = mul2(v[n][i], both(rstd));
+      if (a.q != nullptr) {
+        uint2 q;
+        const unsigned e = pack_eight(v[n], q);
+        if (c < ng * kGroup) {
+          *reinterpret_cast<uint2*>(a.q + row * ng * kGroup + c) = q;
+          if ((threadIdx.x & 3) == 0) a.scale[row * ng + c / kGroup] = static_cast<std::uint8_t>(e);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[n][i] = fma2(v[n][i], w[n][i], b[n][i]);
+      Part<Y, kAligned>::store(static_cast<Y*>(a.y) + row * a.cols, c, cols, v[n], joined, last);
+    }
   }
 }
 
-// --- backward: groups of threads walk over rows ---
-//
-// A thread keeps its columns from row to row, so their parts of dw and db stay
-// in registers; a block adds its groups' parts up in shared memory and leaves
-// one partial sum of each column, and norm_join adds those. The next row is on
-// its way while one is worked on.
-
-template <typename X, typename Y, bool kAligned, bool kHeld, int kParts>
+// The tensors of a row of the backward pass. kHeld: the normalised input comes
+// from its 8-bit form; kSum: a gradient of the stream is added.
+template <typename X, typename Y, bool kAligned, bool kHeld, bool kSum, int kParts>
 struct BwdRow {
   Part<Y, kAligned> dy[kParts];
-  Part<X, kAligned> s[kHeld ? 1 : kParts];
+  Part<X, kAligned> s[kHeld ? 1 : kParts], ds[kSum ? kParts : 1];
   uint2 q[kHeld ? kParts : 1];  // 8 held values
   unsigned e[kHeld ? kParts : 1];
   float mean, rstd;
 
   __device__ __forceinline__ void load(const NormBwd& a, std::int64_t row, int group, int t) {
     const int cols = static_cast<int>(a.cols);
-    const Y* from = static_cast<const Y*>(a.dy.p) + row * a.dy.ld;
 #pragma unroll
-    for (int n = 0; n < kParts; ++n) dy[n].load(from, (n * group + t) * 8, cols);
+    for (int n = 0; n < kParts; ++n)
+      dy[n].load(static_cast<const Y*>(a.dy.p) + row * a.dy.ld, (n * group + t) * 8, cols);
+    if constexpr (kSum) {
+#pragma unroll
+      for (int n = 0; n < kParts; ++n)
+        ds[n].load(static_cast<const X*>(a.ds.p) + row * a.ds.ld, (n * group + t) * 8, cols);
+    }
     rstd = a.rstd[row];
     if constexpr (!kHeld) {
       mean = a.mean[row];
-      const X* x = static_cast<const X*>(a.s.p) + row * a.s.ld;
 #pragma unroll
-      for (int n = 0; n < kParts; ++n) s[n].load(x, (n * group + t) * 8, cols);
+      for (int n = 0; n < kParts; ++n)
+        s[n].load(static_cast<const X*>(a.s.p) + row * a.s.ld, (n * group + t) * 8, cols);
     } else {
       const int ng = static_cast<int>(held_groups(a.cols));
 #pragma unroll
@@ -211,28 +242,34 @@ struct BwdRow {
   }
 };
 
-template <typename X, typename Y, bool kAligned, bool kHeld, int kParts>
+// A block adds its groups' sums of the columns up in shared memory and leaves one
+// partial sum of each column, and norm_join adds those.
+template <typename X, typename Y, bool kAligned, bool kHeld, bool kSum, int kParts>
 __global__ void __launch_bounds__(kMaxGroup) norm_bwd(const NormBwd a, const int group, float* part) {
   extern __shared__ float sums[];  // [2][cols], where a block has more than one group
-  __shared__ float2 slots[2][32];
+  __shared__ float slots[2][32 * (kMaxGroup / 32)];
   const int id = threadIdx.x / group, t = threadIdx.x - id * group, ids = blockDim.x / group, lane = threadIdx.x & 31;
   const int cols = static_cast<int>(a.cols);
   const float inv = 1.0f / static_cast<float>(cols);
-  float2 dw[kParts][4] = {}, db[kParts][4] = {}, w[kParts][4];
-#pragma unroll
-  for (int n = 0; n < kParts; ++n) load_any<kAligned>(a.w, a.wt, 0, (n * group + t) * 8, cols, w[n]);
   const std::int64_t stride = static_cast<std::int64_t>(gridDim.x) * ids;
   std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * ids + id;
-  BwdRow<X, Y, kAligned, kHeld, kParts> next;
-  if (row < a.rows) next.load(a, row, group, t);
+  BwdRow<X, Y, kAligned, kHeld, kSum, kParts> in;
+  if (row < a.rows) in.load(a, row, group, t);
+  float2 dw[kParts][4] = {}, db[kParts][4] = {}, w[kParts][4];
+#pragma unroll
+  for (int n = 0; n < kParts; ++n) load_any<kAligned>(a.w, a.wt, (n * group + t) * 8, cols, w[n]);
   for (unsigned turn = 0; row < a.rows; row += stride, turn ^= 1u) {
-    const BwdRow<X, Y, kAligned, kHeld, kParts> now = next;
-    if (row + stride < a.rows) next.load(a, row + stride, group, t);
-    float2 g[kParts][4], h[kParts][4], c1 = {0.0f, 0.0f}, c2 = {0.0f, 0.0f};
+    float2 g[kParts][4], h[kParts][4], ds[kSum ? kParts : 1][4], c1 = {0.0f, 0.0f}, c2 = {0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < kParts; ++n) {
-      now.normalised(n, h[n]);
-      now.dy[n].get(g[n]);
+      in.normalised(n, h[n]);
+      in.dy[n].get(g[n]);
+      if constexpr (kSum) in.ds[n].get(ds[n]);
+    }
+    const float rstd = in.rstd;
+    if (row + stride < a.rows) in.load(a, row + stride, group, t);
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         dw[n][i] = fma2(g[n][i], h[n][i], dw[n][i]);
@@ -242,23 +279,21 @@ __global__ void __launch_bounds__(kMaxGroup) norm_bwd(const NormBwd a, const int
         c2 = fma2(g[n][i], h[n][i], c2);
       }
     }
-    const float2 c = group_sum(float2{c1.x + c1.y, c2.x + c2.y}, group, id, slots[turn] + id * (group >> 5));
-    const float2 k0 = both(-c.x * inv), k1 = both(-c.y * inv), r = both(now.rstd);
+    const float2 c = group_sum2(float2{c1.x + c1.y, c2.x + c2.y}, group, id, slots[turn] + id * 32);
+    const float2 k0 = both(-c.x * inv), k1 = both(-c.y * inv), r = both(rstd);
 #pragma unroll
     for (int n = 0; n < kParts; ++n) {
       const int at = (n * group + t) * 8;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) g[n][i] = mul2(fma2(h[n][i], k1, add2(g[n][i], k0)), r);
-      if (a.ds.p != nullptr) {
-        Part<X, kAligned> k;
-        float2 ds[4];
-        k.load(static_cast<const X*>(a.ds.p) + row * a.ds.ld, at, cols);
-        k.get(ds);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) g[n][i] = add2(g[n][i], ds[i]);
+      for (int i = 0; i < 4; ++i) {
+        g[n][i] = mul2(fma2(h[n][i], k1, add2(g[n][i], k0)), r);
+        if constexpr (kSum) g[n][i] = add2(g[n][i], ds[n][i]);
       }
       Part<X, kAligned>::store(static_cast<X*>(a.dx) + row * a.cols, at, cols, g[n], lane > 0, lane == 31);
-      if (a.dr != nullptr) store_any<kAligned>(a.dr, a.rt, row * a.cols, at, cols, g[n], lane > 0, lane == 31);
+      if constexpr (!std::is_same<X, Y>::value) {
+        if (a.dr != nullptr)
+          Part<Y, kAligned>::store(static_cast<Y*>(a.dr) + row * a.cols, at, cols, g[n], lane > 0, lane == 31);
+      }
     }
   }
   if (part == nullptr) return;
@@ -407,8 +442,8 @@ __global__ void __launch_bounds__(32 * kColRows) norm_bwd_columns(const NormBwd 
   }
 }
 
-// The stream's type and the norm's: one type, or a 32-bit stream with a norm of
-// 16 bits (autocast). Other pairs are swept.
+// The stream's type, the norm's and the residual's: one type, or a 32-bit stream
+// with a norm of 16 bits (autocast) and a residual of either. Others are swept.
 bool paired(Type x, Type y) { return x == y || x == Type::f32; }
 template <typename F>
 void with_pair(Type x, Type y, F f) {
@@ -420,86 +455,128 @@ void with_pair(Type x, Type y, F f) {
     f(__half(), __half());
 }
 
-// How the backward pass is laid out.
-struct BwdPlan {
-  bool aligned;
-  int parts, group, ids, blocks;  // parts 0: sweeps, with `blocks` row shares
-};
-
 bool aligned(const void* p, std::int64_t ld, std::int64_t cols) { return p == nullptr || aligned_rows(p, ld, cols); }
 
-// Threads of a group that hold `cols` in up to `parts` parts each.
-int group_of(std::int64_t cols, int parts) {
-  return static_cast<int>((cols + 8 * parts * 32 - 1) / (8 * parts * 32)) * 32;
-}
+// A row's threads and how many rows a block and the GPU work on at once.
+struct Walk {
+  bool aligned;
+  int parts, group, ids;  // parts 0: the row is too long, or its types are rare
+};
 
-BwdPlan plan_of(const NormBwd& a) {
-  BwdPlan p{};
-  p.aligned = aligned(a.dy.p, a.dy.ld, a.cols) && aligned(a.ds.p, a.ds.ld, a.cols) && aligned(a.s.p, a.s.ld, a.cols) &&
-              aligned(a.w, a.cols, a.cols);
-  // One part a thread keeps the registers (two sums and two values for each
-  // element) near 80 and the loads of many rows in flight; long rows take two.
-  p.parts = a.cols <= 8 * kMaxGroup ? 1 : a.cols <= 16 * kMaxGroup ? 2 : 0;
-  if (!paired(a.xt, a.dy.t)) p.parts = 0;
-  const int sms = sm_count();
-  if (p.parts == 0) {
-    const std::int64_t blocks = (a.cols + 31) / 32, want = (8ll * sms + blocks - 1) / blocks, most = (a.rows + 63) / 64;
-    p.blocks = static_cast<int>(want < most ? want : most);
-    return p;
-  }
-  p.group = group_of(a.cols, p.parts);
-  p.ids = p.group < 384 ? 384 / p.group : 1;
-  // two blocks an SM, or fewer where a group would have under four rows
-  const std::int64_t want = (a.rows + 4ll * p.ids - 1) / (4ll * p.ids);
-  p.blocks = static_cast<int>(want < 2 * sms ? want : 2 * sms);
+Walk walk_of(std::int64_t cols, bool aligned, bool types, int ones) {
+  Walk p{};
+  p.aligned = aligned;
+  // Two parts a thread halve the cost of a row's sums; up to `ones` columns one
+  // part fits a row better (768 columns are 96 threads of one, or 64 with 16
+  // idle), or the registers of two would spill.
+  p.parts = !types || cols > 16 * kMaxGroup ? 0 : cols <= ones ? 1 : 2;
+  if (p.parts == 0) return p;
+  p.group = static_cast<int>((cols + 8 * p.parts * 32 - 1) / (8 * p.parts * 32)) * 32;
+  p.ids = p.group < kBlock ? kBlock / p.group : 1;
   return p;
 }
 
-template <typename X, typename Y, bool kAligned, bool kHeld>
-void launch_bwd(const NormBwd& a, const BwdPlan& p, float* part, cudaStream_t stream) {
-  const int threads = p.group * p.ids;
-  const std::size_t smem = p.ids > 1 ? 2 * sizeof(float) * a.cols : 0;
-  if (p.parts == 1)
-    norm_bwd<X, Y, kAligned, kHeld, 1><<<p.blocks, threads, smem, stream>>>(a, p.group, part);
+// Blocks that fill the GPU, or fewer where a group would have under `least` rows.
+template <auto kKernel>
+int blocks_of(const Walk& p, std::int64_t rows, int least) {
+  static const int registers = [] {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, kKernel) == cudaSuccess ? (at.numRegs + 7) / 8 * 8 : 128;
+  }();
+  const int threads = p.group * p.ids, fit = 65536 / (registers * threads);
+  const std::int64_t most = static_cast<std::int64_t>(sm_count()) * (fit < 1 ? 1 : fit);
+  const std::int64_t want = (rows + static_cast<std::int64_t>(least) * p.ids - 1) / (static_cast<std::int64_t>(least) * p.ids);
+  return static_cast<int>(want < most ? want : most);
+}
+
+Walk walk_of(const NormBwd& a) {
+  const bool all = aligned(a.dy.p, a.dy.ld, a.cols) && aligned(a.ds.p, a.ds.ld, a.cols) &&
+                   aligned(a.s.p, a.s.ld, a.cols) && aligned(a.w, a.cols, a.cols);
+  return walk_of(a.cols, all, paired(a.xt, a.dy.t) && (a.dr == nullptr || a.rt == a.dy.t),
+                 a.ds.p != nullptr ? 8 * kMaxGroup : 4 * kMaxGroup);
+}
+
+// Shares of the rows of a sweep over the columns.
+int sweep_shares(const NormBwd& a) {
+  const std::int64_t blocks = (a.cols + 31) / 32, want = (8ll * sm_count() + blocks - 1) / blocks;
+  const std::int64_t most = (a.rows + 63) / 64;
+  return static_cast<int>(want < most ? want : most);
+}
+
+constexpr int kMostPartials = 16;  // blocks an SM: 2 * 16 * 148 sums of a column at most
+
+template <auto kKernel>
+void go_fwd(const NormFwd& a, const Walk& p, cudaStream_t stream) {
+  kKernel<<<blocks_of<kKernel>(p, a.rows, 1), p.group * p.ids, 0, stream>>>(a, p.group);
+}
+
+template <typename X, typename Y, typename S>
+void launch_fwd(const NormFwd& a, const Walk& p, cudaStream_t stream) {
+  if (p.aligned)
+    p.parts == 1 ? go_fwd<norm_fwd<X, Y, S, true, 1>>(a, p, stream) : go_fwd<norm_fwd<X, Y, S, true, 2>>(a, p, stream);
   else
-    norm_bwd<X, Y, kAligned, kHeld, 2><<<p.blocks, threads, smem, stream>>>(a, p.group, part);
+    p.parts == 1 ? go_fwd<norm_fwd<X, Y, S, false, 1>>(a, p, stream) : go_fwd<norm_fwd<X, Y, S, false, 2>>(a, p, stream);
+}
+
+template <auto kKernel>
+int go_bwd(const NormBwd& a, const Walk& p, float* part, cudaStream_t stream) {
+  int blocks = blocks_of<kKernel>(p, a.rows, 4);
+  if (blocks > kMostPartials * sm_count()) blocks = kMostPartials * sm_count();
+  kKernel<<<blocks, p.group * p.ids, p.ids > 1 ? 2 * sizeof(float) * a.cols : 0, stream>>>(a, p.group, part);
+  return blocks;
+}
+
+template <typename X, typename Y, bool kAligned, bool kHeld, bool kSum>
+int launch_bwd(const NormBwd& a, const Walk& p, float* part, cudaStream_t stream) {
+  return p.parts == 1 ? go_bwd<norm_bwd<X, Y, kAligned, kHeld, kSum, 1>>(a, p, part, stream)
+                      : go_bwd<norm_bwd<X, Y, kAligned, kHeld, kSum, 2>>(a, p, part, stream);
 }
 
 }  // namespace
 
 cudaError_t norm_forward(const NormFwd& a, cudaStream_t stream) {
-  if (a.cols > 8 * kFwdParts * kMaxGroup || !paired(a.x.t, a.yt)) {
+  const bool all = aligned(a.x.p, a.x.ld, a.cols) && aligned(a.r.p, a.r.ld, a.cols) && aligned(a.w, a.cols, a.cols) &&
+                   aligned(a.b, a.cols, a.cols);
+  const Walk p = walk_of(a.cols, all, paired(a.x.t, a.yt) && (a.r.p == nullptr || a.r.t == a.x.t || a.r.t == a.yt),
+                         8 * kMaxGroup);
+  if (p.parts == 0) {
     const std::int64_t most = 32ll * sm_count();
     norm_fwd_sweep<<<static_cast<unsigned>(a.rows < most ? a.rows : most), kSweep, 0, stream>>>(a);
   } else {
-    const bool all = aligned(a.x.p, a.x.ld, a.cols) && aligned(a.r.p, a.r.ld, a.cols) &&
-                     aligned(a.w, a.cols, a.cols) && aligned(a.b, a.cols, a.cols);
-    const int group = group_of(a.cols, kFwdParts), ids = group < 256 ? 256 / group : 1;
-    const unsigned blocks = static_cast<unsigned>((a.rows + ids - 1) / ids);
     with_pair(a.x.t, a.yt, [&](auto x, auto y) {
       using X = decltype(x);
       using Y = decltype(y);
-      if (all)
-        norm_fwd<X, Y, true><<<blocks, group * ids, 0, stream>>>(a, group);
+      if (a.r.p == nullptr)
+        launch_fwd<X, Y, None>(a, p, stream);
+      else if (a.r.t == a.x.t)
+        launch_fwd<X, Y, X>(a, p, stream);
       else
-        norm_fwd<X, Y, false><<<blocks, group * ids, 0, stream>>>(a, group);
+        launch_fwd<X, Y, Y>(a, p, stream);
     });
   }
   commux_ops::g_launches++;
   return cudaGetLastError();
 }
 
-std::int64_t norm_backward_work(const NormBwd& a) { return 2ll * plan_of(a).blocks * a.cols; }
+std::int64_t norm_backward_work(const NormBwd& a) {
+  const Walk p = walk_of(a);
+  if (p.parts == 0) return 2ll * sweep_shares(a) * a.cols;
+  const std::int64_t most = static_cast<std::int64_t>(kMostPartials) * sm_count();
+  const std::int64_t want = (a.rows + 4ll * p.ids - 1) / (4ll * p.ids);
+  return 2 * (want < most ? want : most) * a.cols;
+}
 
 cudaError_t norm_backward(const NormBwd& a, cudaStream_t stream) {
-  const BwdPlan p = plan_of(a);
+  const Walk p = walk_of(a);
   const bool columns = a.dw != nullptr || a.db != nullptr;
+  int parts = 0;
   if (p.parts == 0) {
     const std::int64_t most = 32ll * sm_count();
     norm_bwd_sweep<<<static_cast<unsigned>(a.rows < most ? a.rows : most), kSweep, 0, stream>>>(a);
     commux_ops::g_launches++;
     if (columns) {
-      norm_bwd_columns<<<dim3(static_cast<unsigned>((a.cols + 31) / 32), p.blocks), dim3(32, kColRows), 0, stream>>>(
+      parts = sweep_shares(a);
+      norm_bwd_columns<<<dim3(static_cast<unsigned>((a.cols + 31) / 32), parts), dim3(32, kColRows), 0, stream>>>(
           a, a.work);
       commux_ops::g_launches++;
     }
@@ -508,20 +585,21 @@ cudaError_t norm_backward(const NormBwd& a, cudaStream_t stream) {
       using X = decltype(x);
       using Y = decltype(y);
       float* part = columns ? a.work : nullptr;
-      if (p.aligned && a.q != nullptr)
-        launch_bwd<X, Y, true, true>(a, p, part, stream);
-      else if (p.aligned)
-        launch_bwd<X, Y, true, false>(a, p, part, stream);
-      else if (a.q != nullptr)
-        launch_bwd<X, Y, false, true>(a, p, part, stream);
-      else
-        launch_bwd<X, Y, false, false>(a, p, part, stream);
+      auto sum = [&](auto aligned, auto held) {
+        constexpr bool kAligned = decltype(aligned)::value, kHeld = decltype(held)::value;
+        parts = a.ds.p != nullptr ? launch_bwd<X, Y, kAligned, kHeld, true>(a, p, part, stream)
+                                  : launch_bwd<X, Y, kAligned, kHeld, false>(a, p, part, stream);
+      };
+      auto held = [&](auto aligned) {
+        a.q != nullptr ? sum(aligned, std::true_type()) : sum(aligned, std::false_type());
+      };
+      p.aligned ? held(std::true_type()) : held(std::false_type());
     });
     commux_ops::g_launches++;
   }
   if (columns) {
     norm_join<<<dim3(static_cast<unsigned>((a.cols + 31) / 32), 2), dim3(32, kJoin), 0, stream>>>(
-        a.work, p.blocks, a.cols, a.dw, a.db, a.wt);
+        a.work, parts, a.cols, a.dw, a.db, a.wt);
     commux_ops::g_launches++;
   }
   return cudaGetLastError();

@@ -27,11 +27,14 @@ constexpr int kStages = 3;                // dy and 8-bit tiles in flight
 constexpr int kWide = 2;                  // widened tiles
 constexpr int kBox = 64 * kK * 2;         // a 64-wide bf16 box of a step
 constexpr int kBytesA = kM * kK * 2, kBytesQ = kN * kK, kBytesB = kN * kK * 2;
-constexpr int kOffQ = kStages * kBytesA, kOffB = kOffQ + kStages * kBytesQ, kOffBars = kOffB + kWide * kBytesB;
+constexpr int kBytesS = kK * (kN / kGroup) * 4;  // a step's steps (scales) as floats
+constexpr int kOffQ = kStages * kBytesA, kOffB = kOffQ + kStages * kBytesQ, kOffS = kOffB + kWide * kBytesB;
+constexpr int kOffBars = kOffS + kStages * kBytesS;
 constexpr int kSmem = kOffBars + 256 + 1024;  // and room to align
 constexpr int kConvert = 8;               // widening warps, which also write the results
 constexpr int kColumn = 4;                // warps that sum dy's columns
-constexpr int kThreads = 32 * (2 + kConvert + kColumn);
+constexpr int kScale = 2;                 // warps that fetch scales, a lane to a token
+constexpr int kThreads = 32 * (2 + kConvert + kColumn + kScale);
 constexpr int kSlot = kM * kN + kM;       // floats of a partial tile: sums, then db
 
 // Steps of all tiles in a row are dealt out evenly to the CTAs: a CTA's range
@@ -155,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kStages; ++s) {
       async::mbar_init(&full_a[s], 1);
       async::mbar_init(&empty_a[s], 1 + kColumn);
-      async::mbar_init(&full_q[s], 1);
+      async::mbar_init(&full_q[s], 1 + kScale);
       async::mbar_init(&empty_q[s], kConvert);
     }
     for (int s = 0; s < kWide; ++s) {
@@ -261,22 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (std::int64_t at = begin; ok && at < end; ++seg) {
       const Segment s = segment(p, at, begin, end);
       const bool busy = unit * 16 < s.n;
-      const std::int64_t group = s.n0 / kGroup + (unit >> 1);
-      unsigned next[4];
-      auto fetch = [&](int k) {  // the scales of a step's four rows of this lane
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const std::int64_t t = static_cast<std::int64_t>(k) * kK + j * 16 + row0;
-          next[j] = t < p.rows && group < p.groups ? scale[t * p.groups + group] : 1u;
-        }
-      };
-      fetch(s.first);
       for (int k = s.first; k < s.last; ++k, ++i) {
         const unsigned sq = i % kStages, sb = i % kWide;
-        unsigned e[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = next[j];
-        if (k + 1 < s.last) fetch(k + 1);
         ok = async::bounded_wait(&full_q[sq], i / kStages & 1u, bound) &&
              async::bounded_wait(&empty_b[sb], i / kWide & 1u ^ 1u, bound);
         if (!__all_sync(0xffffffffu, ok)) {
@@ -284,6 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         const unsigned char* from = smem + kOffQ + sq * kBytesQ;
+        const float* steps = reinterpret_cast<const float*>(smem + kOffS + sq * kBytesS) + (unit >> 1);
         unsigned char* to = smem + kOffB + sb * kBytesB + block * kBox;
         if (busy) {
 #pragma unroll
@@ -291,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int r = j * 16 + row0;
             uint4 v = *reinterpret_cast<const uint4*>(from + r * kN + unit * 16);
             v.x ^= 0x80808080u, v.y ^= 0x80808080u, v.z ^= 0x80808080u, v.w ^= 0x80808080u;
-            const float2 step = both(step_of(e[j]));
+            const float2 step = both(steps[r * (kN / kGroup)]);
             const uint4 lo = {widen2(v.x, 0, step), widen2(v.x, 2, step), widen2(v.y, 0, step), widen2(v.y, 2, step)};
             const uint4 hi = {widen2(v.z, 0, step), widen2(v.z, 2, step), widen2(v.w, 0, step), widen2(v.w, 2, step)};
             // odd blocks write their halves the other way round: the 8 lanes of
@@ -357,6 +347,49 @@ __global__ void __launch_bounds__(kThreads, 1)
       // every warp has read its `turn` before any widens the next tile
       ok = async::bounded_wait(sums_empty, seg & 1u, bound);
       ok = __all_sync(0xffffffffu, ok);
+    }
+  } else if (warp >= 2 + kConvert + kColumn) {  // --- scales
+    // They are bytes at any alignment, which TMA cannot fetch; the widening warps
+    // spent more than half of their time on waiting for their own loads of them.
+    // Two steps are on their way while one is written.
+    const int token = (warp - 2 - kConvert - kColumn) * 32 + lane;
+    constexpr int kEach = kN / kGroup;
+    unsigned i = 0;
+    bool ok = true;
+    for (std::int64_t at = begin; ok && at < end;) {
+      const Segment s = segment(p, at, begin, end);
+      const int some = static_cast<int>(p.groups - s.n0 / kGroup < kEach ? p.groups - s.n0 / kGroup : kEach);
+      unsigned ahead[2][kEach];
+      auto fetch = [&](int k, unsigned (&e)[kEach]) {
+        const std::int64_t t = static_cast<std::int64_t>(k) * kK + token;
+        const std::uint8_t* from = scale + t * p.groups + s.n0 / kGroup;
+        const bool in = k < s.last && t < p.rows;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          e[j] = 1;
+          if (in && j < some) e[j] = from[j];
+        }
+      };
+      fetch(s.first, ahead[0]);
+      fetch(s.first + 1, ahead[1]);
+      auto put = [&](int k, unsigned (&e)[kEach]) {
+        const unsigned sq = i % kStages;
+        ok = async::bounded_wait(&empty_q[sq], i / kStages & 1u ^ 1u, bound);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        float4* to = reinterpret_cast<float4*>(smem + kOffS + sq * kBytesS) + token * (kEach / 4);
+        to[0] = float4{step_of(e[0]), step_of(e[1]), step_of(e[2]), step_of(e[3])};
+        to[1] = float4{step_of(e[4]), step_of(e[5]), step_of(e[6]), step_of(e[7])};
+        fetch(k + 2, e);
+        __syncwarp();
+        if (lane == 0) async::mbar_arrive(&full_q[sq]);
+        ++i;
+      };
+      for (int k = s.first; ok && k < s.last; k += 2) {
+        put(k, ahead[0]);
+        if (ok && k + 1 < s.last) put(k + 1, ahead[1]);
+      }
+      at += s.last - s.first;
     }
   } else {  // --- sums of dy's columns
     const int c = (warp - 2 - kConvert) * 32 + lane;  // columns 2c and 2c + 1 of the tile

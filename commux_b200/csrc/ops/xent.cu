@@ -17,6 +17,8 @@
 
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "async.cuh"
 #include "train_utils.cuh"
 
@@ -25,6 +27,14 @@ namespace train {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// The largest value of a warp; NaN if there is one.
+__device__ __forceinline__ float largest(float v) {
+  float m;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+
 constexpr int kEach = 32;      // elements of a thread
 constexpr int kSweep = 512;
 
@@ -76,21 +86,13 @@ struct Row {
   static constexpr int E = 16 / sizeof(T), kVectors = kEach / E;
   float2 v[kEach / 2];
 
-  // vector k; elements [from, to) of its E are the row's, the others do not count
-  __device__ __forceinline__ void take(int k, uint4 w, int from, int to) {
+  __device__ __forceinline__ void take(int k, uint4 w) {
     float2* p = v + k * (E / 2);
     if constexpr (sizeof(T) == 4) {
       p[0] = float2{__uint_as_float(w.x), __uint_as_float(w.y)};
       p[1] = float2{__uint_as_float(w.z), __uint_as_float(w.w)};
     } else {
       p[0] = Elem<T>::get2(w.x), p[1] = Elem<T>::get2(w.y), p[2] = Elem<T>::get2(w.z), p[3] = Elem<T>::get2(w.w);
-    }
-    if (from > 0 || to < E) {
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        if (2 * i < from || 2 * i >= to) p[i].x = -INFINITY;
-        if (2 * i + 1 < from || 2 * i + 1 >= to) p[i].y = -INFINITY;
-      }
     }
   }
 
@@ -113,20 +115,41 @@ struct Row {
   }
 };
 
-// Vector `at` of a row part of `cols` elements that starts `shift` elements
-// into vector 0: which of its elements are the part's.
+// A row part of `cols` elements that starts `shift` elements into vector 0:
+// which elements of vector `at` are the part's.
 template <int E>
-__device__ __forceinline__ void part_of(int at, int shift, int cols, int& from, int& to) {
-  from = at == 0 ? shift : 0;
-  to = min(E, shift + cols - at * E);
+struct Span {
+  int from, to;
+  __device__ __forceinline__ Span(int at, int shift, int cols)
+      : from(at == 0 ? shift : 0), to(min(E, shift + cols - at * E)) {}
+  __device__ __forceinline__ bool none() const { return to <= 0; }
+  __device__ __forceinline__ bool all() const { return from == 0 && to == E; }
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 minus_infinities() {
+  const unsigned w = sizeof(T) == 4 ? 0xff800000u : Elem<T>::kType == Type::bf16 ? 0xff80ff80u : 0xfc00fc00u;
+  return {w, w, w, w};
 }
 
-// Gradient of a row part: columns [first, first + cols), `shift` as it is in dx.
-// Where dx has the logits' shift (`aligned`) its vectors are those of the
-// registers. A row that does not count has a scale and an f of 0.
+// What is not the part's in the first and last vector of a part becomes -inf, in
+// the shared memory that this thread alone reads it from. (In registers every
+// vector of every thread would pay for the test of each element.)
 template <typename T>
+__device__ __forceinline__ void blank(uint4* vector, Span<Row<T>::E> s) {
+  T* v = reinterpret_cast<T*>(vector);
+#pragma unroll 1
+  for (int i = 0; i < Row<T>::E; ++i)
+    if (i < s.from || i >= s.to) v[i] = Elem<T>::put(-INFINITY);
+}
+
+// Gradient of a row part, to dx, but for what the target takes from its own.
+// Where dx has the logits' shift (`aligned`) its vectors are those of the
+// registers. `spare`: shared memory of this thread. kWhole: there is no shift
+// and no part of a vector, here and in the logits.
+template <typename T, bool kWhole>
 __device__ __forceinline__ void write_part(T* dx, Row<T>& r, int cols, int shift, bool aligned, int threads, int t,
-                                           int mine, float scale, float f) {
+                                           float scale, uint4* spare) {
   constexpr int E = Row<T>::E;
 #pragma unroll
   for (int k = 0; k < Row<T>::kVectors; ++k) {
@@ -135,49 +158,53 @@ __device__ __forceinline__ void write_part(T* dx, Row<T>& r, int cols, int shift
     float2* v = r.v + k * (E / 2);
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) v[i] = mul2(v[i], both(scale));
-    const int hit = mine - at * E;  // the target among these
-    if (hit >= 0 && hit < E) {
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        if (hit == 2 * i) v[i].x -= f;
-        if (hit == 2 * i + 1) v[i].y -= f;
-      }
-    }
-    int from, to;
-    part_of<E>(at, shift, cols, from, to);
+    uint4 w;
+    if constexpr (sizeof(T) == 4)
+      w = uint4{__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y)};
+    else
+      w = uint4{Elem<T>::put2(v[0]), Elem<T>::put2(v[1]), Elem<T>::put2(v[2]), Elem<T>::put2(v[3])};
     T* out = dx + at * E - shift;
-    if (aligned && from == 0 && to == E) {
-      uint4 w;
-      if constexpr (sizeof(T) == 4)
-        w = uint4{__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y)};
-      else
-        w = uint4{Elem<T>::put2(v[0]), Elem<T>::put2(v[1]), Elem<T>::put2(v[2]), Elem<T>::put2(v[3])};
+    if constexpr (kWhole) {
+      *reinterpret_cast<uint4*>(out) = w;
+      continue;
+    }
+    const Span<E> span(at, shift, cols);
+    if (aligned && span.all()) {
       *reinterpret_cast<uint4*>(out) = w;
     } else {
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        if (2 * i >= from && 2 * i < to) out[2 * i] = Elem<T>::put(v[i].x);
-        if (2 * i + 1 >= from && 2 * i + 1 < to) out[2 * i + 1] = Elem<T>::put(v[i].y);
-      }
+      *spare = w;
+      const T* from = reinterpret_cast<const T*>(spare);
+#pragma unroll 1
+      for (int i = span.from; i < span.to; ++i) out[i] = from[i];
     }
   }
 }
 
-// The rows that are ignored get zeros, whatever they hold.
-template <typename T>
+// A row part's gradient; `owner`: this thread holds the target, `logit` is its
+// value. The target's element is written over by the thread that wrote it.
+template <typename T, bool kWhole>
 __device__ __forceinline__ void write_row_part(const Xent& a, Row<T>& r, std::int64_t row, int first, int cols,
                                                int shift, bool aligned, int threads, int t, std::int64_t target,
-                                               float f, float inv) {
+                                               bool owner, float logit, float m, float s, float f, uint4* spare) {
   T* dx = static_cast<T*>(a.dx) + row * a.cols + first;
-  if (target == a.ignore) {
+  if (target == a.ignore) {  // zeros, whatever the row holds
 #pragma unroll
     for (int i = 0; i < kEach / 2; ++i) r.v[i] = float2{0.0f, 0.0f};
-    write_part<T>(dx, r, cols, shift, aligned, threads, t, -1, 0.0f, 0.0f);
-  } else {
-    const bool bad = bad_target(a, target);
-    const int mine = bad ? -1 : static_cast<int>(target - first + shift);  // in elements of the vectors
-    write_part<T>(dx, r, cols, shift, aligned, threads, t, mine, bad ? nan_value() : f * inv, f);
+    write_part<T, kWhole>(dx, r, cols, shift, aligned, threads, t, 0.0f, spare);
+    return;
   }
+  const bool bad = bad_target(a, target);
+  const float scale = bad ? nan_value() : f * (1.0f / s);
+  write_part<T, kWhole>(dx, r, cols, shift, aligned, threads, t, scale, spare);
+  if (owner && !bad)
+    static_cast<T*>(a.dx)[row * a.cols + target] = Elem<T>::put(exp2_fast((logit - m) * kLog2e) * scale - f);
+}
+
+// The thread (of a row's part) that holds the target; the first one where no
+// element is the target, so that somebody writes the loss.
+template <int E>
+__device__ __forceinline__ int owner_of(const Xent& a, std::int64_t target, int shift, int threads) {
+  return target == a.ignore || bad_target(a, target) ? 0 : static_cast<int>((target + shift) / E % threads);
 }
 
 __device__ __forceinline__ int shift_of(const void* p, int size) {
@@ -189,6 +216,7 @@ __device__ __forceinline__ int shift_of(const void* p, int size) {
 template <typename T>
 __global__ void __launch_bounds__(512) xent_rows(const Xent a, const int group) {
   __shared__ float slots[2][32];
+  __shared__ uint4 spare[512];
   constexpr int E = Row<T>::E;
   const int id = threadIdx.x / group, t = threadIdx.x - id * group, warps = group >> 5, lane = t & 31;
   const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * (blockDim.x / group) + id;
@@ -197,25 +225,31 @@ __global__ void __launch_bounds__(512) xent_rows(const Xent a, const int group) 
   const T* x = static_cast<const T*>(a.x.p) + row * a.x.ld;
   const int shift = shift_of(x, sizeof(T));
   const std::int64_t target = a.target[row];
-  const float logit = t == 0 ? target_logit(a, row, target) : 0.0f;  // on its way early
+  const bool owner = t == owner_of<E>(a, target, shift, group);
+  const float logit = owner ? target_logit(a, row, target) : 0.0f;  // on its way early
   Row<T> r;
   uint4 w[Row<T>::kVectors];
 #pragma unroll
   for (int k = 0; k < Row<T>::kVectors; ++k) {
     const int at = k * group + t;
+    w[k] = minus_infinities<T>();
     if (at * E < shift + cols) w[k] = *reinterpret_cast<const uint4*>(x - shift + at * E);
   }
 #pragma unroll
   for (int k = 0; k < Row<T>::kVectors; ++k) {
-    int from, to;
-    part_of<E>(k * group + t, shift, cols, from, to);
-    r.take(k, w[k], from, to);
+    const Span<E> span(k * group + t, shift, cols);
+    if (!span.all() && !span.none()) {
+      spare[threadIdx.x] = w[k];
+      blank<T>(&spare[threadIdx.x], span);
+      w[k] = spare[threadIdx.x];
+    }
+    r.take(k, w[k]);
   }
-  float m = warp_max(r.max());
+  float m = largest(r.max());
   if (warps > 1) {
     if (lane == 0) slots[0][t >> 5] = m;
     __syncthreads();
-    m = warp_max(lane < warps ? slots[0][lane] : -INFINITY);
+    m = largest(lane < warps ? slots[0][lane] : -INFINITY);
   }
   float s = warp_sum(r.exponentials(m));
   if (warps > 1) {
@@ -223,11 +257,11 @@ __global__ void __launch_bounds__(512) xent_rows(const Xent a, const int group) 
     __syncthreads();
     s = warp_sum(lane < warps ? slots[1][lane] : 0.0f);
   }
-  if (t == 0) finish_row(a, row, target, logit, m, s);
+  if (owner) finish_row(a, row, target, logit, m, s);
   if (a.dx != nullptr) {
     const bool aligned = shift_of(static_cast<T*>(a.dx) + row * a.cols, sizeof(T)) == shift;
-    write_row_part<T>(a, r, row, 0, cols, shift, aligned, group, t, target,
-                  1.0f / (a.reduction == 1 ? a.work[0] : 1.0f), 1.0f / s);
+    write_row_part<T, false>(a, r, row, 0, cols, shift, aligned, group, t, target, owner, logit, m, s,
+                      1.0f / (a.reduction == 1 ? a.work[0] : 1.0f), &spare[threadIdx.x]);
   }
 }
 
@@ -259,11 +293,12 @@ __device__ __forceinline__ void send(float* to, std::uint64_t* bar, int rank, fl
                : "memory");
 }
 
-template <typename T, int kC>
+template <typename T, int kC, bool kWhole>
 __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* status, std::uint64_t limit_ns) {
   extern __shared__ __align__(128) unsigned char ring[];
   __shared__ std::uint64_t full[kRing], joined[2][2];
   __shared__ float slots[2][32], ranks[2][2][8];
+  __shared__ uint4 spare[kLong];
   __shared__ int gave_up;
   constexpr int E = Row<T>::E, kV = Row<T>::kVectors;
   namespace cg = cooperative_groups;
@@ -289,7 +324,7 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
   // Pieces are numbered through the rows; piece n goes to slot n % kRing. Every
   // row of this block has the same pieces but for one that a shift may add.
   auto vectors = [&](std::int64_t row) {
-    return cols == 0 ? 0 : (shift_of(part(row), sizeof(T)) + cols + E - 1) / E;
+    return kWhole ? cols / E : cols == 0 ? 0 : (shift_of(part(row), sizeof(T)) + cols + E - 1) / E;
   };
   auto pieces = [&](std::int64_t row) { return (vectors(row) + kLong - 1) / kLong; };
   unsigned issued = 0, used = 0;
@@ -325,32 +360,43 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
     return ranks[set][which][lane & (kC - 1)];
   };
   for (std::int64_t row = mine; row < a.rows; row += clusters, ++round) {
-    const int n = pieces(row), shift = shift_of(part(row), sizeof(T));
+    const int n = pieces(row), shift = kWhole ? 0 : shift_of(part(row), sizeof(T));
     const std::int64_t target = a.target[row];
-    const float logit = t == 0 && rank == 0 ? target_logit(a, row, target) : 0.0f;  // on its way early
+    // the part that holds the target, or the first one where none does
+    const bool here = target == a.ignore || bad_target(a, target) ? rank == 0 : target >= first && target - first < cols;
+    const bool owner = here && t == owner_of<E>(a, target, shift - first, kLong);
+    const float logit = owner ? target_logit(a, row, target) : 0.0f;  // on its way early
     Row<T> r;
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
-      uint4 w = {0, 0, 0, 0};
+      uint4 w = minus_infinities<T>();
       if (k < n) {
         const unsigned slot = (used + k) % kRing;
         async::bounded_wait(&full[slot], (used + k) / kRing & 1u, bound);
-        w = *reinterpret_cast<const uint4*>(ring + slot * kPiece + t * 16);
+        uint4* vector = reinterpret_cast<uint4*>(ring + slot * kPiece) + t;
+        const Span<E> span(k * kLong + t, shift, cols);
+        if (kWhole) {
+          if ((k * kLong + t) * E < cols) w = *vector;
+        } else if (!span.none()) {
+          if (!span.all()) {
+            blank<T>(vector, span);
+            async::fence_async();  // the slot's next copy comes after these writes
+          }
+          w = *vector;
+        }
       }
-      int from, to;
-      part_of<E>(k * kLong + t, shift, cols, from, to);
-      r.take(k, w, from, to);
+      r.take(k, w);
     }
     used += n;
-    float m = warp_max(r.max());
+    float m = largest(r.max());
     if (lane == 0) slots[0][t >> 5] = m;
     __syncthreads();  // and every thread has its elements: their pieces are free
     if (t == 0) {
       async::fence_async();
       request();
     }
-    m = warp_max(slots[0][lane]);
-    if constexpr (kC > 1) m = warp_max(exchange(0, m));
+    m = largest(slots[0][lane]);
+    if constexpr (kC > 1) m = largest(exchange(0, m));
     float s = warp_sum(r.exponentials(m));
     if (lane == 0) slots[1][t >> 5] = s;
     __syncthreads();
@@ -359,10 +405,10 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
       const float part = exchange(1, s);
       s = warp_sum(lane < kC ? part : 0.0f);
     }
-    if (t == 0 && rank == 0) finish_row(a, row, target, logit, m, s);
+    if (owner) finish_row(a, row, target, logit, m, s);
     if (a.dx != nullptr) {
-      const bool aligned = shift_of(static_cast<T*>(a.dx) + row * a.cols + first, sizeof(T)) == shift;
-      write_row_part<T>(a, r, row, first, cols, shift, aligned, kLong, t, target, f, 1.0f / s);
+      const bool aligned = kWhole || shift_of(static_cast<T*>(a.dx) + row * a.cols + first, sizeof(T)) == shift;
+      write_row_part<T, kWhole>(a, r, row, first, cols, shift, aligned, kLong, t, target, owner, logit, m, s, f, &spare[t]);
     }
   }
   // shared memory outlives the copies, and what other blocks send, also where a wait gave up
@@ -422,9 +468,10 @@ unsigned grid_of(std::int64_t rows) {
   return static_cast<unsigned>(rows < 1 ? 1 : rows < most ? rows : most);
 }
 
-template <typename T, int kC>
+template <typename T, int kC, bool kWhole>
 cudaError_t launch_long(const Xent& a, cudaStream_t stream) {
-  cudaError_t rc = cudaFuncSetAttribute(xent_long<T, kC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  const auto kernel = xent_long<T, kC, kWhole>;
+  const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
   if (rc != cudaSuccess) return rc;
   const std::int64_t most = sm_count() / kC;
   cudaLaunchConfig_t cfg{};
@@ -440,7 +487,7 @@ cudaError_t launch_long(const Xent& a, cudaStream_t stream) {
   cfg.numAttrs = 1;
   unsigned* status = nullptr;
   commux_ops::status_word(&status);
-  return cudaLaunchKernelEx(&cfg, xent_long<T, kC>, a, status, commux_ops::wait_limit_ns());
+  return cudaLaunchKernelEx(&cfg, kernel, a, status, commux_ops::wait_limit_ns());
 }
 
 template <typename T>
@@ -461,8 +508,15 @@ cudaError_t launch_rows(const Xent& a, cudaStream_t stream) {
     xent_sweep<<<grid_of(a.rows), kSweep, 0, stream>>>(a);
     return cudaSuccess;
   }
-  return c == 1 ? launch_long<T, 1>(a, stream)
-                : c == 2 ? launch_long<T, 2>(a, stream) : c == 4 ? launch_long<T, 4>(a, stream) : launch_long<T, 8>(a, stream);
+  const bool whole = a.cols % E == 0 && a.x.ld % E == 0 && reinterpret_cast<std::uintptr_t>(a.x.p) % 16 == 0;
+  auto go = [&](auto blocks) {
+    constexpr int kC = decltype(blocks)::value;
+    return whole ? launch_long<T, kC, true>(a, stream) : launch_long<T, kC, false>(a, stream);
+  };
+  return c == 1   ? go(std::integral_constant<int, 1>())
+         : c == 2 ? go(std::integral_constant<int, 2>())
+         : c == 4 ? go(std::integral_constant<int, 4>())
+                  : go(std::integral_constant<int, 8>());
 }
 
 }  // namespace

@@ -59,18 +59,6 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, std::uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<std::uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(std::uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 // Writes of this thread to shared memory become visible to TMA and the tensor core.
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -82,18 +70,104 @@ struct Bound {
   std::uint64_t limit_ns;
 };
 
-__device__ __forceinline__ bool bounded_wait(std::uint64_t* bar, unsigned parity, const Bound& b) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const std::uint64_t t0 = gtimer();
-  while (!mbar_try_wait(bar, parity)) {
-    if (*b.gave_up != 0) return false;
-    if (gtimer() - t0 > b.limit_ns) {
-      *b.gave_up = 1;
-      if (b.status != nullptr) atomicExch(b.status, 1u);
+// The waits below take the barrier's address in shared memory.
+template <bool kCluster>
+__device__ __forceinline__ bool try_wait(std::uint32_t bar, unsigned parity) {
+  unsigned done;
+  if constexpr (kCluster)  // a barrier that the cluster's other CTAs arrive on
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.b32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.b32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  return done != 0;
+}
+
+template <bool kCluster>
+__device__ __noinline__ bool wait_longer(std::uint32_t bar, unsigned parity, volatile int* gave_up, unsigned* status,
+                                         std::uint64_t limit_ns) {
+  std::uint64_t since = 0;
+  for (unsigned tries = 1; !try_wait<kCluster>(bar, parity); ++tries) {
+    if (tries % 64 != 0) continue;  // the timer and the flag in one of many tries
+    if (*gave_up != 0) return false;
+    const std::uint64_t now = gtimer();
+    if (since == 0) since = now;
+    if (now - since > limit_ns) {
+      *gave_up = 1;
+      if (status != nullptr) atomicExch(status, 1u);
       return false;
     }
   }
   return true;
 }
+
+// Short where the wait is over already: a lone thread that feeds the tensor core
+// pays for every instruction between two products.
+template <bool kCluster = false>
+__device__ __forceinline__ bool wait(std::uint32_t bar, unsigned parity, const Bound& b) {
+  if (try_wait<kCluster>(bar, parity)) return true;
+  return wait_longer<kCluster>(bar, parity, b.gave_up, b.status, b.limit_ns);
+}
+
+__device__ __forceinline__ void arrive(std::uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void init(std::uint32_t bar, unsigned count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void expect_tx(std::uint32_t bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void load_2d(std::uint32_t dst, const CUtensorMap* map, int x, int y, std::uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<std::uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void load_3d(std::uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                        std::uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<std::uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+// A last wait, for what is in flight after another wait gave up.
+__device__ __forceinline__ void settle(std::uint32_t bar, unsigned parity, std::uint64_t limit_ns) {
+  for (const std::uint64_t t0 = gtimer(); !try_wait<false>(bar, parity) && gtimer() - t0 <= limit_ns;) {
+  }
+}
+
+// True in one lane of the warp.
+__device__ __forceinline__ bool elect() {
+  unsigned one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
+}
+
+// Place in a ring of n slots, and the parity of its round.
+struct Place {
+  unsigned slot = 0, round = 0;
+  __device__ __forceinline__ void next(unsigned n) {
+    if (++slot == n) {
+      slot = 0;
+      round ^= 1u;
+    }
+  }
+};
 
 }  // namespace async

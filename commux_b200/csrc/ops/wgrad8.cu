@@ -19,32 +19,40 @@ namespace train {
 
 namespace {
 
-// A CTA's tile of dw and its step over tokens. 256 x 256 fp32 sums fill the
-// 512 columns of tensor memory (two M = 128 halves side by side), and each
-// widened X tile feeds two products, which halves the widening per product.
-constexpr int kM = 256, kN = 256, kK = 64;
-constexpr int kStages = 3;                // dy and 8-bit tiles in flight
-constexpr int kWide = 2;                  // widened tiles
-constexpr int kBox = 64 * kK * 2;         // a 64-wide bf16 box of a step
-constexpr int kBytesA = kM * kK * 2, kBytesQ = kN * kK, kBytesB = kN * kK * 2;
-constexpr int kBytesS = kK * (kN / kGroup) * 4;  // a step's steps (scales) as floats
+// Two CTAs (a cluster, on neighbouring SMs) share a tile of dw and each product:
+// both hold 128 rows of an M = 256 half, and each widens half of the columns, so
+// an operand is brought and widened once for both. What bounds such a tile next
+// to the products is shared memory: a token's tiles are written by TMA, read and
+// written by the widening and read by the products. That is 24 cycles of 128
+// bytes for 16 cycles of products on one CTA's 256 x 256 tile (which ran at half
+// of the products' rate), and 16 for 16 here. The 2 x 256 columns of a CTA's sums
+// fill tensor memory.
+constexpr int kM = 512, kN = 256, kK = 64;    // a pair's tile, tokens of a step
+constexpr int kStages = 4;                    // dy and 8-bit tiles in flight
+constexpr int kWide = 3;                      // widened tiles
+constexpr int kDone = 12;                     // steps of which it is known whether they were read
+constexpr int kBox = 64 * kK * 2;             // a 64-wide bf16 box of a step
+constexpr int kOwnN = kN / 2;                 // columns that a CTA widens, at most
+constexpr int kBytesA = kM / 2 * kK * 2, kBytesQ = kOwnN * kK, kBytesB = kOwnN * kK * 2;
+constexpr int kBytesS = kK * (kOwnN / kGroup) * 4;  // a step's scales as pairs of bf16
 constexpr int kOffQ = kStages * kBytesA, kOffB = kOffQ + kStages * kBytesQ, kOffS = kOffB + kWide * kBytesB;
 constexpr int kOffBars = kOffS + kStages * kBytesS;
-constexpr int kSmem = kOffBars + 256 + 1024;  // and room to align
-constexpr int kConvert = 8;               // widening warps, which also write the results
-constexpr int kColumn = 4;                // warps that sum dy's columns
-constexpr int kScale = 2;                 // warps that fetch scales, a lane to a token
+constexpr int kBarBytes = 512;
+constexpr int kSmem = kOffBars + kBarBytes + 1024;  // and room to align
+constexpr int kConvert = 8;                   // widening warps, which also write the results
+constexpr int kColumn = 4;                    // warps that sum dy's columns
+constexpr int kScale = kK / 32;               // warps that fetch scales, a lane to a token
 constexpr int kThreads = 32 * (2 + kConvert + kColumn + kScale);
-constexpr int kSlot = kM * kN + kM;       // floats of a partial tile: sums, then db
+constexpr int kSlot = kM * kN + kM;           // floats of a partial tile: sums, then db
 
-// Steps of all tiles in a row are dealt out evenly to the CTAs: a CTA's range
-// may begin and end inside a tile. A tile that one CTA holds whole is written
+// Steps of all tiles in a row are dealt out evenly to the pairs: a pair's range
+// may begin and end inside a tile. A tile that one pair holds whole is written
 // at once, the others' parts go to slots that wgrad_join adds up in order.
 struct Plan {
   std::int64_t rows, cols, outs, groups;
-  int tiles_n, tiles, steps, ctas, planes;
-  __host__ __device__ std::int64_t begin(int cta) const {
-    return static_cast<std::int64_t>(tiles) * steps * cta / ctas;
+  int tiles_n, tiles, steps, pairs, planes;
+  __host__ __device__ std::int64_t begin(int pair) const {
+    return static_cast<std::int64_t>(tiles) * steps * pair / pairs;
   }
 };
 
@@ -63,42 +71,75 @@ __device__ __forceinline__ void write_dw(const Plan& p, const Out& out, std::int
   store(out.dw, out.dwt, o * p.cols + i, v);
 }
 
-// Two neighbouring bytes (of u = q + 128) times the step, as two bf16. A byte
-// in the low bits of 2^23's mantissa is 2^23 + u; less 2^23 + 128 that is q,
-// and q s has its low 16 bits clear, so its upper half is the bf16.
-__device__ __forceinline__ unsigned widen2(unsigned word, int at, float2 step) {
-  const unsigned sel = 0x7540u + static_cast<unsigned>(at);
-  const float2 u = {__uint_as_float(__byte_perm(word, 0x4b000000u, sel)),
-                    __uint_as_float(__byte_perm(word, 0x4b000000u, sel + 1))};
-  const float2 v = mul2(add2(u, both(-8388736.0f)), step);
-  return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
+// Two neighbouring values times their step, as two bf16. In bf16, 0x4300 and the
+// low 7 bits of q are 128 + (q mod 128), 0x4300 and its sign bit are 128 or 256;
+// the difference is q, and a power of two times it is exact.
+__device__ __forceinline__ unsigned widen2(unsigned word, unsigned at, __nv_bfloat162 step) {
+  const unsigned p = __byte_perm(word, 0x43434343u, at), low = p & 0xff7fff7fu, sign = p & 0xff80ff80u;
+  const __nv_bfloat162 q = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&low),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&sign));
+  const __nv_bfloat162 v = __hmul2(q, step);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+
+// A scale byte's step as a pair of bf16.
+__device__ __forceinline__ unsigned step_pair(unsigned e) {
+  const unsigned s = e == 255u ? 0x7fffu : e << 7;
+  return s << 16 | s;
 }
 
 // Both operands have their M or N elements adjacent: blocks of 64 elements
 // (128-byte rows, one for each token, 128-byte swizzle), kBox bytes from one
-// block to the next, 1024 bytes from 8 tokens to the next 8.
-__device__ __forceinline__ std::uint64_t operand(std::uint32_t smem) {
-  return static_cast<std::uint64_t>((smem & 0x3ffffu) >> 4) | static_cast<std::uint64_t>(kBox >> 4) << 16 |
-         static_cast<std::uint64_t>(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// block to the next, 1024 bytes from 8 tokens to the next 8. The low word of a
+// descriptor holds the address and the first distance, the high word the rest.
+__device__ __forceinline__ unsigned operand(std::uint32_t smem) {
+  return (smem & 0x3ffffu) >> 4 | static_cast<unsigned>(kBox >> 4) << 16;
 }
+constexpr unsigned kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
 
-// fp32 sums of bf16 products, both operands M/N-major, M = 128
+// fp32 sums of bf16 products, both operands M/N-major, M = 256 over the pair
 __device__ __forceinline__ unsigned mma_form(int n) {
-  return 1u << 4 | 1u << 7 | 1u << 10 | 1u << 15 | 1u << 16 | static_cast<unsigned>(n >> 3) << 17 | (128u >> 4) << 24;
+  return 1u << 4 | 1u << 7 | 1u << 10 | 1u << 15 | 1u << 16 | static_cast<unsigned>(n >> 3) << 17 | (256u >> 4) << 24;
 }
 
-__device__ __forceinline__ void mma(std::uint32_t d, std::uint64_t a, std::uint64_t b, unsigned form, bool add) {
+__device__ __forceinline__ void mma(std::uint32_t d, unsigned a, unsigned b, unsigned form, unsigned add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(form), "r"(static_cast<unsigned>(add))
+      "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.u32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(form), "r"(add), "r"(kOperandHigh)
       : "memory");
 }
 
-__device__ __forceinline__ void commit(std::uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   async::smem_u32(bar))
-               : "memory");
+// One half's products of a step; `add` 0: the first of them begins the sums.
+__device__ __forceinline__ void mma_step(std::uint32_t d, unsigned a, unsigned b, unsigned form, unsigned add) {
+  mma(d, a, b, form, add);
+#pragma unroll
+  for (int kk = 1; kk < kK / 16; ++kk) mma(d, a + kk * (2048 >> 4), b + kk * (2048 >> 4), form, 1);  // 16 tokens on
+}
+
+// Arrives on this barrier in both CTAs once the products issued so far are done.
+__device__ __forceinline__ void commit(std::uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<std::uint16_t>(3))
+      : "memory");
+}
+
+__device__ __forceinline__ void sync_pair() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// The address of CTA 0's copy of a barrier, and an arrival there. What this CTA's
+// threads wrote to its shared memory for the products has passed a proxy fence
+// before; a release over the cluster would also wait for every result on its way
+// to memory.
+__device__ __forceinline__ std::uint32_t leaders(std::uint32_t bar) {
+  std::uint32_t there;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(bar));
+  return there;
+}
+__device__ __forceinline__ void arrive_there(std::uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void load_sums(float (&v)[32], std::uint32_t at) {
@@ -116,10 +157,10 @@ __device__ __forceinline__ void load_sums(float (&v)[32], std::uint32_t at) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-struct Segment {  // a CTA's part of a tile
+struct Segment {  // a pair's part of a tile
   int tile, first, last;  // steps [first, last)
   bool whole, head;
-  int m0, n0, halves, boxes, n;
+  int m0, n0, halves, n;  // n: columns of the products, a multiple of 64
 };
 
 __device__ __forceinline__ Segment segment(const Plan& p, std::int64_t at, std::int64_t begin, std::int64_t end) {
@@ -132,237 +173,310 @@ __device__ __forceinline__ Segment segment(const Plan& p, std::int64_t at, std::
   s.head = at == begin;
   s.m0 = s.tile / p.tiles_n * kM;
   s.n0 = s.tile % p.tiles_n * kN;
-  const std::int64_t m = p.outs - s.m0, n = p.cols - s.n0;
-  s.boxes = m >= kM ? kM / 64 : static_cast<int>((m + 63) / 64);
-  s.halves = s.boxes > 2 ? 2 : 1;
-  s.n = n >= kN ? kN : static_cast<int>((n + 15) / 16 * 16);
+  const std::int64_t n = p.cols - s.n0;
+  s.halves = p.outs - s.m0 > kM / 2 ? 2 : 1;
+  s.n = n >= kN ? kN : static_cast<int>((n + 63) / 64 * 64);
   return s;
 }
 
-__global__ void __launch_bounds__(kThreads, 1)
+// Row of the tile of a CTA's local row (0 to 255): 128 of each half
+__device__ __forceinline__ int tile_row(int local, int rank) { return (local >> 7) * 256 + rank * 128 + (local & 127); }
+
+// kOne: dy is one bf16 term. Then a step has one dy tile, and one barrier tells
+// the products that everything of a step is there and another that it was read:
+// the thread that issues the products is the narrowest place of the kernel (it
+// cost twice the products' time with a wait for each tile).
+template <bool kOne>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     wgrad_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_q, const Plan p,
                 const Out out, const std::uint8_t* scale, unsigned* status, std::uint64_t limit_ns) {
   extern __shared__ unsigned char raw[];
   unsigned char* smem = raw + ((1024u - (async::smem_u32(raw) & 1023u)) & 1023u);
-  std::uint64_t* bars = reinterpret_cast<std::uint64_t*>(smem + kOffBars);
-  std::uint64_t *full_a = bars, *empty_a = bars + 3, *full_q = bars + 6, *empty_q = bars + 9, *full_b = bars + 12,
-                *empty_b = bars + 14, *sums_full = bars + 16, *sums_empty = bars + 17, *column_full = bars + 18,
-                *drained = bars + 19;
-  std::uint32_t* tmem_at = reinterpret_cast<std::uint32_t*>(bars + 20);
-  volatile int* gave_up = reinterpret_cast<volatile int*>(bars + 21);
-  __shared__ float column[kM];
+  // Barriers, by their addresses. In both CTAs: tiles of its own, widened tiles
+  // that were read, results. Used in CTA 0, which issues the products: peer_a (the
+  // other CTA's dy tiles are there), full_b (both have widened), sums_empty (both
+  // have the results). With kOne, done replaces empty_b and the products' part of
+  // empty_a, and full_b includes dy's tiles.
+  const std::uint32_t base = async::smem_u32(smem), bars = base + kOffBars;
+  const std::uint32_t full_a = bars, empty_a = full_a + 8 * kStages, full_q = empty_a + 8 * kStages,
+                      empty_q = full_q + 8 * kStages, peer_a = empty_q + 8 * kStages, full_b = peer_a + 8 * kStages,
+                      empty_b = full_b + 8 * kWide, sums_full = empty_b + 8 * kWide, sums_empty = sums_full + 8,
+                      turned = sums_full + 16, column_full = sums_full + 24, drained = sums_full + 32,
+                      done = sums_full + 40;
+  constexpr int kAfter = kOffBars + 8 * (5 * kStages + 2 * kWide + 5 + kDone);
+  std::uint32_t* tmem_at = reinterpret_cast<std::uint32_t*>(smem + kAfter);
+  volatile int* gave_up = reinterpret_cast<volatile int*>(smem + kAfter + 8);
+  static_assert((5 * kStages + 2 * kWide + 7 + kDone) * 8 <= kBarBytes, "barriers");
+  static_assert(kConvert * 32 * 32 * 4 <= kWide * kBytesB, "the results are turned round in the widened tiles");
+  __shared__ float column[kM / 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pair = static_cast<int>(blockIdx.x >> 1), rank = static_cast<int>(blockIdx.x & 1);
   const async::Bound bound{gave_up, status, limit_ns};
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      async::mbar_init(&full_a[s], 1);
-      async::mbar_init(&empty_a[s], 1 + kColumn);
-      async::mbar_init(&full_q[s], 1 + kScale);
-      async::mbar_init(&empty_q[s], kConvert);
+      async::init(full_a + 8 * s, 1);
+      async::init(empty_a + 8 * s, (kOne ? 0 : 1) + kColumn);
+      async::init(full_q + 8 * s, 1 + kScale);
+      async::init(empty_q + 8 * s, kConvert);
+      async::init(peer_a + 8 * s, 1);
     }
     for (int s = 0; s < kWide; ++s) {
-      async::mbar_init(&full_b[s], kConvert);
-      async::mbar_init(&empty_b[s], 1);
+      async::init(full_b + 8 * s, 2 * kConvert);
+      async::init(empty_b + 8 * s, 1);
     }
-    async::mbar_init(sums_full, 1);
-    async::mbar_init(sums_empty, kConvert);
-    async::mbar_init(column_full, kColumn);
-    async::mbar_init(drained, 1);
+    async::init(sums_full, 1);
+    async::init(sums_empty, 2 * kConvert);
+    async::init(turned, kConvert);
+    async::init(column_full, kColumn);
+    async::init(drained, 1);
+    for (int s = 0; s < kDone; ++s) async::init(done + 8 * s, 1);
     *gave_up = 0;
     async::fence_async();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(async::smem_u32(tmem_at))
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(async::smem_u32(tmem_at))
                  : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  sync_pair();  // both CTAs have their barriers and their tensor memory
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const std::uint32_t tmem = *tmem_at;
 
-  const std::int64_t begin = p.begin(blockIdx.x), end = p.begin(blockIdx.x + 1);
+  const std::int64_t begin = p.begin(pair), end = p.begin(pair + 1);
   // db of a tile's rows: wanted by the tiles of the first column block, and by
   // all where the norm's bias multiplies it
   auto sums_columns = [&](const Segment& s) { return out.b != nullptr || (out.db != nullptr && s.n0 == 0); };
 
   if (warp == 0) {  // --- loads
-    if (lane == 0) {
-      unsigned ia = 0, iq = 0;
-      bool ok = true;
-      for (std::int64_t at = begin; ok && at < end;) {
-        const Segment s = segment(p, at, begin, end);
-        for (int k = s.first; ok && k < s.last; ++k) {
-          const int t0 = k * kK;
-          unsigned st = iq % kStages;
-          ok = async::bounded_wait(&empty_q[st], iq / kStages & 1u ^ 1u, bound);
-          if (!ok) break;
-          async::mbar_expect_tx(&full_q[st], kBytesQ);
-          async::tma_load_2d(smem + kOffQ + st * kBytesQ, &map_q, s.n0, t0, &full_q[st]);
-          ++iq;
-          for (int pl = 0; pl < p.planes; ++pl) {
-            st = ia % kStages;
-            ok = async::bounded_wait(&empty_a[st], ia / kStages & 1u ^ 1u, bound);
-            if (!ok) break;
-            async::mbar_expect_tx(&full_a[st], s.boxes * kBox);
-            for (int b = 0; b < s.boxes; ++b)
-              async::tma_load_3d(smem + st * kBytesA + b * kBox, &map_a, s.m0 + 64 * b, t0, pl, &full_a[st]);
-            ++ia;
-          }
-        }
-        at += s.last - s.first;
+    // All lanes go through the loop and one issues, here and for the products: the
+    // addresses then stay in the warp's uniform registers.
+    const bool chosen = async::elect();
+    async::Place ia, iq, freed;  // freed: the step whose read frees this one's dy tile
+    std::int64_t loaded_a = 0, loaded_q = 0;
+    bool ok = true;
+    for (std::int64_t at = begin; ok && at < end;) {
+      const Segment s = segment(p, at, begin, end);
+      const int n0 = s.n0 + rank * (s.n / 2);
+      // boxes that hold rows of dw; what the others' memory holds meets only sums
+      // that are not written
+      int m[4], boxes = 0;
+      for (int b = 0; b < 4; ++b) {
+        m[b] = s.m0 + tile_row(64 * b, rank);
+        boxes += m[b] < p.outs;
       }
-      // the CTA's shared memory outlives the copies also where a wait gave up
-      for (unsigned i = ia > kStages ? ia - kStages : 0; !ok && i < ia; ++i)
-        async::mbar_wait(&full_a[i % kStages], i / kStages & 1u, limit_ns);
-      for (unsigned i = iq > kStages ? iq - kStages : 0; !ok && i < iq; ++i)
-        async::mbar_wait(&full_q[i % kStages], i / kStages & 1u, limit_ns);
+      for (int k = s.first; ok && k < s.last; ++k) {
+        ok = __all_sync(0xffffffffu, async::wait(empty_q + 8 * iq.slot, iq.round ^ 1u, bound));
+        if (!ok) break;
+        if (chosen) {
+          async::expect_tx(full_q + 8 * iq.slot, kBytesQ);
+          async::load_2d(base + kOffQ + iq.slot * kBytesQ, &map_q, n0, k * kK, full_q + 8 * iq.slot);
+        }
+        iq.next(kStages);
+        ++loaded_q;
+        for (int pl = 0; pl < (kOne ? 1 : p.planes); ++pl) {
+          ok = async::wait(empty_a + 8 * ia.slot, ia.round ^ 1u, bound);
+          if (kOne && loaded_a >= kStages) {
+            ok = ok && async::wait(done + 8 * freed.slot, freed.round, bound);
+            freed.next(kDone);
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (chosen) {
+            async::expect_tx(full_a + 8 * ia.slot, boxes * kBox);
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              if (m[b] < p.outs)
+                async::load_3d(base + ia.slot * kBytesA + b * kBox, &map_a, m[b], k * kK, pl, full_a + 8 * ia.slot);
+          }
+          ia.next(kStages);
+          ++loaded_a;
+        }
+      }
+      at += s.last - s.first;
+    }
+    // the CTA's shared memory outlives the copies also where a wait gave up
+    for (std::int64_t i = loaded_a > kStages ? loaded_a - kStages : 0; !ok && i < loaded_a; ++i)
+      async::settle(full_a + 8 * static_cast<unsigned>(i % kStages), static_cast<unsigned>(i / kStages) & 1u, limit_ns);
+    for (std::int64_t i = loaded_q > kStages ? loaded_q - kStages : 0; !ok && i < loaded_q; ++i)
+      async::settle(full_q + 8 * static_cast<unsigned>(i % kStages), static_cast<unsigned>(i / kStages) & 1u, limit_ns);
+  } else if (warp == 1 && rank == 1) {  // --- tells CTA 0 of this CTA's dy tiles
+    if (!kOne && lane == 0) {
+      const std::uint32_t there = leaders(peer_a);
+      async::Place ia;
+      for (std::int64_t n = (end - begin) * p.planes; n > 0; --n) {
+        if (!async::wait(full_a + 8 * ia.slot, ia.round, bound)) break;
+        arrive_there(there + 8 * ia.slot);
+        ia.next(kStages);
+      }
     }
   } else if (warp == 1) {  // --- products
-    if (lane == 0) {
-      unsigned ia = 0, ib = 0, seg = 0;
-      bool ok = true;
-      for (std::int64_t at = begin; ok && at < end; ++seg) {
-        const Segment s = segment(p, at, begin, end);
-        const unsigned form = mma_form(s.n);
-        ok = async::bounded_wait(sums_empty, seg & 1u ^ 1u, bound);
-        for (int k = s.first; ok && k < s.last; ++k) {
-          const unsigned sb = ib % kWide;
-          ok = async::bounded_wait(&full_b[sb], ib / kWide & 1u, bound);
-          for (int pl = 0; ok && pl < p.planes; ++pl) {
-            const unsigned sa = ia % kStages;
-            ok = async::bounded_wait(&full_a[sa], ia / kStages & 1u, bound);
+    const bool chosen = async::elect();
+    async::Place ia, ib, steps;
+    unsigned seg = 0;
+    bool ok = true;
+    const unsigned a0 = operand(base), b0 = operand(base + kOffB);
+    for (std::int64_t at = begin; ok && at < end; ++seg) {
+      const Segment s = segment(p, at, begin, end);
+      const unsigned form = mma_form(s.n);
+      ok = async::wait<true>(sums_empty, seg & 1u ^ 1u, bound);
+      unsigned add = 0;
+      for (int k = s.first; ok && k < s.last; ++k) {
+        ok = __all_sync(0xffffffffu, async::wait<true>(full_b + 8 * ib.slot, ib.round, bound));
+        const unsigned b = b0 + ib.slot * (kBytesB >> 4);
+        for (int pl = 0; ok && pl < (kOne ? 1 : p.planes); ++pl) {
+          if (!kOne) {
+            ok = async::wait(full_a + 8 * ia.slot, ia.round, bound) &&
+                 async::wait<true>(peer_a + 8 * ia.slot, ia.round, bound);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const std::uint64_t a = operand(async::smem_u32(smem + sa * kBytesA));
-            const std::uint64_t b = operand(async::smem_u32(smem + kOffB + sb * kBytesB));
-            for (int h = 0; h < s.halves; ++h)
-#pragma unroll
-              for (int kk = 0; kk < kK / 16; ++kk)  // 16 tokens are 2048 bytes of every block
-                mma(tmem + h * kN, a + (h * 2 * kBox + kk * 2048 >> 4), b + (kk * 2048 >> 4), form,
-                    k != s.first || pl != 0 || kk != 0);
-            commit(&empty_a[sa]);
-            ++ia;
           }
-          if (ok) commit(&empty_b[sb]);
-          ++ib;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const unsigned a = a0 + ia.slot * (kBytesA >> 4);
+          if (chosen) {
+            mma_step(tmem, a, b, form, add);
+            if (s.halves == 2) mma_step(tmem + kN, a + (2 * kBox >> 4), b, form, add);
+            if (!kOne) commit(empty_a + 8 * ia.slot);
+          }
+          add = 1;
+          ia.next(kStages);
         }
-        if (ok) commit(sums_full);
-        at += s.last - s.first;
+        if (ok && chosen) commit(kOne ? done + 8 * steps.slot : empty_b + 8 * ib.slot);
+        ib.next(kWide);
+        steps.next(kDone);
       }
-      if (!ok) {  // products in flight read shared memory and write tensor memory
-        commit(drained);
-        async::mbar_wait(drained, 0, limit_ns);
-      }
+      if (ok && chosen) commit(sums_full);
+      at += s.last - s.first;
+    }
+    if (!ok) {  // products in flight read shared memory and write tensor memory
+      if (chosen) commit(drained);
+      async::settle(drained, 0, limit_ns);
     }
   } else if (warp < 2 + kConvert) {  // --- widening, and the results
-    const int cw = warp - 2, unit = lane & 15, row0 = cw * 2 + (lane >> 4);
-    const int block = unit >> 2, odd = block & 1;
-    unsigned i = 0, seg = 0;
+    // A warp takes two tokens' 128 columns at a time, a lane 8 of them: 8 bytes
+    // in, one 16-byte column of a swizzled row out, both without bank conflicts.
+    const int cw = warp - 2, in = lane & 15, block = in >> 3, unit = in & 7, row0 = cw * 2 + (lane >> 4);
+    const std::uint32_t leaders_b = leaders(full_b), leaders_sums = leaders(sums_empty);
+    async::Place iq, ib, freed;
+    unsigned seg = 0, widened = 0;
     bool ok = true;
     for (std::int64_t at = begin; ok && at < end; ++seg) {
       const Segment s = segment(p, at, begin, end);
-      const bool busy = unit * 16 < s.n;
-      for (int k = s.first; k < s.last; ++k, ++i) {
-        const unsigned sq = i % kStages, sb = i % kWide;
-        ok = async::bounded_wait(&full_q[sq], i / kStages & 1u, bound) &&
-             async::bounded_wait(&empty_b[sb], i / kWide & 1u ^ 1u, bound);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
+      const bool busy = in * 8 < s.n / 2;
+      for (int k = s.first; k < s.last; ++k) {
+        ok = async::wait(full_q + 8 * iq.slot, iq.round, bound);
+        if (!kOne) {
+          ok = ok && async::wait(empty_b + 8 * ib.slot, ib.round ^ 1u, bound);
+        } else if (widened < kWide) {
+          ++widened;
+        } else {
+          ok = ok && async::wait(done + 8 * freed.slot, freed.round, bound);
+          freed.next(kDone);
         }
-        const unsigned char* from = smem + kOffQ + sq * kBytesQ;
-        const float* steps = reinterpret_cast<const float*>(smem + kOffS + sq * kBytesS) + (unit >> 1);
-        unsigned char* to = smem + kOffB + sb * kBytesB + block * kBox;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const unsigned char* from = smem + kOffQ + iq.slot * kBytesQ + in * 8;
+        const unsigned* steps = reinterpret_cast<const unsigned*>(smem + kOffS + iq.slot * kBytesS) + (in >> 2);
+        unsigned char* to = smem + kOffB + ib.slot * kBytesB + block * kBox;
         if (busy) {
+          constexpr int kTurns = kK / (2 * kConvert);
+          uint2 v[kTurns];
+          unsigned two[kTurns];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = j * 16 + row0;
-            uint4 v = *reinterpret_cast<const uint4*>(from + r * kN + unit * 16);
-            v.x ^= 0x80808080u, v.y ^= 0x80808080u, v.z ^= 0x80808080u, v.w ^= 0x80808080u;
-            const float2 step = both(steps[r * (kN / kGroup)]);
-            const uint4 lo = {widen2(v.x, 0, step), widen2(v.x, 2, step), widen2(v.y, 0, step), widen2(v.y, 2, step)};
-            const uint4 hi = {widen2(v.z, 0, step), widen2(v.z, 2, step), widen2(v.w, 0, step), widen2(v.w, 2, step)};
-            // odd blocks write their halves the other way round: the 8 lanes of
-            // a store then meet 8 different 16-byte columns of the banks
-            const int u = (unit & 3) * 2;
-            unsigned char* row = to + r * 128;
-            *reinterpret_cast<uint4*>(row + (((u + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
-            *reinterpret_cast<uint4*>(row + (((u + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
+          for (int j = 0; j < kTurns; ++j) {
+            const int r = j * 2 * kConvert + row0;
+            v[j] = *reinterpret_cast<const uint2*>(from + r * kOwnN);
+            two[j] = steps[r * (kOwnN / kGroup)];
+          }
+#pragma unroll
+          for (int j = 0; j < kTurns; ++j) {
+            const int r = j * 2 * kConvert + row0;
+            const __nv_bfloat162 step = *reinterpret_cast<const __nv_bfloat162*>(&two[j]);
+            *reinterpret_cast<uint4*>(to + r * 128 + ((unit ^ (r & 7)) << 4)) =
+                uint4{widen2(v[j].x, 0x4140u, step), widen2(v[j].x, 0x4342u, step), widen2(v[j].y, 0x4140u, step),
+                      widen2(v[j].y, 0x4342u, step)};
           }
         }
         async::fence_async();
         __syncwarp();
         if (lane == 0) {
-          async::mbar_arrive(&empty_q[sq]);
-          async::mbar_arrive(&full_b[sb]);
+          async::arrive(empty_q + 8 * iq.slot);
+          // one warp's arrival stands for dy's tile too; its places are the 8-bit
+          // tile's. The others have arrived long before.
+          if (kOne && cw == 0) ok = async::wait(full_a + 8 * iq.slot, iq.round, bound);
+          if (ok) arrive_there(leaders_b + 8 * ib.slot);
         }
+        if (kOne) ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        iq.next(kStages);
+        ib.next(kWide);
       }
       if (!ok) break;
-      ok = async::bounded_wait(sums_full, seg & 1u, bound) && async::bounded_wait(column_full, seg & 1u, bound);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
+      ok = async::wait(sums_full, seg & 1u, bound) && async::wait(column_full, seg & 1u, bound);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      // A warp reads the lanes (rows) of its quarter; a block of 32 x 32 is
-      // turned round in the widened tiles' memory, which nothing reads now, so
-      // that every store is one row of 32 neighbours.
+      // A warp reads the lanes (rows) of its quarter; a block of 32 x 32 is turned
+      // round in the widened tiles' memory, which nothing reads now, so that every
+      // store is one row of 32 neighbours.
       const int quarter = warp & 3, h = cw >> 2;
-      float* turn = reinterpret_cast<float*>(smem + kOffB) + cw * 32 * 33;
-      const int rows0 = h * 128 + quarter * 32;
-      float* slot = out.slots + (2 * static_cast<std::int64_t>(blockIdx.x) + (s.head ? 0 : 1)) * kSlot;
+      float* turn = reinterpret_cast<float*>(smem + kOffB) + cw * 32 * 32;
+      const int local0 = h * 128 + quarter * 32, rows0 = tile_row(local0, rank);
+      float* slot = out.slots + (2 * static_cast<std::int64_t>(pair) + (s.head ? 0 : 1)) * kSlot;
       if (h < s.halves) {
         for (int c = 0; c * 32 < s.n; ++c) {
           float v[32];
           load_sums(v, tmem + (static_cast<std::uint32_t>(quarter * 32) << 16) + h * kN + c * 32);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = v[j];
+          for (int j = 0; j < 32; ++j) turn[lane * 32 + (j ^ lane)] = v[j];
           __syncwarp();
           const std::int64_t i0 = s.n0 + c * 32 + lane;
           if (s.whole) {
             for (int r = 0; r < 32; ++r) {
               const std::int64_t o = s.m0 + rows0 + r;
-              if (o < p.outs && i0 < p.cols) write_dw(p, out, o, i0, turn[r * 33 + lane], column[rows0 + r]);
+              if (o < p.outs && i0 < p.cols) write_dw(p, out, o, i0, turn[r * 32 + (lane ^ r)], column[local0 + r]);
             }
           } else {
 #pragma unroll 8
-            for (int r = 0; r < 32; ++r) slot[(rows0 + r) * kN + c * 32 + lane] = turn[r * 33 + lane];
+            for (int r = 0; r < 32; ++r) slot[(rows0 + r) * kN + c * 32 + lane] = turn[r * 32 + (lane ^ r)];
           }
           __syncwarp();
         }
         if ((s.whole ? s.n0 == 0 && out.db != nullptr : true) && sums_columns(s)) {
           const std::int64_t o = s.m0 + rows0 + lane;
           if (!s.whole)
-            slot[kM * kN + rows0 + lane] = column[rows0 + lane];
+            slot[kM * kN + rows0 + lane] = column[local0 + lane];
           else if (o < p.outs)
-            store(out.db, out.dwt, o, column[rows0 + lane]);
+            store(out.db, out.dwt, o, column[local0 + lane]);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) async::mbar_arrive(sums_empty);
+      if (lane == 0) {
+        async::arrive(turned);
+        arrive_there(leaders_sums);
+      }
       at += s.last - s.first;
       // every warp has read its `turn` before any widens the next tile
-      ok = async::bounded_wait(sums_empty, seg & 1u, bound);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = __all_sync(0xffffffffu, async::wait(turned, seg & 1u, bound));
     }
   } else if (warp >= 2 + kConvert + kColumn) {  // --- scales
-    // They are bytes at any alignment, which TMA cannot fetch; the widening warps
-    // spent more than half of their time on waiting for their own loads of them.
-    // Two steps are on their way while one is written.
+    // They are bytes at any alignment, which TMA cannot fetch. Two steps are on
+    // their way while one is written.
     const int token = (warp - 2 - kConvert - kColumn) * 32 + lane;
-    constexpr int kEach = kN / kGroup;
-    unsigned i = 0;
+    constexpr int kEach = kOwnN / kGroup;
+    async::Place iq;
     bool ok = true;
     for (std::int64_t at = begin; ok && at < end;) {
       const Segment s = segment(p, at, begin, end);
-      const int some = static_cast<int>(p.groups - s.n0 / kGroup < kEach ? p.groups - s.n0 / kGroup : kEach);
+      const std::int64_t group = (s.n0 + rank * (s.n / 2)) / kGroup, left = p.groups - group;
+      const int some = static_cast<int>(left < kEach ? left : kEach);
       unsigned ahead[2][kEach];
       auto fetch = [&](int k, unsigned (&e)[kEach]) {
         const std::int64_t t = static_cast<std::int64_t>(k) * kK + token;
-        const std::uint8_t* from = scale + t * p.groups + s.n0 / kGroup;
+        const std::uint8_t* from = scale + t * p.groups + group;
         const bool in = k < s.last && t < p.rows;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
@@ -373,17 +487,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       fetch(s.first, ahead[0]);
       fetch(s.first + 1, ahead[1]);
       auto put = [&](int k, unsigned (&e)[kEach]) {
-        const unsigned sq = i % kStages;
-        ok = async::bounded_wait(&empty_q[sq], i / kStages & 1u ^ 1u, bound);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = __all_sync(0xffffffffu, async::wait(empty_q + 8 * iq.slot, iq.round ^ 1u, bound));
         if (!ok) return;
-        float4* to = reinterpret_cast<float4*>(smem + kOffS + sq * kBytesS) + token * (kEach / 4);
-        to[0] = float4{step_of(e[0]), step_of(e[1]), step_of(e[2]), step_of(e[3])};
-        to[1] = float4{step_of(e[4]), step_of(e[5]), step_of(e[6]), step_of(e[7])};
+        static_assert(kEach == 4, "a token's scales are one vector");
+        reinterpret_cast<uint4*>(smem + kOffS + iq.slot * kBytesS)[token] =
+            uint4{step_pair(e[0]), step_pair(e[1]), step_pair(e[2]), step_pair(e[3])};
         fetch(k + 2, e);
         __syncwarp();
-        if (lane == 0) async::mbar_arrive(&full_q[sq]);
-        ++i;
+        if (lane == 0) async::arrive(full_q + 8 * iq.slot);
+        iq.next(kStages);
       };
       for (int k = s.first; ok && k < s.last; k += 2) {
         put(k, ahead[0]);
@@ -394,23 +506,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {  // --- sums of dy's columns
     const int c = (warp - 2 - kConvert) * 32 + lane;  // columns 2c and 2c + 1 of the tile
     const int block = c >> 5, unit = (c & 31) >> 2, in = (c & 3) * 4;
-    unsigned i = 0, seg = 0;
+    async::Place ia;
+    unsigned seg = 0;
     bool ok = true;
     for (std::int64_t at = begin; ok && at < end; ++seg) {
       const Segment s = segment(p, at, begin, end);
-      const bool busy = sums_columns(s) && block < s.boxes;
+      const bool busy = sums_columns(s) && s.m0 + tile_row(64 * block, rank) < p.outs;
       float v0 = 0.0f, v1 = 0.0f;
-      for (std::int64_t k = static_cast<std::int64_t>(s.last - s.first) * p.planes; k > 0; --k, ++i) {
-        const unsigned sa = i % kStages;
-        ok = async::bounded_wait(&full_a[sa], i / kStages & 1u, bound);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+      for (std::int64_t k = static_cast<std::int64_t>(s.last - s.first) * p.planes; k > 0; --k) {
+        ok = __all_sync(0xffffffffu, async::wait(full_a + 8 * ia.slot, ia.round, bound));
+        if (!ok) break;
         if (busy) {
           // a step's 64 tokens are added up first: a sum over many tokens then
           // has one rounding of its own size for each step, not for each token
-          const unsigned char* from = smem + sa * kBytesA + block * kBox + in;
+          const unsigned char* from = smem + ia.slot * kBytesA + block * kBox + in;
           float a0 = 0.0f, a1 = 0.0f;
 #pragma unroll 16
           for (int t = 0; t < kK; ++t) {
@@ -422,26 +531,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           v1 += a1;
         }
         __syncwarp();
-        if (lane == 0) async::mbar_arrive(&empty_a[sa]);
+        if (lane == 0) async::arrive(empty_a + 8 * ia.slot);
+        ia.next(kStages);
       }
       // the last tile's sums have been read once its results are out
-      ok = ok && async::bounded_wait(sums_empty, seg & 1u ^ 1u, bound);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      ok = __all_sync(0xffffffffu, ok && async::wait(turned, seg & 1u ^ 1u, bound));
+      if (!ok) break;
       column[2 * c] = v0;
       column[2 * c + 1] = v1;
       __syncwarp();
-      if (lane == 0) async::mbar_arrive(column_full);
+      if (lane == 0) async::arrive(column_full);
       at += s.last - s.first;
     }
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  sync_pair();  // neither CTA's memory is in use by the other
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// Tiles whose steps several CTAs shared: their parts in the order of the steps.
+// Tiles whose steps several pairs shared: their parts in the order of the steps.
 // A block takes kJoinRows rows of a tile, a thread four neighbours of a few rows.
 constexpr int kJoinRows = 16;
 constexpr int kJoinThreads = 256;
@@ -452,13 +563,13 @@ __global__ void __launch_bounds__(kJoinThreads) wgrad_join(const Plan p, const O
   if (m0 + r0 >= p.outs) return;
   if (threadIdx.x == 0) {
     const std::int64_t lo = static_cast<std::int64_t>(tile) * p.steps, hi = lo + p.steps;
-    int c = static_cast<int>(lo * p.ctas / (static_cast<std::int64_t>(p.tiles) * p.steps));
+    int c = static_cast<int>(lo * p.pairs / (static_cast<std::int64_t>(p.tiles) * p.steps));
     while (p.begin(c + 1) <= lo) ++c;  // the quotient rounds down twice
-    // the first part is a CTA's last one unless the CTA begins with it; every
-    // later part is its CTA's first
+    // the first part is a pair's last one unless the pair begins with it; every
+    // later part is its pair's first
     first_slot = 2 * c + (p.begin(c) >= lo ? 0 : 1);
     int n = 1;
-    while (p.begin(c + n) < hi && c + n < p.ctas) ++n;
+    while (p.begin(c + n) < hi && c + n < p.pairs) ++n;
     parts = n;
   }
   __syncthreads();
@@ -557,19 +668,21 @@ Plan plan_of(const Wgrad8& a) {
   p.tiles = static_cast<int>((a.outs + kM - 1) / kM) * p.tiles_n;
   p.steps = static_cast<int>((a.rows + kK - 1) / kK);
   // One CTA an SM. Where whole shares of the tiles fill nearly all of them,
-  // every CTA has one part of one tile; otherwise parts may cross tiles. No
-  // tile is cut into parts under 4 steps, which cost about what a CTA's start
+  // every pair has one part of one tile; otherwise parts may cross tiles. No
+  // tile is cut into parts under 4 steps, which cost about what a pair's start
   // and end do.
-  const int sms = sm_count();
+  const int most_pairs = sm_count() / 2;
   const std::int64_t total = static_cast<std::int64_t>(p.tiles) * p.steps;
-  std::int64_t n = p.tiles <= sms && sms / p.tiles * p.tiles * 10 >= sms * 9 ? sms / p.tiles * p.tiles : sms;
+  std::int64_t n = most_pairs;
+  if (p.tiles <= most_pairs && most_pairs / p.tiles * p.tiles * 10 >= most_pairs * 9)
+    n = most_pairs / p.tiles * p.tiles;
   const std::int64_t most = (total + 3) / 4 > p.tiles ? (total + 3) / 4 : p.tiles;
   if (n > most) n = most;
-  p.ctas = static_cast<int>(n);
+  p.pairs = static_cast<int>(n);
   return p;
 }
 
-std::int64_t slots_bytes(const Plan& p) { return 2ll * p.ctas * kSlot * static_cast<std::int64_t>(sizeof(float)); }
+std::int64_t slots_bytes(const Plan& p) { return 2ll * p.pairs * kSlot * static_cast<std::int64_t>(sizeof(float)); }
 std::int64_t terms_ld(const Wgrad8& a) { return (a.outs + 7) / 8 * 8; }
 
 }  // namespace
@@ -602,7 +715,7 @@ cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
   const cuuint32_t box_a[3] = {64, kK, 1};
   const cuuint64_t dim_q[2] = {static_cast<cuuint64_t>(p.groups) * kGroup, static_cast<cuuint64_t>(a.rows)};
   const cuuint64_t stride_q[1] = {static_cast<cuuint64_t>(p.groups) * kGroup};
-  const cuuint32_t box_q[2] = {kN, kK};
+  const cuuint32_t box_q[2] = {kOwnN, kK};
   if (encode(&map_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(dy), dim_a, stride_a, box_a, one,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
@@ -610,15 +723,16 @@ cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
-  const cudaError_t set = cudaFuncSetAttribute(wgrad_tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  const auto kernel = p.planes == 1 ? wgrad_tiles<true> : wgrad_tiles<false>;
+  const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (set != cudaSuccess) return set;
   const Out out{a.dw, a.db, a.dwt, a.w, a.b, a.wt, static_cast<float*>(a.work)};
   unsigned* status = nullptr;
   commux_ops::status_word(&status);
-  wgrad_tiles<<<p.ctas, kThreads, kSmem, stream>>>(map_a, map_q, p, out, a.scale, status, commux_ops::wait_limit_ns());
+  kernel<<<2 * p.pairs, kThreads, kSmem, stream>>>(map_a, map_q, p, out, a.scale, status, commux_ops::wait_limit_ns());
   commux_ops::g_launches++;
   bool joined = false;
-  for (int c = 1; c < p.ctas && !joined; ++c) joined = p.begin(c) % p.steps != 0;
+  for (int c = 1; c < p.pairs && !joined; ++c) joined = p.begin(c) % p.steps != 0;
   if (joined) {
     wgrad_join<<<dim3(p.tiles, kM / kJoinRows), kJoinThreads, 0, stream>>>(p, out);
     commux_ops::g_launches++;

@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
     const unsigned set = round & 1u;
     if (t == 0) async::mbar_expect_tx(&joined[set][which], kC * 4);
     if (t < kC) send(&ranks[set][which][rank], &joined[set][which], t, v);
-    async::bounded_wait(&joined[set][which], round >> 1 & 1u, bound);
+    async::wait(async::smem_u32(&joined[set][which]), round >> 1 & 1u, bound);
     return ranks[set][which][lane & (kC - 1)];
   };
   for (std::int64_t row = mine; row < a.rows; row += clusters, ++round) {
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
       uint4 w = minus_infinities<T>();
       if (k < n) {
         const unsigned slot = (used + k) % kRing;
-        async::bounded_wait(&full[slot], (used + k) / kRing & 1u, bound);
+        async::wait(async::smem_u32(&full[slot]), (used + k) / kRing & 1u, bound);
         uint4* vector = reinterpret_cast<uint4*>(ring + slot * kPiece) + t;
         const Span<E> span(k * kLong + t, shift, cols);
         if (kWhole) {
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* st
   }
   // shared memory outlives the copies, and what other blocks send, also where a wait gave up
   if (t == 0 && gave_up != 0)
-    for (unsigned n = used; n < issued; ++n) async::mbar_wait(&full[n % kRing], n / kRing & 1u, limit_ns);
+    for (unsigned n = used; n < issued; ++n) async::settle(async::smem_u32(&full[n % kRing]), n / kRing & 1u, limit_ns);
   if constexpr (kC > 1) cg::this_cluster().sync();
 }
 

@@ -82,6 +82,11 @@ struct Elem<__nv_bfloat16> {
     const __nv_bfloat162 r = __floats2bfloat162_rn(v.x, v.y);
     return *reinterpret_cast<const unsigned*>(&r);
   }
+  static __device__ __forceinline__ unsigned larger2(unsigned a, unsigned b) {  // NaN if either is
+    const __nv_bfloat162 r =
+        __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const unsigned*>(&r);
+  }
   static __device__ __forceinline__ float2 rounded2(float2 v) { return get2(put2(v)); }
 };
 template <>
@@ -91,6 +96,10 @@ struct Elem<__half> {
   static __device__ __forceinline__ float2 get2(unsigned w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
   static __device__ __forceinline__ unsigned put2(float2 v) {
     const __half2 r = __floats2half2_rn(v.x, v.y);
+    return *reinterpret_cast<const unsigned*>(&r);
+  }
+  static __device__ __forceinline__ unsigned larger2(unsigned a, unsigned b) {  // NaN if either is
+    const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const unsigned*>(&r);
   }
   static __device__ __forceinline__ float2 rounded2(float2 v) { return get2(put2(v)); }

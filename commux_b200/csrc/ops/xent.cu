@@ -7,13 +7,11 @@
 // log2(e), which such a value would overflow. A row of only -inf has no
 // softmax: its loss and gradient are NaN, as is every row with NaN or +inf.
 //
-// A row is read once and lives in the registers of its threads, 32 elements
-// each, from the maximum to the gradient. Rows up to 16 K elements have a block
-// of their own and many blocks an SM, so that some load while others compute.
-// Longer rows fill an SM's registers; there one block of 1024 threads walks
-// over rows, whose elements come through shared memory by bulk copies that run
-// ahead of it, and up to 8 blocks (a cluster) share a row that is longer still
-// or one of few.
+// A row is read once. Short rows live in the registers of a warp or a small
+// block, 32 elements a thread, from the maximum to the gradient, with many blocks
+// an SM, so that some load while others compute. Longer ones come through shared
+// memory by bulk copies that run ahead of blocks which walk over rows, and up to 8
+// blocks (a cluster) share a row that is longer still or one of few.
 
 #include <cooperative_groups.h>
 
@@ -66,10 +64,9 @@ __device__ __forceinline__ float target_logit(const Xent& a, std::int64_t row, s
 }
 
 // What is known of a row once its maximum and sum are (one thread).
-__device__ __forceinline__ void finish_row(const Xent& a, std::int64_t row, std::int64_t target, float logit, float m,
+__device__ __forceinline__ void finish_row(const Xent& a, std::int64_t row, bool ignored, float logit, float m,
                                            float s) {
-  const float loss = target != a.ignore ? logf(s) + (m - logit) : 0.0f;
-  (a.reduction == 0 ? a.loss : a.work + 1)[row] = loss;
+  (a.reduction == 0 ? a.loss : a.work + 1)[row] = ignored ? 0.0f : logf(s) + (m - logit);
   a.stats[row] = m;
   a.stats[a.rows + row] = s;
 }
@@ -96,11 +93,17 @@ struct Row {
     }
   }
 
-  __device__ __forceinline__ float max() const {
-    float m = larger(v[0].x, v[0].y);
-#pragma unroll
-    for (int i = 1; i < kEach / 2; ++i) m = larger(m, v[i].x, v[i].y);
-    return m;
+  // The largest element of a vector, NaN if it has one. 16-bit elements are
+  // compared two at a time, before they are widened.
+  static __device__ __forceinline__ float max(uint4 w) {
+    if constexpr (sizeof(T) == 4) {
+      return larger(larger(__uint_as_float(w.x), __uint_as_float(w.y)),
+                    larger(__uint_as_float(w.z), __uint_as_float(w.w)));
+    } else {
+      const unsigned m = Elem<T>::larger2(Elem<T>::larger2(w.x, w.y), Elem<T>::larger2(w.z, w.w));
+      const float2 f = Elem<T>::get2(m);
+      return larger(f.x, f.y);
+    }
   }
 
   __device__ __forceinline__ float exponentials(float m) {
@@ -132,24 +135,47 @@ __device__ __forceinline__ uint4 minus_infinities() {
   return {w, w, w, w};
 }
 
-// What is not the part's in the first and last vector of a part becomes -inf, in
-// the shared memory that this thread alone reads it from. (In registers every
-// vector of every thread would pay for the test of each element.)
+// The first and the last vector of a part, in functions of their own: inlined,
+// every vector of every thread would pay for the test of each element.
+
+// What is not the part's becomes -inf.
 template <typename T>
-__device__ __forceinline__ void blank(uint4* vector, Span<Row<T>::E> s) {
-  T* v = reinterpret_cast<T*>(vector);
-#pragma unroll 1
-  for (int i = 0; i < Row<T>::E; ++i)
-    if (i < s.from || i >= s.to) v[i] = Elem<T>::put(-INFINITY);
+__device__ __noinline__ uint4 blanked(uint4 w, int from, int to) {
+  constexpr int E = Row<T>::E;
+  unsigned u[4] = {w.x, w.y, w.z, w.w};
+  const uint4 none = minus_infinities<T>();
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (i >= from && i < to) continue;
+    if constexpr (E == 4)
+      u[i] = none.x;
+    else
+      u[i / 2] = i & 1 ? (u[i / 2] & 0xffffu) | (none.x & 0xffff0000u) : (u[i / 2] & 0xffff0000u) | (none.x & 0xffffu);
+  }
+  return {u[0], u[1], u[2], u[3]};
+}
+
+// Elements [from, to) of a vector, one by one.
+template <typename T>
+__device__ __noinline__ void store_some(T* out, uint4 w, int from, int to) {
+  constexpr int E = Row<T>::E;
+  const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (i < from || i >= to) continue;
+    if constexpr (E == 4)
+      reinterpret_cast<unsigned*>(out)[i] = u[i];
+    else
+      reinterpret_cast<unsigned short*>(out)[i] = static_cast<unsigned short>(u[i / 2] >> (16 * (i & 1)));
+  }
 }
 
 // Gradient of a row part, to dx, but for what the target takes from its own.
 // Where dx has the logits' shift (`aligned`) its vectors are those of the
-// registers. `spare`: shared memory of this thread. kWhole: there is no shift
-// and no part of a vector, here and in the logits.
-template <typename T, bool kWhole>
+// registers.
+template <typename T>
 __device__ __forceinline__ void write_part(T* dx, Row<T>& r, int cols, int shift, bool aligned, int threads, int t,
-                                           float scale, uint4* spare) {
+                                           float scale) {
   constexpr int E = Row<T>::E;
 #pragma unroll
   for (int k = 0; k < Row<T>::kVectors; ++k) {
@@ -164,38 +190,30 @@ __device__ __forceinline__ void write_part(T* dx, Row<T>& r, int cols, int shift
     else
       w = uint4{Elem<T>::put2(v[0]), Elem<T>::put2(v[1]), Elem<T>::put2(v[2]), Elem<T>::put2(v[3])};
     T* out = dx + at * E - shift;
-    if constexpr (kWhole) {
-      *reinterpret_cast<uint4*>(out) = w;
-      continue;
-    }
     const Span<E> span(at, shift, cols);
-    if (aligned && span.all()) {
+    if (aligned && span.all())
       *reinterpret_cast<uint4*>(out) = w;
-    } else {
-      *spare = w;
-      const T* from = reinterpret_cast<const T*>(spare);
-#pragma unroll 1
-      for (int i = span.from; i < span.to; ++i) out[i] = from[i];
-    }
+    else
+      store_some<T>(out, w, span.from, span.to);
   }
 }
 
 // A row part's gradient; `owner`: this thread holds the target, `logit` is its
 // value. The target's element is written over by the thread that wrote it.
-template <typename T, bool kWhole>
+template <typename T>
 __device__ __forceinline__ void write_row_part(const Xent& a, Row<T>& r, std::int64_t row, int first, int cols,
                                                int shift, bool aligned, int threads, int t, std::int64_t target,
-                                               bool owner, float logit, float m, float s, float f, uint4* spare) {
+                                               bool owner, float logit, float m, float s, float f) {
   T* dx = static_cast<T*>(a.dx) + row * a.cols + first;
   if (target == a.ignore) {  // zeros, whatever the row holds
 #pragma unroll
     for (int i = 0; i < kEach / 2; ++i) r.v[i] = float2{0.0f, 0.0f};
-    write_part<T, kWhole>(dx, r, cols, shift, aligned, threads, t, 0.0f, spare);
+    write_part<T>(dx, r, cols, shift, aligned, threads, t, 0.0f);
     return;
   }
   const bool bad = bad_target(a, target);
   const float scale = bad ? nan_value() : f * (1.0f / s);
-  write_part<T, kWhole>(dx, r, cols, shift, aligned, threads, t, scale, spare);
+  write_part<T>(dx, r, cols, shift, aligned, threads, t, scale);
   if (owner && !bad)
     static_cast<T*>(a.dx)[row * a.cols + target] = Elem<T>::put(exp2_fast((logit - m) * kLog2e) * scale - f);
 }
@@ -211,12 +229,13 @@ __device__ __forceinline__ int shift_of(const void* p, int size) {
   return static_cast<int>(reinterpret_cast<std::uintptr_t>(p) % 16) / size;
 }
 
-// --- rows up to kEach * 512: a block (or a warp of one) to a row ---
+// --- rows up to 32 * 128: a block (or a warp of one) to a row ---
+
+constexpr int kRowThreads = 128;
 
 template <typename T>
-__global__ void __launch_bounds__(512) xent_rows(const Xent a, const int group) {
+__global__ void __launch_bounds__(kRowThreads) xent_rows(const Xent a, const int group) {
   __shared__ float slots[2][32];
-  __shared__ uint4 spare[512];
   constexpr int E = Row<T>::E;
   const int id = threadIdx.x / group, t = threadIdx.x - id * group, warps = group >> 5, lane = t & 31;
   const std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * (blockDim.x / group) + id;
@@ -238,14 +257,13 @@ __global__ void __launch_bounds__(512) xent_rows(const Xent a, const int group) 
 #pragma unroll
   for (int k = 0; k < Row<T>::kVectors; ++k) {
     const Span<E> span(k * group + t, shift, cols);
-    if (!span.all() && !span.none()) {
-      spare[threadIdx.x] = w[k];
-      blank<T>(&spare[threadIdx.x], span);
-      w[k] = spare[threadIdx.x];
-    }
+    if (!span.all() && !span.none()) w[k] = blanked<T>(w[k], span.from, span.to);
     r.take(k, w[k]);
   }
-  float m = largest(r.max());
+  float m = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < Row<T>::kVectors; ++k) m = larger(m, Row<T>::max(w[k]));
+  m = largest(m);
   if (warps > 1) {
     if (lane == 0) slots[0][t >> 5] = m;
     __syncthreads();
@@ -257,20 +275,30 @@ __global__ void __launch_bounds__(512) xent_rows(const Xent a, const int group) 
     __syncthreads();
     s = warp_sum(lane < warps ? slots[1][lane] : 0.0f);
   }
-  if (owner) finish_row(a, row, target, logit, m, s);
+  if (owner) finish_row(a, row, target == a.ignore, logit, m, s);
   if (a.dx != nullptr) {
     const bool aligned = shift_of(static_cast<T*>(a.dx) + row * a.cols, sizeof(T)) == shift;
-    write_row_part<T, false>(a, r, row, 0, cols, shift, aligned, group, t, target, owner, logit, m, s,
-                      1.0f / (a.reduction == 1 ? a.work[0] : 1.0f), &spare[threadIdx.x]);
+    write_row_part<T>(a, r, row, 0, cols, shift, aligned, group, t, target, owner, logit, m, s,
+                      1.0f / (a.reduction == 1 ? a.work[0] : 1.0f));
   }
 }
 
-// --- longer rows: blocks of 1024 threads, clusters of `kC` to a row ---
+// --- longer rows: a block of `kThreads` walks over rows, clusters of `kC` blocks share one ---
+//
+// A block has 64 bytes a thread of every row, an SM 1024 threads in one, two or
+// four blocks: the smallest that holds a row, so that more rows are under way. One
+// barrier a row: while a row's sum is joined,
+// so is the next row's maximum, and then each thread writes its vectors of the one
+// and fills the registers with the exponentials of the other, vector by vector.
+// Stores, conversions and exponentials, each of which would bound a phase of its
+// own, run side by side (with two barriers and a phase for each, 211 us for 8192
+// rows of 32000 bf16). The next row stays in shared memory until then, its
+// maximum and its exponentials read it from there.
 
-constexpr int kLong = 1024;
-constexpr int kPiece = kLong * 16;           // bytes of one vector a thread, one bulk copy
-constexpr int kRing = 12;                    // pieces in shared memory
-constexpr int kRingBytes = kRing * kPiece;
+constexpr int kLong = 1024;    // threads of an SM
+constexpr int kVectors = 4;    // 16-byte vectors of a thread
+constexpr int kBuffers = 3;    // rows in shared memory
+constexpr int buffer_bytes(int threads) { return kVectors * threads * 16; }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, std::uint64_t* bar) {
   asm volatile(
@@ -281,139 +309,260 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned b
 }
 
 // Leaves v in the shared memory of block `rank` of the cluster, at its copy of
-// `to`, and counts its 4 bytes on that block's copy of `bar`. Unlike a cluster
+// `to`, and counts its bytes on that block's copy of `bar`. Unlike a cluster
 // barrier it does not wait for this thread's stores of gradients to arrive
 // (which cost 8 us a row).
-__device__ __forceinline__ void send(float* to, std::uint64_t* bar, int rank, float v) {
+__device__ __forceinline__ void send(float2* to, std::uint64_t* bar, int rank, float2 v) {
   std::uint32_t at, there;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(async::smem_u32(to)), "r"(rank));
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(async::smem_u32(bar)), "r"(rank));
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(at),
-               "r"(__float_as_uint(v)), "r"(there)
+  const unsigned long long w = static_cast<unsigned long long>(__float_as_uint(v.y)) << 32 | __float_as_uint(v.x);
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(at), "l"(w),
+               "r"(there)
                : "memory");
 }
 
-template <typename T, int kC, bool kWhole>
-__global__ void __launch_bounds__(kLong, 1) xent_long(const Xent a, unsigned* status, std::uint64_t limit_ns) {
-  extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ std::uint64_t full[kRing], joined[2][2];
-  __shared__ float slots[2][32], ranks[2][2][8];
-  __shared__ uint4 spare[kLong];
+template <typename T, int kThreads, int kC, bool kWhole>
+__global__ void __launch_bounds__(kThreads, kLong / kThreads)
+    xent_long(const Xent a, unsigned* status, std::uint64_t limit_ns) {
+  constexpr int kPiece = kThreads * 16;  // bytes of one vector a thread, one bulk copy
+  constexpr int kBuffer = buffer_bytes(kThreads), kWarps = kThreads / 32;
+  extern __shared__ __align__(128) unsigned char buffers[];
+  __shared__ std::uint64_t full[kBuffers], joined[2];
+  __shared__ float2 slots[2][kWarps], ranks[2][8];  // (sum of a row, maximum of the next)
+  __shared__ float factors[2];                      // of a row's gradient
   __shared__ int gave_up;
-  constexpr int E = Row<T>::E, kV = Row<T>::kVectors;
+  // What single warps keep from row to row is in shared memory too: registers
+  // would hold it in every thread, and the exponentials need them.
+  __shared__ struct {
+    const char* x;  // the row that is asked for next
+    std::int64_t row;
+    unsigned slot, round;  // its buffer, and the parity of that buffer's turn
+  } asked;
+  __shared__ int edge[32];
+  __shared__ float e_edge[32];
+  __shared__ struct {
+    std::int64_t target;  // of the row that is finished next
+    float f, last_grad;
+    T* last_at;
+  } note;
+  constexpr int E = 16 / sizeof(T);
   namespace cg = cooperative_groups;
-  const int t = threadIdx.x, lane = t & 31;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  // What one thread or a few do for a row is spread over warps, since a barrier
+  // waits for the slowest: the first asks for rows, the last two write down the
+  // loss and what a row's ends need.
+  const bool asks = warp == 0, edges = !kWhole && warp == kWarps - 2, notes = warp == kWarps - 1;
   int rank = 0;
   if constexpr (kC > 1) rank = cg::this_cluster().block_rank();
-  const std::int64_t clusters = gridDim.x / kC, mine = blockIdx.x / kC;
+  const int clusters = gridDim.x / kC;
   // this block's part of every row; parts begin on whole vectors of the columns
   const std::int64_t share = ((a.cols + kC - 1) / kC + E - 1) / E * E;
   const int first = static_cast<int>(share * rank);
   const int cols = static_cast<int>(a.cols - first < share ? (a.cols > first ? a.cols - first : 0) : share);
   if (t == 0) {
-    for (int i = 0; i < kRing; ++i) async::mbar_init(&full[i], 1);
+    for (int i = 0; i < kBuffers; ++i) async::mbar_init(&full[i], 1);
     if constexpr (kC > 1)
-      for (int i = 0; i < 4; ++i) async::mbar_init(&joined[i >> 1][i & 1], 1);
+      for (int i = 0; i < 2; ++i) async::mbar_init(&joined[i], 1);
     gave_up = 0;
     async::fence_async();
   }
   __syncthreads();
   if constexpr (kC > 1) cg::this_cluster().sync();  // every block has started: its shared memory can be written
   const async::Bound bound{&gave_up, status, limit_ns};
-  auto part = [&](std::int64_t row) { return static_cast<const T*>(a.x.p) + row * a.x.ld + first; };
-  // Pieces are numbered through the rows; piece n goes to slot n % kRing. Every
-  // row of this block has the same pieces but for one that a shift may add.
-  auto vectors = [&](std::int64_t row) {
-    return kWhole ? cols / E : cols == 0 ? 0 : (shift_of(part(row), sizeof(T)) + cols + E - 1) / E;
+
+  // a row's part: of the logits, and of dx, whose rows lie alike to their vectors
+  const std::int64_t row0 = blockIdx.x / kC;
+  const char* x = reinterpret_cast<const char*>(static_cast<const T*>(a.x.p) + row0 * a.x.ld + first);
+  const std::int64_t x_step = clusters * a.x.ld * static_cast<std::int64_t>(sizeof(T));
+  auto shift_at = [](const char* p) {  // elements before the part in its first vector
+    return kWhole ? 0 : static_cast<int>(reinterpret_cast<std::uintptr_t>(p) & 15) / static_cast<int>(sizeof(T));
   };
-  auto pieces = [&](std::int64_t row) { return (vectors(row) + kLong - 1) / kLong; };
-  unsigned issued = 0, used = 0;
-  std::int64_t ahead = mine;  // the row, and its piece, to ask for next
-  int piece = 0;
-  auto request = [&] {  // thread 0: pieces while they find room
-    while (ahead < a.rows) {
-      const T* x = part(ahead);
-      const char* from = reinterpret_cast<const char*>(x - shift_of(x, sizeof(T)));
-      const int n = pieces(ahead), bytes = vectors(ahead) * 16;
-      for (; piece < n; ++piece, ++issued) {
-        if (issued == used + kRing) return;
-        const unsigned slot = issued % kRing;
-        const unsigned size = min(kPiece, bytes - piece * kPiece);
-        async::mbar_expect_tx(&full[slot], size);
-        bulk_load(ring + slot * kPiece, from + piece * kPiece, size, &full[slot]);
-      }
-      ahead += clusters;
-      piece = 0;
+
+  auto request = [&] {  // the first warp: a row, a lane to a piece of it
+    if (asked.row >= a.rows) return;
+    const char* from = asked.x;
+    const unsigned slot = asked.slot;
+    const int skip = kWhole ? 0 : static_cast<int>(reinterpret_cast<std::uintptr_t>(from) & 15);
+    const int bytes = cols == 0 ? 0 : (skip + cols * static_cast<int>(sizeof(T)) + 15) & ~15;
+    __syncwarp();
+    if (lane == 0) {
+      async::mbar_expect_tx(&full[slot], bytes);
+      asked.x = from + x_step;
+      asked.row += clusters;
+      asked.slot = slot + 1 < kBuffers ? slot + 1 : 0;
+      if (asked.slot == 0) asked.round ^= 1u;
     }
+    __syncwarp();
+    const int left = bytes - lane * kPiece;
+    if (lane < kVectors && left > 0)
+      bulk_load(buffers + slot * kBuffer + lane * kPiece, from - skip + lane * kPiece, min(left, kPiece), &full[slot]);
   };
-  if (t == 0) request();
-  const float f = 1.0f / (a.reduction == 1 ? a.work[0] : 1.0f);
-  // A value of each of the cluster's blocks to all of them. Slots and barriers
-  // come in two sets: a block that is a row ahead writes to the other one, and
-  // it cannot be two ahead.
-  unsigned round = 0;
-  auto exchange = [&](int which, float v) {
-    const unsigned set = round & 1u;
-    if (t == 0) async::mbar_expect_tx(&joined[set][which], kC * 4);
-    if (t < kC) send(&ranks[set][which][rank], &joined[set][which], t, v);
-    async::wait(async::smem_u32(&joined[set][which]), round >> 1 & 1u, bound);
-    return ranks[set][which][lane & (kC - 1)];
+  if (asks) {
+    if (lane == 0) {
+      asked.x = x;
+      asked.row = row0;
+      asked.slot = asked.round = 0;
+    }
+    __syncwarp();
+    for (int i = 0; i < kBuffers; ++i) request();
+  }
+
+  // Whether a vector of this thread is the part's, whole. The elements of a part
+  // before its first whole vector and after its last one, under E each, go to the
+  // lanes of one warp, one by one.
+  auto has = [&](int k, int shift) {
+    const int at = (k * kThreads + t) * E;
+    return kWhole ? at < cols : at >= shift && at + E <= shift + cols;
   };
-  for (std::int64_t row = mine; row < a.rows; row += clusters, ++round) {
-    const int n = pieces(row), shift = kWhole ? 0 : shift_of(part(row), sizeof(T));
-    const std::int64_t target = a.target[row];
-    // the part that holds the target, or the first one where none does
-    const bool here = target == a.ignore || bad_target(a, target) ? rank == 0 : target >= first && target - first < cols;
-    const bool owner = here && t == owner_of<E>(a, target, shift - first, kLong);
-    const float logit = owner ? target_logit(a, row, target) : 0.0f;  // on its way early
-    Row<T> r;
+  // this lane's such element, counted from the first vector; -1 without one
+  auto edge_of = [&](int shift) {
+    const int head = min(shift > 0 ? E - shift : 0, cols), tail = min((shift + cols) % E, cols - head);
+    return lane < head ? shift + lane : lane - head < tail ? shift + cols - tail + lane - head : -1;
+  };
+  async::Place begins;  // the buffer of the row that begins
+  auto vector_of = [&](int k) {
+    return reinterpret_cast<const uint4*>(buffers + begins.slot * kBuffer + k * kPiece) + t;
+  };
+  auto element = [&](int at) { return load(buffers + begins.slot * kBuffer, Elem<T>::kType, at); };
+
+  // The sum (x) and the maximum (y) of the blocks of a row, to all threads.
+  async::Place set;
+  auto join = [&](float sum, float top) {
+    sum = warp_sum(sum);
+    top = largest(top);
+    if (lane == 0) slots[set.slot][warp] = float2{sum, top};
+    __syncthreads();  // also: nobody reads the finished row's buffer any more
+    float2 v = slots[set.slot][lane & (kWarps - 1)];
+    v = float2{warp_sum(lane < kWarps ? v.x : 0.0f), largest(v.y)};
+    if constexpr (kC > 1) {
+      // slots and barriers come in two sets: a block that is a row ahead writes to
+      // the other one, and it cannot be two ahead
+      if (t == 0) async::mbar_expect_tx(&joined[set.slot], kC * 8);
+      if (t < kC) send(&ranks[set.slot][rank], &joined[set.slot], t, v);
+      if (t == 0) async::wait(async::smem_u32(&joined[set.slot]), set.round, bound);
+      __syncthreads();
+      v = ranks[set.slot][lane & (kC - 1)];
+      v = float2{warp_sum(lane < kC ? v.x : 0.0f), largest(v.y)};
+    }
+    return v;
+  };
+
+  if (notes && lane == 0) {
+    note.target = a.ignore;
+    note.f = 1.0f / (a.reduction == 1 ? a.work[0] : 1.0f);
+    note.last_at = nullptr;
+  }
+  // loads that are used a turn later: the next row's target, a row's logit there
+  std::int64_t next_target = notes && lane == 0 && row0 < a.rows ? a.target[row0] : a.ignore;
+  float logit = 0.0f;
+  auto counts = [&](std::int64_t t) { return t != a.ignore && !bad_target(a, t); };
+
+  float2 e[kVectors][E / 2];  // exponentials of the row that is finished next
+  float m = 0.0f, sum = 0.0f;
+  int shift = 0;
+  T* dx = static_cast<T*>(a.dx) + (row0 - clusters) * a.cols + first;  // of the row that is finished
+  bool finishes = false;  // the first turn has no row to finish, the last none to begin
+  for (std::int64_t row = row0;; row += clusters, begins.next(kBuffers), set.next(2)) {
+    const bool more = row < a.rows;
+    const int next_shift = shift_at(x);
+    float top = -INFINITY;
+    if (more) {
+      // one lane of a warp asks: a thousand threads at a barrier are served one by one
+      if (lane == 0) async::wait(async::smem_u32(&full[begins.slot]), begins.round, bound);
+      __syncwarp();
 #pragma unroll
-    for (int k = 0; k < kV; ++k) {
-      uint4 w = minus_infinities<T>();
-      if (k < n) {
-        const unsigned slot = (used + k) % kRing;
-        async::wait(async::smem_u32(&full[slot]), (used + k) / kRing & 1u, bound);
-        uint4* vector = reinterpret_cast<uint4*>(ring + slot * kPiece) + t;
-        const Span<E> span(k * kLong + t, shift, cols);
-        if (kWhole) {
-          if ((k * kLong + t) * E < cols) w = *vector;
-        } else if (!span.none()) {
-          if (!span.all()) {
-            blank<T>(vector, span);
-            async::fence_async();  // the slot's next copy comes after these writes
-          }
-          w = *vector;
-        }
+      for (int k = 0; k < kVectors; ++k)
+        if (has(k, next_shift)) top = larger(top, Row<T>::max(*vector_of(k)));
+      if (edges) {
+        const int at = edge_of(next_shift);
+        if (at >= 0) top = larger(top, element(at));
       }
-      r.take(k, w);
     }
-    used += n;
-    float m = largest(r.max());
-    if (lane == 0) slots[0][t >> 5] = m;
-    __syncthreads();  // and every thread has its elements: their pieces are free
-    if (t == 0) {
+    if (notes && lane == 0)
+      factors[set.slot] = note.target == a.ignore ? 0.0f : bad_target(a, note.target) ? nan_value() : note.f;
+    const float2 v = join(sum, top);
+    if (asks && finishes) {
       async::fence_async();
       request();
     }
-    m = largest(slots[0][lane]);
-    if constexpr (kC > 1) m = largest(exchange(0, m));
-    float s = warp_sum(r.exponentials(m));
-    if (lane == 0) slots[1][t >> 5] = s;
-    __syncthreads();
-    s = warp_sum(slots[1][lane]);
-    if constexpr (kC > 1) {
-      const float part = exchange(1, s);
-      s = warp_sum(lane < kC ? part : 0.0f);
+    const bool write = finishes && a.dx != nullptr;
+    const float factor = factors[set.slot], scale = factor * (1.0f / v.x);
+    if (write && factor == 0.0f) {  // an ignored row: zeros, whatever it holds
+      for (int i = t; i < cols; i += kThreads) dx[i] = Elem<T>::put(0.0f);
     }
-    if (owner) finish_row(a, row, target, logit, m, s);
-    if (a.dx != nullptr) {
-      const bool aligned = kWhole || shift_of(static_cast<T*>(a.dx) + row * a.cols + first, sizeof(T)) == shift;
-      write_row_part<T, kWhole>(a, r, row, first, cols, shift, aligned, kLong, t, target, owner, logit, m, s, f, &spare[t]);
+    const bool gradient = write && factor != 0.0f;  // NaN too
+    float2 part_sum = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+      if (gradient && has(k, shift)) {
+        uint4 w;
+        if constexpr (sizeof(T) == 4) {
+          const float2 p = mul2(e[k][0], both(scale)), q = mul2(e[k][1], both(scale));
+          w = uint4{__float_as_uint(p.x), __float_as_uint(p.y), __float_as_uint(q.x), __float_as_uint(q.y)};
+        } else {
+          w = uint4{Elem<T>::put2(mul2(e[k][0], both(scale))), Elem<T>::put2(mul2(e[k][1], both(scale))),
+                    Elem<T>::put2(mul2(e[k][2], both(scale))), Elem<T>::put2(mul2(e[k][3], both(scale)))};
+        }
+        *reinterpret_cast<uint4*>(dx - shift + (k * kThreads + t) * E) = w;
+      }
+      if (more && has(k, next_shift)) {
+        const uint4 w = *vector_of(k);
+        float2 z[E / 2];
+        if constexpr (sizeof(T) == 4) {
+          z[0] = float2{__uint_as_float(w.x), __uint_as_float(w.y)};
+          z[1] = float2{__uint_as_float(w.z), __uint_as_float(w.w)};
+        } else {
+          z[0] = Elem<T>::get2(w.x), z[1] = Elem<T>::get2(w.y), z[2] = Elem<T>::get2(w.z), z[3] = Elem<T>::get2(w.w);
+        }
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+          const float2 y = mul2(add2(z[i], both(-v.y)), both(kLog2e));
+          e[k][i] = float2{exp2_fast(y.x), exp2_fast(y.y)};
+          part_sum = add2(part_sum, e[k][i]);
+        }
+      }
     }
+    if (edges) {
+      if (gradient && edge[lane] >= 0) dx[edge[lane] - shift] = Elem<T>::put(e_edge[lane] * scale);
+      if (more) {
+        const int at = edge_of(next_shift);
+        const float y = at >= 0 ? exp2_fast((element(at) - v.y) * kLog2e) : 0.0f;
+        part_sum.x += y;
+        edge[lane] = at;
+        e_edge[lane] = y;
+      }
+    }
+    if (notes && lane == 0) {
+      // The target's gradient takes the place of what another thread wrote a turn
+      // ago, on the other side of a barrier.
+      if (note.last_at != nullptr) *note.last_at = Elem<T>::put(note.last_grad);
+      note.last_at = nullptr;
+      if (finishes) {
+        if (rank == 0) finish_row(a, row - clusters, note.target == a.ignore, logit, m, v.x);
+        if (write && counts(note.target) && note.target >= first && note.target - first < cols) {
+          note.last_at = dx + (note.target - first);
+          note.last_grad = exp2_fast((logit - m) * kLog2e) * scale - factor;
+        }
+      }
+      note.target = next_target;
+      logit = more && counts(next_target) ? load(a.x.p, a.x.t, row * a.x.ld + next_target) : nan_value();
+      next_target = row + clusters < a.rows ? a.target[row + clusters] : a.ignore;
+    }
+    if (!more) break;
+    sum = part_sum.x + part_sum.y;
+    m = v.y;
+    shift = next_shift;
+    x += x_step;
+    dx += clusters * a.cols;
+    finishes = true;
   }
+  __syncthreads();
+  if (notes && lane == 0 && note.last_at != nullptr) *note.last_at = Elem<T>::put(note.last_grad);
   // shared memory outlives the copies, and what other blocks send, also where a wait gave up
   if (t == 0 && gave_up != 0)
-    for (unsigned n = used; n < issued; ++n) async::settle(async::smem_u32(&full[n % kRing]), n / kRing & 1u, limit_ns);
+    for (unsigned i = 0; i < kBuffers; ++i)
+      async::settle(async::smem_u32(&full[i]), i < asked.slot ? asked.round : asked.round ^ 1u, limit_ns);
   if constexpr (kC > 1) cg::this_cluster().sync();
 }
 
@@ -448,7 +597,7 @@ __global__ void __launch_bounds__(kSweep) xent_sweep(const Xent a) {
         s += exp2_fast((load(a.x.p, a.x.t, row * a.x.ld + i) - m) * kLog2e);
       s = block_sum(s, slots);
     }
-    if (threadIdx.x == 0) finish_row(a, row, target, target_logit(a, row, target), m, s);
+    if (threadIdx.x == 0) finish_row(a, row, target == a.ignore, target_logit(a, row, target), m, s);
     if (a.dx != nullptr) write_row(a, row, m, s, target, 1.0f / count, target != a.ignore);
   }
 }
@@ -468,16 +617,16 @@ unsigned grid_of(std::int64_t rows) {
   return static_cast<unsigned>(rows < 1 ? 1 : rows < most ? rows : most);
 }
 
-template <typename T, int kC, bool kWhole>
+template <typename T, int kThreads, int kC, bool kWhole>
 cudaError_t launch_long(const Xent& a, cudaStream_t stream) {
-  const auto kernel = xent_long<T, kC, kWhole>;
-  const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  const auto kernel = xent_long<T, kThreads, kC, kWhole>;
+  constexpr int kBytes = kBuffers * buffer_bytes(kThreads);
+  const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (rc != cudaSuccess) return rc;
-  const std::int64_t most = sm_count() / kC;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((a.rows < most ? a.rows : most) * kC));
-  cfg.blockDim = dim3(kLong);
-  cfg.dynamicSmemBytes = kRingBytes;
+  cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / kC * kC));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -485,6 +634,16 @@ cudaError_t launch_long(const Xent& a, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  // The clusters that run at once (an SM count of a GPU part need not be a
+  // multiple of kC): one more would wait for another to finish all its rows.
+  static std::atomic<int> known{0};
+  int most = known.load(std::memory_order_relaxed);
+  if (most == 0) {
+    if (kC == 1 || cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1)
+      most = sm_count() * (kLong / kThreads) / kC;
+    known.store(most, std::memory_order_relaxed);
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>((a.rows < most ? a.rows : most) * kC));
   unsigned* status = nullptr;
   commux_ops::status_word(&status);
   return cudaLaunchKernelEx(&cfg, kernel, a, status, commux_ops::wait_limit_ns());
@@ -494,29 +653,41 @@ template <typename T>
 cudaError_t launch_rows(const Xent& a, cudaStream_t stream) {
   constexpr int E = Row<T>::E;
   const std::int64_t need = a.cols + E - 1;  // with the longest shift
-  if (need <= kEach * 512) {
+  if (need <= kEach * kRowThreads) {
     const int group = static_cast<int>((need + kEach * 32 - 1) / (kEach * 32)) * 32;
     const int ids = group == 32 ? 4 : 1;
     xent_rows<T><<<static_cast<unsigned>((a.rows + ids - 1) / ids), group * ids, 0, stream>>>(a, group);
     return cudaSuccess;
   }
-  // the fewest blocks that hold a row, and more where the rows leave SMs idle
+  const bool whole = a.cols % E == 0 && a.x.ld % E == 0 && reinterpret_cast<std::uintptr_t>(a.x.p) % 16 == 0;
+  if (a.dx != nullptr && !(a.x.ld % E == a.cols % E && reinterpret_cast<std::uintptr_t>(a.x.p) % 16 ==
+                                                           reinterpret_cast<std::uintptr_t>(a.dx) % 16)) {
+    // rows of dx lie otherwise to their vectors than the logits' (a slice of a wider tensor at an odd place)
+    xent_sweep<<<grid_of(a.rows), kSweep, 0, stream>>>(a);
+    return cudaSuccess;
+  }
+  auto go = [&](auto threads, auto blocks) {
+    constexpr int kThreads = decltype(threads)::value, kC = decltype(blocks)::value;
+    return whole ? launch_long<T, kThreads, kC, true>(a, stream) : launch_long<T, kThreads, kC, false>(a, stream);
+  };
+  const std::integral_constant<int, 1> one;
+  // Many rows: the smallest block that holds one. Where the rows leave SMs idle,
+  // or a row is longer than a block's, more blocks to a row.
+  const bool few = a.rows * 2 <= sm_count();
+  if (!few && need <= kVectors * 256 * E) return go(std::integral_constant<int, 256>(), one);
+  if (!few && need <= kVectors * 512 * E) return go(std::integral_constant<int, 512>(), one);
   int c = 1;
-  const int most = kEach * kLong - E;
+  const int most = kVectors * kLong * E - E;
   while (c < 8 && ((a.cols + c - 1) / c + E > most || a.rows * c * 2 <= sm_count())) c *= 2;
   if ((a.cols + c - 1) / c + E > most) {
     xent_sweep<<<grid_of(a.rows), kSweep, 0, stream>>>(a);
     return cudaSuccess;
   }
-  const bool whole = a.cols % E == 0 && a.x.ld % E == 0 && reinterpret_cast<std::uintptr_t>(a.x.p) % 16 == 0;
-  auto go = [&](auto blocks) {
-    constexpr int kC = decltype(blocks)::value;
-    return whole ? launch_long<T, kC, true>(a, stream) : launch_long<T, kC, false>(a, stream);
-  };
-  return c == 1   ? go(std::integral_constant<int, 1>())
-         : c == 2 ? go(std::integral_constant<int, 2>())
-         : c == 4 ? go(std::integral_constant<int, 4>())
-                  : go(std::integral_constant<int, 8>());
+  const std::integral_constant<int, kLong> all;
+  return c == 1   ? go(all, one)
+         : c == 2 ? go(all, std::integral_constant<int, 2>())
+         : c == 4 ? go(all, std::integral_constant<int, 4>())
+                  : go(all, std::integral_constant<int, 8>());
 }
 
 }  // namespace

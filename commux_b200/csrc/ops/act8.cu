@@ -29,11 +29,33 @@ __device__ __forceinline__ float2 sigmoid2(float2 x, float2 sq) {  // 1 / (1 + e
   return {inverse_fast(d.x), inverse_fast(d.y)};
 }
 
+// exact form: Phi(-|x|) = (1 - erf(z)) / 2 at z = |x| / sqrt(2), by the fit of
+// Hastings (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26):
+// erf(z) = 1 - (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), within 1.5e-7.
+// exp(-z^2) is also the density that the slope needs. The halves of the
+// coefficients leave Phi, and 1 - that for a positive x.
+struct Normal {
+  float2 cdf, bell;  // Phi(x), exp(-x^2 / 2)
+};
+__device__ __forceinline__ Normal normal(float2 x) {
+  const float2 z = {fabsf(x.x) * 0.70710678118654752f, fabsf(x.y) * 0.70710678118654752f};
+  const float2 d = fma2(z, both(0.3275911f), both(1.0f)), t = {inverse_fast(d.x), inverse_fast(d.y)};
+  float2 s = fma2(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+  s = fma2(t, s, both(0.5f * 1.421413741f));
+  s = fma2(t, s, both(0.5f * -0.284496736f));
+  s = fma2(t, s, both(0.5f * 0.254829592f));
+  const float2 y = mul2(mul2(z, z), both(-kE));
+  Normal n;
+  n.bell = float2{exp2_fast(y.x), exp2_fast(y.y)};
+  s = mul2(mul2(s, t), n.bell);
+  n.cdf = float2{x.x > 0.0f ? 1.0f - s.x : s.x, x.y > 0.0f ? 1.0f - s.y : s.y};
+  return n;
+}
+
 template <bool kTanh>
 __device__ __forceinline__ float2 gelu(float2 x) {
   if constexpr (kTanh) return mul2(x, sigmoid2(x, mul2(x, x)));
-  const float2 z = mul2(x, both(0.70710678118654752f));
-  return mul2(mul2(x, both(0.5f)), add2(float2{erff(z.x), erff(z.y)}, both(1.0f)));
+  return mul2(x, normal(x).cdf);
 }
 
 template <bool kTanh>
@@ -46,9 +68,8 @@ __device__ __forceinline__ float2 gelu_slope(float2 x) {
     const float2 rest = fma2(sig, both(-1.0f), both(1.0f));
     return fma2(mul2(x, sig), mul2(rest, fma2(sq, both(3.0f * kC * kK), both(kK))), sig);
   }
-  const float2 z = mul2(x, both(0.70710678118654752f)), p = mul2(mul2(x, x), both(-0.5f * kE));
-  const float2 cdf = fma2(float2{erff(z.x), erff(z.y)}, both(0.5f), both(0.5f));
-  return fma2(mul2(x, both(0.39894228040143268f)), float2{exp2_fast(p.x), exp2_fast(p.y)}, cdf);
+  const Normal n = normal(x);
+  return fma2(mul2(x, both(0.39894228040143268f)), n.bell, n.cdf);
 }
 
 // What a pass does with its values; the passes differ in that alone. A pass

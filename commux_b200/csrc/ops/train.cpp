@@ -188,10 +188,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     if (train) {
       // the packed form replaces the stream itself in what is kept
       ctx->save_for_backward({pack ? Tensor() : s.defined() ? s : x, held.q, held.scale, stats, weight});
-      ctx->saved_data["has_bias"] = b.defined();
-      ctx->saved_data["xt"] = static_cast<int64_t>(x.scalar_type());
-      ctx->saved_data["rt"] = r.t.defined() ? static_cast<int64_t>(residual->scalar_type()) : int64_t{-1};
-      ctx->saved_data["sizes"] = x.sizes().vec();
+      // dtypes of x and of the residual, and whether there is a bias, in one number: every entry costs host time
+      ctx->saved_data["kinds"] = static_cast<int64_t>(x.scalar_type()) |
+                                 (r.t.defined() ? static_cast<int64_t>(residual->scalar_type()) : int64_t{0xff}) << 8 |
+                                 static_cast<int64_t>(b.defined()) << 16;
     }
     return outs;
   }
@@ -201,17 +201,16 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     no_second_order(who);
     const auto saved = ctx->get_saved_variables();
     const Tensor &kept = saved[0], &q = saved[1], &scale = saved[2], &stats = saved[3], &weight = saved[4];
-    const auto xt = static_cast<at::ScalarType>(ctx->saved_data["xt"].toInt());
-    const auto rt = ctx->saved_data["rt"].toInt();
-    const auto sizes = ctx->saved_data["sizes"].toIntVector();
-    const bool has_bias = ctx->saved_data["has_bias"].toBool(), has_residual = rt >= 0;
+    const int64_t kinds = ctx->saved_data["kinds"].toInt();
+    const auto xt = static_cast<at::ScalarType>(kinds & 0xff), rt = static_cast<at::ScalarType>(kinds >> 8 & 0xff);
+    const bool has_bias = kinds >> 16 != 0, has_residual = (kinds >> 8 & 0xff) != 0xff;
     const Tensor dy = grads[0], ds = has_residual ? grads[1] : Tensor();
     variable_list out(8);
     const auto opts = stats.options();
     if (!dy.defined()) {  // only the stream was used
       if (ds.defined()) {
         out[0] = ds;
-        if (has_residual) out[1] = ds.to(static_cast<at::ScalarType>(rt));
+        if (has_residual) out[1] = ds.to(rt);
       }
       return out;
     }
@@ -223,12 +222,12 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     train::NormBwd a{};
     a.rows = stats.size(1);
     a.cols = w.size(0);
+    const auto sizes = dy.sizes();
     const Tensor dx = at::empty(sizes, opts.dtype(xt));
     Tensor dr;
     // graph edges are counted over the tensors that were given
     const bool need_r = has_residual && ctx->needs_input_grad(1);
-    if (need_r && static_cast<at::ScalarType>(rt) != xt)
-      dr = at::empty(sizes, opts.dtype(static_cast<at::ScalarType>(rt)));
+    if (need_r && rt != xt) dr = at::empty(sizes, opts.dtype(rt));
     const size_t w_edge = has_residual ? 2 : 1;
     const bool need_w = ctx->needs_input_grad(w_edge), need_b = has_bias && ctx->needs_input_grad(w_edge + 1);
     const Tensor dw = need_w ? at::empty_like(w) : Tensor(), db = need_b ? at::empty_like(w) : Tensor();
@@ -307,9 +306,10 @@ Tensor unpack8(const Tensor& q, const Tensor& scale, std::vector<int64_t> sizes,
 
 // --- GELU ------------------------------------------------------------------------
 
-struct Gelu8 : torch::autograd::Function<Gelu8> {
+template <bool kTanh>
+struct Gelu8 : torch::autograd::Function<Gelu8<kTanh>> {
   // returns y, then its 8-bit form (if packed)
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, bool tanh_form, bool pack, bool train) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, bool pack, bool train) {
     const char* who = "gelu8";
     const Mat m = matrix(x, who, "x");
     c10::cuda::CUDAGuard guard(x.device());
@@ -327,11 +327,10 @@ struct Gelu8 : torch::autograd::Function<Gelu8> {
       a.yscale = s_ptr(hy.scale);
       a.rows = m.n;
       a.cols = m.cols;
-      a.tanh_form = tanh_form;
+      a.tanh_form = kTanh;
       C10_CUDA_CHECK(train::gelu8_forward(a, stream_of(x)));
     }
-    ctx->save_for_backward({h.q, h.scale});
-    ctx->saved_data["tanh"] = tanh_form;
+    if (train) ctx->save_for_backward({h.q, h.scale});
     variable_list outs{y};
     if (pack) {
       outs.push_back(hy.q);
@@ -345,7 +344,7 @@ struct Gelu8 : torch::autograd::Function<Gelu8> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* who = "gelu8";
     no_second_order(who);
-    variable_list out(4);
+    variable_list out(3);
     if (!grads[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const Mat m = matrix(grads[0], who, "gradient");
@@ -359,7 +358,7 @@ struct Gelu8 : torch::autograd::Function<Gelu8> {
       a.dx = dx.data_ptr();
       a.rows = m.n;
       a.cols = m.cols;
-      a.tanh_form = ctx->saved_data["tanh"].toBool();
+      a.tanh_form = kTanh;
       C10_CUDA_CHECK(train::gelu8_backward(a, stream_of(dx)));
     }
     out[0] = dx;
@@ -367,7 +366,9 @@ struct Gelu8 : torch::autograd::Function<Gelu8> {
   }
 };
 
-variable_list gelu8(const Tensor& x, bool tanh_form, bool pack) { return Gelu8::apply(x, tanh_form, pack, graph(x)); }
+variable_list gelu8(const Tensor& x, bool tanh_form, bool pack) {
+  return tanh_form ? Gelu8<true>::apply(x, pack, graph(x)) : Gelu8<false>::apply(x, pack, graph(x));
+}
 
 // --- linear ----------------------------------------------------------------------
 

@@ -140,10 +140,9 @@ __device__ __forceinline__ void write_four(const Plan& p, const Out& out, std::i
     *reinterpret_cast<float4*>(static_cast<float*>(out.dw) + o * p.cols + i) = v;
     return;
   }
-  write_dw(p, out, o, i, v.x, db);
-  if (i + 1 < p.cols) write_dw(p, out, o, i + 1, v.y, db);
-  if (i + 2 < p.cols) write_dw(p, out, o, i + 2, v.z, db);
-  if (i + 3 < p.cols) write_dw(p, out, o, i + 3, v.w, db);
+#pragma unroll 1
+  for (int k = 0; k < 4 && i + k < p.cols; ++k)
+    write_dw(p, out, o, i + k, k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w, db);
 }
 
 __device__ __forceinline__ void sync_pair() {
@@ -474,12 +473,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int r = j * 4 + sub;
-            const float4 u = turn[r * 8 + (four ^ (r & 7))];
+            float4* mine = &turn[r * 8 + (four ^ (r & 7))];
+            const float4 u = *mine;
             w[j] = float4{w[j].x + u.x, w[j].y + u.y, w[j].z + u.z, w[j].w + u.w};
             if (!last)
               place[j * kN] = w[j];
             else
-              write_four(p, out, s.m0 + rows0 + r, s.n0 + c * 32 + four * 4, w[j], column[local0 + r]);
+              *mine = w[j];
+          }
+          if (last) {
+            // not unrolled: a small product spends its time on fetching instructions
+#pragma unroll 1
+            for (int r = sub; r < 32; r += 4)
+              write_four(p, out, s.m0 + rows0 + r, s.n0 + c * 32 + four * 4, turn[r * 8 + (four ^ (r & 7))],
+                         column[local0 + r]);
           }
           __syncwarp();
         }
@@ -759,7 +766,12 @@ cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
   const auto kernel = p.planes == 1 ? wgrad_tiles<true> : wgrad_tiles<false>;
-  const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static const cudaError_t set = [] {  // an attribute of the functions, for every device
+    const cudaError_t e = cudaFuncSetAttribute(wgrad_tiles<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    return e != cudaSuccess
+               ? e
+               : cudaFuncSetAttribute(wgrad_tiles<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  }();
   if (set != cudaSuccess) return set;
   const Out out{a.dw, a.db, a.dwt, a.w, a.b, a.wt, static_cast<float*>(a.work)};
   unsigned* status = nullptr;

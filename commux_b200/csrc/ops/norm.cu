@@ -485,7 +485,7 @@ int blocks_of(const Walk& p, std::int64_t rows, int least) {
   }();
   const int threads = p.group * p.ids, fit = 65536 / (registers * threads);
   const std::int64_t most = static_cast<std::int64_t>(sm_count()) * (fit < 1 ? 1 : fit);
-  const std::int64_t want = (rows + static_cast<std::int64_t>(least) * p.ids - 1) / (static_cast<std::int64_t>(least) * p.ids);
+  const std::int64_t each = static_cast<std::int64_t>(least) * p.ids, want = (rows + each - 1) / each;
   return static_cast<int>(want < most ? want : most);
 }
 
@@ -515,7 +515,8 @@ void launch_fwd(const NormFwd& a, const Walk& p, cudaStream_t stream) {
   if (p.aligned)
     p.parts == 1 ? go_fwd<norm_fwd<X, Y, S, true, 1>>(a, p, stream) : go_fwd<norm_fwd<X, Y, S, true, 2>>(a, p, stream);
   else
-    p.parts == 1 ? go_fwd<norm_fwd<X, Y, S, false, 1>>(a, p, stream) : go_fwd<norm_fwd<X, Y, S, false, 2>>(a, p, stream);
+    p.parts == 1 ? go_fwd<norm_fwd<X, Y, S, false, 1>>(a, p, stream)
+                 : go_fwd<norm_fwd<X, Y, S, false, 2>>(a, p, stream);
 }
 
 template <auto kKernel>

@@ -214,7 +214,8 @@ struct Part {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) u[i] = __funnelshift_r(u[i], u[i + 1], (back & 1) * 16);
       }
-      const int from = joined ? 0 : shift, to = cols - c + shift;  // elements [from, to) of the vectors are to be written
+      // elements [from, to) of the vectors are to be written
+      const int from = joined ? 0 : shift, to = cols - c + shift;
       T* at = row + c - shift;
 #pragma unroll
       for (int k = 0; k < kWords / 4; ++k) {
@@ -245,6 +246,21 @@ struct Part {
 // Rows of whole parts on 16-byte boundaries.
 inline bool aligned_rows(const void* p, std::int64_t ld, std::int64_t cols) {
   return cols % 8 == 0 && ld % 8 == 0 && reinterpret_cast<std::uintptr_t>(p) % 16 == 0;
+}
+
+// Lets a kernel use more than 48 KB of shared memory: an attribute of the kernel
+// on each device, set at its first use there.
+template <auto kKernel>
+cudaError_t allow_shared(int bytes) {
+  static std::atomic<std::uint64_t> done{0};
+  int device = 0;
+  cudaError_t rc = cudaGetDevice(&device);
+  if (rc != cudaSuccess) return rc;
+  const std::uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_relaxed) & bit) != 0) return cudaSuccess;
+  rc = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (rc == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return rc;
 }
 
 // Calls f with a value of the element type that t names.

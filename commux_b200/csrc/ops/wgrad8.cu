@@ -724,7 +724,9 @@ Plan plan_of(const Wgrad8& a) {
   return p;
 }
 
-std::int64_t slots_bytes(const Plan& p) { return static_cast<std::int64_t>(p.slots) * p.pairs * kSlot * static_cast<std::int64_t>(sizeof(float)); }
+std::int64_t slots_bytes(const Plan& p) {
+  return static_cast<std::int64_t>(p.slots) * p.pairs * kSlot * static_cast<std::int64_t>(sizeof(float));
+}
 std::int64_t terms_ld(const Wgrad8& a) { return (a.outs + 7) / 8 * 8; }
 
 }  // namespace
@@ -766,12 +768,8 @@ cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
   const auto kernel = p.planes == 1 ? wgrad_tiles<true> : wgrad_tiles<false>;
-  static const cudaError_t set = [] {  // an attribute of the functions, for every device
-    const cudaError_t e = cudaFuncSetAttribute(wgrad_tiles<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    return e != cudaSuccess
-               ? e
-               : cudaFuncSetAttribute(wgrad_tiles<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  }();
+  const cudaError_t set =
+      p.planes == 1 ? allow_shared<wgrad_tiles<true>>(kSmem) : allow_shared<wgrad_tiles<false>>(kSmem);
   if (set != cudaSuccess) return set;
   const Out out{a.dw, a.db, a.dwt, a.w, a.b, a.wt, static_cast<float*>(a.work)};
   unsigned* status = nullptr;

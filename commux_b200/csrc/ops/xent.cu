@@ -621,7 +621,7 @@ template <typename T, int kThreads, int kC, bool kWhole>
 cudaError_t launch_long(const Xent& a, cudaStream_t stream) {
   const auto kernel = xent_long<T, kThreads, kC, kWhole>;
   constexpr int kBytes = kBuffers * buffer_bytes(kThreads);
-  const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  const cudaError_t rc = allow_shared<xent_long<T, kThreads, kC, kWhole>>(kBytes);
   if (rc != cudaSuccess) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / kC * kC));

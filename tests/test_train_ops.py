@@ -73,7 +73,8 @@ NORM_TYPES = [(F32, F32, F32, F32), (F32, BF16, F32, BF16), (BF16, BF16, BF16, B
 
 @gpu
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 768), (3, 31), (5, 33), (257, 768), (64, 1000), (33, 1001),
-                                       (7, 4096), (5, 5003), (3, 8192), (2, 20011), (2, 40000), (1300, 8)])
+                                       (7, 4096), (5, 5003), (3, 8192), (2, 20011), (2, 40000), (1300, 8),
+                                       (900, 200), (1100, 2056), (700, 4100), (650, 6001)])
 @pytest.mark.parametrize("xt,yt,wt,rt", NORM_TYPES)
 @pytest.mark.parametrize("residual,pack", [(False, False), (True, False), (False, True), (True, True)])
 def test_layer_norm(rows, cols, xt, yt, wt, rt, residual, pack):
@@ -347,6 +348,31 @@ def test_weight_grad8(rows, cols, outs, dtype, out):
 
 
 @gpu
+@pytest.mark.parametrize("rows,cols,outs,out", [(4000, 2050, 9000, F32), (2000, 2100, 9000, BF16),
+                                                (6000, 700, 1500, F32)])
+@pytest.mark.parametrize("after_norm", [False, True])
+def test_weight_grad8_many_tiles(rows, cols, outs, out, after_norm):
+    # tiles that one pair holds whole, tiles that several share, and sums that are cut
+    g = gen(rows)
+    x, dy = randn(g, rows, cols, dtype=BF16), randn(g, rows, outs, dtype=BF16)
+    w, b = (1 + 0.2 * randn(g, cols), randn(g, cols)) if after_norm else (None, None)
+    kept = ops.layer_norm(x, w, b, pack=True)[1] if after_norm else ops.pack8(x)
+    dw, db = ops.weight_grad8(dy, kept, bias=True, out_dtype=out)
+    v = ops.Act8(kept.q, kept.scale, kept.shape, F32).unpack().double()
+    mag = v.abs()
+    if after_norm:
+        v, mag = v * w.double() + b.double(), mag * w.double().abs() + b.double().abs()
+    close(dw, dy.double().t() @ v, dy.double().abs().t() @ mag, rows + 64, "dw")
+    close(db, dy.double().sum(0), dy.double().abs().sum(0), rows + 64, "db")
+    if out == F32 and not after_norm:
+        # A sum of 16 tokens' products is cut off, not rounded, when it is added to
+        # the others: half a unit (2^-24 to 2^-25 of the sum) each on average, over
+        # 96 additions at most. Twice that holds the error's norm.
+        off = (dw.double() - dy.double().t() @ v).norm() / (dy.double().t() @ v).norm()
+        assert float(off) <= 2 * 96 * 2.0 ** -24.5, float(off)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("with_bias", [False, True])
 def test_weight_grad8_after_a_norm(dtype, with_bias):
@@ -524,6 +550,34 @@ def test_cross_entropy_targets():
     assert ops.cross_entropy(y, t, reduction="none").shape == (2, 3)
 
 
+@gpu
+@pytest.mark.parametrize("rows,cols", [(700, 3000), (900, 5003), (600, 8192), (400, 9001), (300, 20000), (310, 16379),
+                                       (200, 32001), (160, 60000), (150, 120001)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_cross_entropy_many_rows(rows, cols, dtype):
+    # several rows to a block: what one row leaves behind must not reach the next
+    g = gen(rows + cols)
+    x = randn(g, rows, cols, dtype=dtype, scale=2.0)
+    target = torch.randint(0, cols, (rows,), generator=g, device="cuda")
+    target[::7] = -100
+    target[0] = 0
+    target[2], target[3] = cols - 1, cols - 2
+    x[5::11, cols // 3:] = -math.inf
+    target[5::11] %= cols // 3
+    x[7] = math.nan
+    target[7] = -100  # ignored, whatever it holds
+    x.requires_grad_()
+    loss = ops.cross_entropy(x, target)
+    (dx,) = torch.autograd.grad(loss, x)
+    keep = torch.arange(rows, device="cuda") != 7
+    each, grad, mag, valid = xent64(x.detach().double()[keep], target[keep], -100)
+    n = valid.sum()
+    size = x.detach().double()[keep].abs().nan_to_num(posinf=0).amax(1) + 16
+    close(loss.detach(), each.sum() / n, (size * valid).sum() / n, 32 + rows / 32, "loss")
+    close(dx[keep], grad / n, mag.nan_to_num() / n, 16, "dx")
+    assert dx[7].eq(0).all()
+
+
 # --- gradients against differences -------------------------------------------
 
 def _differences(f, xs, seed, step=2.0 ** -7):
@@ -645,6 +699,22 @@ def test_offsets_past_32_bits(what):
 
 
 @gpu
+def test_no_wait_gave_up():
+    # the status word of the kernels' bounded waits, after a few of each that wait
+    from commux_b200 import _ops
+
+    g = gen(61)
+    for rows, cols in ((300, 500), (40, 40000)):
+        x = randn(g, rows, cols, dtype=BF16).requires_grad_()
+        loss = ops.cross_entropy(x, torch.randint(0, cols, (rows,), generator=g, device="cuda"))
+        torch.autograd.grad(loss, x)
+        ops.weight_grad8(randn(g, rows, 700, dtype=BF16), ops.pack8(x))
+        ops.weight_grad8(randn(g, rows, 70), ops.pack8(x))
+    torch.cuda.synchronize()
+    assert _ops.kernel_status() == 0
+
+
+@gpu
 def test_refusals_on_device():
     x, w = torch.zeros(4, 32, device="cuda"), torch.ones(32, device="cuda")
     for bad in (dict(weight=torch.ones(31, device="cuda")), dict(weight=w.double()), dict(weight=w.cpu()),
@@ -725,7 +795,7 @@ def test_gpt_step(autocast):
         with torch.autocast("cuda", dtype=BF16, enabled=autocast):
             loss = m(idx, target)
         loss.backward()
-        losses.append(float(loss))
+        losses.append(float(loss.detach()))
     assert abs(losses[0] - losses[1]) <= (2e-2 if autocast else 1e-4), losses
     for (name, p), q in zip(plain.named_parameters(), held.parameters()):
         assert q.grad.dtype == p.grad.dtype

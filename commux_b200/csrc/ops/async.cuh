@@ -92,8 +92,8 @@ __device__ __forceinline__ bool try_wait(std::uint32_t bar, unsigned parity) {
 }
 
 template <bool kCluster>
-__device__ __noinline__ bool wait_longer(std::uint32_t bar, unsigned parity, volatile int* gave_up, unsigned* status,
-                                         std::uint64_t limit_ns) {
+__device__ __forceinline__ bool wait_here(std::uint32_t bar, unsigned parity, volatile int* gave_up, unsigned* status,
+                                          std::uint64_t limit_ns) {
   std::uint64_t since = 0;
   for (unsigned tries = 1; !try_wait<kCluster>(bar, parity); ++tries) {
     if (tries % 64 != 0) continue;  // the timer and the flag in one of many tries
@@ -109,12 +109,24 @@ __device__ __noinline__ bool wait_longer(std::uint32_t bar, unsigned parity, vol
   return true;
 }
 
+template <bool kCluster>
+__device__ __noinline__ bool wait_longer(std::uint32_t bar, unsigned parity, volatile int* gave_up, unsigned* status,
+                                         std::uint64_t limit_ns) {
+  return wait_here<kCluster>(bar, parity, gave_up, status, limit_ns);
+}
+
 // Short where the wait is over already: a lone thread that feeds the tensor core
 // pays for every instruction between two products.
 template <bool kCluster = false>
 __device__ __forceinline__ bool wait(std::uint32_t bar, unsigned parity, const Bound& b) {
   if (try_wait<kCluster>(bar, parity)) return true;
   return wait_longer<kCluster>(bar, parity, b.gave_up, b.status, b.limit_ns);
+}
+
+// For a kernel without registers to spare: the call that wait() may make has every
+// thread keep values in local memory, whether it is made or not.
+__device__ __forceinline__ bool wait_inline(std::uint32_t bar, unsigned parity, const Bound& b) {
+  return wait_here<false>(bar, parity, b.gave_up, b.status, b.limit_ns);
 }
 
 __device__ __forceinline__ void arrive(std::uint32_t bar) {

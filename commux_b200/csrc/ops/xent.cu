@@ -287,13 +287,16 @@ __global__ void __launch_bounds__(kRowThreads) xent_rows(const Xent a, const int
 //
 // A block has 64 bytes a thread of every row, an SM 1024 threads in one, two or
 // four blocks: the smallest that holds a row, so that more rows are under way. One
-// barrier a row: while a row's sum is joined,
-// so is the next row's maximum, and then each thread writes its vectors of the one
-// and fills the registers with the exponentials of the other, vector by vector.
-// Stores, conversions and exponentials, each of which would bound a phase of its
-// own, run side by side (with two barriers and a phase for each, 211 us for 8192
-// rows of 32000 bf16). The next row stays in shared memory until then, its
-// maximum and its exponentials read it from there.
+// barrier a row: while a row's sum is joined, so is the next row's maximum, and then
+// each thread writes its vectors of the one and fills the registers with the
+// exponentials of the other, vector by vector. Stores, conversions and exponentials,
+// each of which would bound a phase of its own, run side by side (with two barriers
+// and a phase for each, 211 us for 8192 rows of 32000 bf16). The next row stays in
+// shared memory until then, its maximum and its exponentials read it from there.
+//
+// A row's chain (wait, maximum, barrier, two reductions) and the instructions bound
+// it next to the memory: 8192 rows of 32000 bf16 with their gradient take 184 us,
+// 5.7 TB/s; 208 us with 32001 columns; 1024 rows of 128001 in clusters of 4 take 146.
 
 constexpr int kLong = 1024;    // threads of an SM
 constexpr int kVectors = 4;    // 16-byte vectors of a thread
@@ -322,6 +325,11 @@ __device__ __forceinline__ void send(float2* to, std::uint64_t* bar, int rank, f
                : "memory");
 }
 
+// kWhole: every row lies in whole vectors. Where one does not, its buffer holds
+// other rows' elements before and after its own. The warp that owns such a vector
+// overwrites them with -inf, so that all threads may take all vectors as they are
+// (with tests of each vector and a warp for what is left over: 259 us for 8192 rows
+// of 32001 bf16), and writes that vector of the gradient element by element.
 template <typename T, int kThreads, int kC, bool kWhole>
 __global__ void __launch_bounds__(kThreads, kLong / kThreads)
     xent_long(const Xent a, unsigned* status, std::uint64_t limit_ns) {
@@ -331,6 +339,7 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
   __shared__ std::uint64_t full[kBuffers], joined[2];
   __shared__ float2 slots[2][kWarps], ranks[2][8];  // (sum of a row, maximum of the next)
   __shared__ float factors[2];                      // of a row's gradient
+  __shared__ uint4 ends[2];                         // a gradient's first and last vector
   __shared__ int gave_up;
   // What single warps keep from row to row is in shared memory too: registers
   // would hold it in every thread, and the exponentials need them.
@@ -339,20 +348,19 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
     std::int64_t row;
     unsigned slot, round;  // its buffer, and the parity of that buffer's turn
   } asked;
-  __shared__ int edge[32];
-  __shared__ float e_edge[32];
   __shared__ struct {
-    std::int64_t target;  // of the row that is finished next
-    float f, last_grad;
+    std::int64_t target, next_target[2];  // of the row that is finished next
+    float f, m, logit;
+    float last_grad;  // the target's gradient of the row before, and its place
     T* last_at;
   } note;
   constexpr int E = 16 / sizeof(T);
   namespace cg = cooperative_groups;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   // What one thread or a few do for a row is spread over warps, since a barrier
-  // waits for the slowest: the first asks for rows, the last two write down the
-  // loss and what a row's ends need.
-  const bool asks = warp == 0, edges = !kWhole && warp == kWarps - 2, notes = warp == kWarps - 1;
+  // waits for the slowest: the first sees to a row's first vector, and of the last
+  // two one asks for rows and one writes down the loss and the target's gradient.
+  const bool asks = warp == kWarps - 2, notes = warp == kWarps - 1;
   int rank = 0;
   if constexpr (kC > 1) rank = cg::this_cluster().block_rank();
   const int clusters = gridDim.x / kC;
@@ -360,26 +368,39 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
   const std::int64_t share = ((a.cols + kC - 1) / kC + E - 1) / E * E;
   const int first = static_cast<int>(share * rank);
   const int cols = static_cast<int>(a.cols - first < share ? (a.cols > first ? a.cols - first : 0) : share);
+  const int vectors = cols == 0 ? 0 : kWhole ? cols / E : (cols + 2 * E - 2) / E;  // that a part may touch
+  // vectors of this warp's threads
+  const int mine = (vectors - warp * 32 + kThreads - 1) / kThreads;
   if (t == 0) {
     for (int i = 0; i < kBuffers; ++i) async::mbar_init(&full[i], 1);
     if constexpr (kC > 1)
       for (int i = 0; i < 2; ++i) async::mbar_init(&joined[i], 1);
     gave_up = 0;
-    async::fence_async();
   }
+  // what no row fills, up to a whole warp's vectors
+  for (int i = 0; i < kBuffers; ++i)
+    for (int v = cols / E + t; v < (vectors + 31) / 32 * 32; v += kThreads)
+      reinterpret_cast<uint4*>(buffers + i * kBuffer)[v] = minus_infinities<T>();
+  async::fence_async();
   __syncthreads();
   if constexpr (kC > 1) cg::this_cluster().sync();  // every block has started: its shared memory can be written
   const async::Bound bound{&gave_up, status, limit_ns};
-
-  // a row's part: of the logits, and of dx, whose rows lie alike to their vectors
-  const std::int64_t row0 = blockIdx.x / kC;
-  const char* x = reinterpret_cast<const char*>(static_cast<const T*>(a.x.p) + row0 * a.x.ld + first);
-  const std::int64_t x_step = clusters * a.x.ld * static_cast<std::int64_t>(sizeof(T));
-  auto shift_at = [](const char* p) {  // elements before the part in its first vector
-    return kWhole ? 0 : static_cast<int>(reinterpret_cast<std::uintptr_t>(p) & 15) / static_cast<int>(sizeof(T));
+  // The long way of a wait is a call, for which every thread keeps values in local
+  // memory, or inlined, which is more code in the loop. 192 or 204 us for 8192 rows of
+  // 32000 bf16, but 213 or 208 of 32001, 127 or 124 for 1024 rows of 128000.
+  auto wait = [&](std::uint64_t& bar, unsigned parity) {
+    if constexpr (kWhole && kC == 1)
+      async::wait(async::smem_u32(&bar), parity, bound);
+    else
+      async::wait_inline(async::smem_u32(&bar), parity, bound);
   };
 
-  auto request = [&] {  // the first warp: a row, a lane to a piece of it
+  // a row's part: of the logits, and of dx, whose rows lie alike to their vectors
+  const int row0 = blockIdx.x / kC;
+  const int turns = row0 < a.rows ? static_cast<int>((a.rows - row0 + clusters - 1) / clusters) : 0;
+  const char* x0 = reinterpret_cast<const char*>(static_cast<const T*>(a.x.p) + row0 * a.x.ld + first);
+
+  auto request = [&] {  // one warp: a row, a lane to a piece of it
     if (asked.row >= a.rows) return;
     const char* from = asked.x;
     const unsigned slot = asked.slot;
@@ -388,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
     __syncwarp();
     if (lane == 0) {
       async::mbar_expect_tx(&full[slot], bytes);
-      asked.x = from + x_step;
+      asked.x = from + clusters * a.x.ld * static_cast<std::int64_t>(sizeof(T));
       asked.row += clusters;
       asked.slot = slot + 1 < kBuffers ? slot + 1 : 0;
       if (asked.slot == 0) asked.round ^= 1u;
@@ -400,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
   };
   if (asks) {
     if (lane == 0) {
-      asked.x = x;
+      asked.x = x0;
       asked.row = row0;
       asked.slot = asked.round = 0;
     }
@@ -408,106 +429,122 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
     for (int i = 0; i < kBuffers; ++i) request();
   }
 
-  // Whether a vector of this thread is the part's, whole. The elements of a part
-  // before its first whole vector and after its last one, under E each, go to the
-  // lanes of one warp, one by one.
-  auto has = [&](int k, int shift) {
-    const int at = (k * kThreads + t) * E;
-    return kWhole ? at < cols : at >= shift && at + E <= shift + cols;
-  };
-  // this lane's such element, counted from the first vector; -1 without one
-  auto edge_of = [&](int shift) {
-    const int head = min(shift > 0 ? E - shift : 0, cols), tail = min((shift + cols) % E, cols - head);
-    return lane < head ? shift + lane : lane - head < tail ? shift + cols - tail + lane - head : -1;
-  };
-  async::Place begins;  // the buffer of the row that begins
-  auto vector_of = [&](int k) {
-    return reinterpret_cast<const uint4*>(buffers + begins.slot * kBuffer + k * kPiece) + t;
-  };
-  auto element = [&](int at) { return load(buffers + begins.slot * kBuffer, Elem<T>::kType, at); };
+  // elements before a part in its first vector
+  const int shift0 = kWhole ? 0 : shift_of(x0, sizeof(T)), shift_step = static_cast<int>(clusters * a.x.ld % E);
+  auto shift_at = [&](int turn) { return kWhole ? 0 : (shift0 + turn * shift_step) & (E - 1); };
+
+  // Whether a vector is one of this warp's.
+  auto holds = [&](int at) { return (at & (kThreads - 1)) >> 5 == warp; };
+  // a part ends in one of two vectors
+  const bool heads = !kWhole && warp == 0, tails = !kWhole && (holds(cols / E) || holds(cols / E + 1));
 
   // The sum (x) and the maximum (y) of the blocks of a row, to all threads.
-  async::Place set;
-  auto join = [&](float sum, float top) {
+  auto join = [&](int turn, float sum, float top) {
+    const int set = turn & 1;
     sum = warp_sum(sum);
     top = largest(top);
-    if (lane == 0) slots[set.slot][warp] = float2{sum, top};
+    if (lane == 0) slots[set][warp] = float2{sum, top};
     __syncthreads();  // also: nobody reads the finished row's buffer any more
-    float2 v = slots[set.slot][lane & (kWarps - 1)];
+    float2 v = slots[set][lane & (kWarps - 1)];
     v = float2{warp_sum(lane < kWarps ? v.x : 0.0f), largest(v.y)};
     if constexpr (kC > 1) {
       // slots and barriers come in two sets: a block that is a row ahead writes to
       // the other one, and it cannot be two ahead
-      if (t == 0) async::mbar_expect_tx(&joined[set.slot], kC * 8);
-      if (t < kC) send(&ranks[set.slot][rank], &joined[set.slot], t, v);
-      if (t == 0) async::wait(async::smem_u32(&joined[set.slot]), set.round, bound);
+      if (t == 0) async::mbar_expect_tx(&joined[set], kC * 8);
+      if (t < kC) send(&ranks[set][rank], &joined[set], t, v);
+      if (t == 0) wait(joined[set], turn >> 1 & 1);
       __syncthreads();
-      v = ranks[set.slot][lane & (kC - 1)];
+      v = ranks[set][lane & (kC - 1)];
       v = float2{warp_sum(lane < kC ? v.x : 0.0f), largest(v.y)};
     }
     return v;
   };
 
+  // The next row's target is asked for a turn before it is used.
+  auto ask_target = [&](int turn) {
+    if (turn < turns)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(async::smem_u32(&note.next_target[turn & 1])),
+                   "l"(a.target + row0 + static_cast<std::int64_t>(turn) * clusters)
+                   : "memory");
+  };
   if (notes && lane == 0) {
+    ask_target(0);
     note.target = a.ignore;
     note.f = 1.0f / (a.reduction == 1 ? a.work[0] : 1.0f);
+    note.m = note.logit = 0.0f;
     note.last_at = nullptr;
   }
-  // loads that are used a turn later: the next row's target, a row's logit there
-  std::int64_t next_target = notes && lane == 0 && row0 < a.rows ? a.target[row0] : a.ignore;
-  float logit = 0.0f;
-  auto counts = [&](std::int64_t t) { return t != a.ignore && !bad_target(a, t); };
+  __syncwarp();
+  auto counts = [&](std::int64_t target) { return target != a.ignore && !bad_target(a, target); };
+  auto owns = [&](std::int64_t target) { return counts(target) && target >= first && target - first < cols; };
+  // The target's gradient takes the place of what another thread wrote a turn ago,
+  // on the other side of a barrier.
+  auto late = [&] {
+    if (lane == 0 && note.last_at != nullptr) *note.last_at = Elem<T>::put(note.last_grad);
+  };
 
   float2 e[kVectors][E / 2];  // exponentials of the row that is finished next
-  float m = 0.0f, sum = 0.0f;
-  int shift = 0;
+  float sum = 0.0f;
   T* dx = static_cast<T*>(a.dx) + (row0 - clusters) * a.cols + first;  // of the row that is finished
-  bool finishes = false;  // the first turn has no row to finish, the last none to begin
-  for (std::int64_t row = row0;; row += clusters, begins.next(kBuffers), set.next(2)) {
-    const bool more = row < a.rows;
-    const int next_shift = shift_at(x);
+  // the first turn has no row to finish, the last none to begin
+  int turn = 0;
+  for (;; ++turn) {
+    const bool more = turn < turns;
+    const int set = turn & 1;
+    const unsigned third = static_cast<unsigned>(turn) / kBuffers, slot = turn - third * kBuffers;
+    const uint4* in = reinterpret_cast<const uint4*>(buffers + slot * kBuffer) + t;
     float top = -INFINITY;
     if (more) {
       // one lane of a warp asks: a thousand threads at a barrier are served one by one
-      if (lane == 0) async::wait(async::smem_u32(&full[begins.slot]), begins.round, bound);
+      if (lane == 0) wait(full[slot], third & 1u);
       __syncwarp();
+      if (heads || tails) {
+        // what is not the part's in its first vector, and from its end to the last one
+        const int before = shift_at(turn), end = before + cols + lane;
+        T* row = reinterpret_cast<T*>(buffers + slot * kBuffer);
+        if (heads && lane < before) row[lane] = Elem<T>::put(-INFINITY);
+        if (tails && end < vectors * E && holds(end / E)) row[end] = Elem<T>::put(-INFINITY);
+        __syncwarp();
+      }
 #pragma unroll
       for (int k = 0; k < kVectors; ++k)
-        if (has(k, next_shift)) top = larger(top, Row<T>::max(*vector_of(k)));
-      if (edges) {
-        const int at = edge_of(next_shift);
-        if (at >= 0) top = larger(top, element(at));
-      }
+        if (k < mine) top = larger(top, Row<T>::max(in[k * kThreads]));
     }
     if (notes && lane == 0)
-      factors[set.slot] = note.target == a.ignore ? 0.0f : bad_target(a, note.target) ? nan_value() : note.f;
-    const float2 v = join(sum, top);
-    if (asks && finishes) {
+      factors[set] = note.target == a.ignore ? 0.0f : bad_target(a, note.target) ? nan_value() : note.f;
+    const float2 v = join(turn, sum, top);
+    if (asks && turn > 0) {
       async::fence_async();
       request();
     }
-    const bool write = finishes && a.dx != nullptr;
-    const float factor = factors[set.slot], scale = factor * (1.0f / v.x);
-    if (write && factor == 0.0f) {  // an ignored row: zeros, whatever it holds
-      for (int i = t; i < cols; i += kThreads) dx[i] = Elem<T>::put(0.0f);
-    }
-    const bool gradient = write && factor != 0.0f;  // NaN too
+    const bool write = turn > 0 && a.dx != nullptr;
+    const float factor = factors[set], scale = factor * inverse_fast(v.x);
+    // whole vectors of the finished row, the first one with what comes before the part
+    const int shift = shift_at(turn - 1), whole = (shift + cols) / E;
+    uint4* out = reinterpret_cast<uint4*>(dx - shift) + t;
     float2 part_sum = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < kVectors; ++k) {
-      if (gradient && has(k, shift)) {
-        uint4 w;
-        if constexpr (sizeof(T) == 4) {
-          const float2 p = mul2(e[k][0], both(scale)), q = mul2(e[k][1], both(scale));
-          w = uint4{__float_as_uint(p.x), __float_as_uint(p.y), __float_as_uint(q.x), __float_as_uint(q.y)};
-        } else {
-          w = uint4{Elem<T>::put2(mul2(e[k][0], both(scale))), Elem<T>::put2(mul2(e[k][1], both(scale))),
-                    Elem<T>::put2(mul2(e[k][2], both(scale))), Elem<T>::put2(mul2(e[k][3], both(scale)))};
+      if (k >= mine) break;
+      if (write) {
+        uint4 w = {0, 0, 0, 0};
+        if (factor != 0.0f) {  // else an ignored row: zeros, whatever it holds
+          if constexpr (sizeof(T) == 4) {
+            const float2 p = mul2(e[k][0], both(scale)), q = mul2(e[k][1], both(scale));
+            w = uint4{__float_as_uint(p.x), __float_as_uint(p.y), __float_as_uint(q.x), __float_as_uint(q.y)};
+          } else {
+            w = uint4{Elem<T>::put2(mul2(e[k][0], both(scale))), Elem<T>::put2(mul2(e[k][1], both(scale))),
+                      Elem<T>::put2(mul2(e[k][2], both(scale))), Elem<T>::put2(mul2(e[k][3], both(scale)))};
+          }
         }
-        *reinterpret_cast<uint4*>(dx - shift + (k * kThreads + t) * E) = w;
+        const int at = k * kThreads + t;
+        if (at < whole && (kWhole || at > 0 || shift == 0))
+          out[k * kThreads] = w;
+        else if (!kWhole && (at == 0 || at == whole))
+          ends[at > 0] = w;
       }
-      if (more && has(k, next_shift)) {
-        const uint4 w = *vector_of(k);
+      if (more) {
+        const uint4 w = in[k * kThreads];
         float2 z[E / 2];
         if constexpr (sizeof(T) == 4) {
           z[0] = float2{__uint_as_float(w.x), __uint_as_float(w.y)};
@@ -523,42 +560,46 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
         }
       }
     }
-    if (edges) {
-      if (gradient && edge[lane] >= 0) dx[edge[lane] - shift] = Elem<T>::put(e_edge[lane] * scale);
-      if (more) {
-        const int at = edge_of(next_shift);
-        const float y = at >= 0 ? exp2_fast((element(at) - v.y) * kLog2e) : 0.0f;
-        part_sum.x += y;
-        edge[lane] = at;
-        e_edge[lane] = y;
-      }
+    if (write && (heads || tails)) {
+      __syncwarp();
+      T* row = dx - shift;
+      if (heads && (shift > 0 || whole == 0) && lane < E && lane >= shift && lane < shift + cols)
+        row[lane] = reinterpret_cast<const T*>(ends)[lane];
+      if (tails && whole > 0 && holds(whole) && lane < shift + cols - whole * E)
+        row[whole * E + lane] = reinterpret_cast<const T*>(ends + 1)[lane];
+      __syncwarp();
     }
-    if (notes && lane == 0) {
-      // The target's gradient takes the place of what another thread wrote a turn
-      // ago, on the other side of a barrier.
-      if (note.last_at != nullptr) *note.last_at = Elem<T>::put(note.last_grad);
-      note.last_at = nullptr;
-      if (finishes) {
-        if (rank == 0) finish_row(a, row - clusters, note.target == a.ignore, logit, m, v.x);
-        if (write && counts(note.target) && note.target >= first && note.target - first < cols) {
-          note.last_at = dx + (note.target - first);
-          note.last_grad = exp2_fast((logit - m) * kLog2e) * scale - factor;
+    if (notes) {
+      late();
+      if (lane == 0) {
+        note.last_at = nullptr;
+        const std::int64_t row = row0 + static_cast<std::int64_t>(turn) * clusters;
+        if (turn > 0) {
+          const bool owner = owns(note.target);
+          // the first block where no block has the target
+          if (owner || (rank == 0 && !counts(note.target)))
+            finish_row(a, row - clusters, note.target == a.ignore, note.logit, note.m, v.x);
+          if (write && owner) {
+            note.last_at = dx + (note.target - first);
+            note.last_grad = exp2_fast((note.logit - note.m) * kLog2e) * scale - factor;
+          }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        const std::int64_t target = note.next_target[set];
+        ask_target(turn + 1);
+        note.m = v.y;
+        note.target = target;
+        note.logit = more && owns(target)
+                         ? load(buffers + slot * kBuffer, Elem<T>::kType, shift_at(turn) + target - first)
+                         : nan_value();
       }
-      note.target = next_target;
-      logit = more && counts(next_target) ? load(a.x.p, a.x.t, row * a.x.ld + next_target) : nan_value();
-      next_target = row + clusters < a.rows ? a.target[row + clusters] : a.ignore;
     }
     if (!more) break;
     sum = part_sum.x + part_sum.y;
-    m = v.y;
-    shift = next_shift;
-    x += x_step;
     dx += clusters * a.cols;
-    finishes = true;
   }
   __syncthreads();
-  if (notes && lane == 0 && note.last_at != nullptr) *note.last_at = Elem<T>::put(note.last_grad);
+  if (notes) late();
   // shared memory outlives the copies, and what other blocks send, also where a wait gave up
   if (t == 0 && gave_up != 0)
     for (unsigned i = 0; i < kBuffers; ++i)

@@ -6,6 +6,7 @@
 // not a difference of moments, so a large mean costs no accuracy.
 // HBM-bound: about 10 operations an element.
 
+#include <atomic>
 #include <type_traits>
 
 #include "train_utils.cuh"
@@ -17,10 +18,12 @@ namespace {
 // Both passes hold a row in registers, so it is read once: `group` threads (whole
 // warps) share it, each with one or two parts of 8 neighbours, and groups walk
 // over rows. A thread keeps its columns from row to row, so the weights, and the
-// backward pass's sums of dw and db, stay in registers, and the next row is on its
-// way while one is worked on. Arithmetic is on pairs of elements. What bounds
-// both is half the memory and half the instructions: converting 16-bit values,
-// the group's reductions and the 8-bit form cost as many as the norm itself.
+// backward pass's sums of dw and db, stay on the SM, and the next row is on its way
+// while one is worked on. Arithmetic is on pairs of elements. What bounds both next to
+// the memory is how many rows are under way (registers) and the instructions: converting
+// 16-bit values, the group's reductions and the 8-bit form cost as many as the norm
+// itself. 32768 rows of 4096 bf16 take 105 us forward (5.1 TB/s), 135 with the 8-bit
+// form (5.0 TB/s), and 146 backward from it (4.6 TB/s).
 constexpr int kMaxGroup = 512;
 constexpr int kBlock = 256;  // threads of a block of several groups, about
 
@@ -111,6 +114,7 @@ struct FwdRow<X, None, kAligned, kParts> {
 
 template <typename X, typename Y, typename S, bool kAligned, int kParts>
 __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int group) {
+  extern __shared__ float4 params[];
   __shared__ float slots[2][kMaxGroup / 32];
   const int id = threadIdx.x / group, t = threadIdx.x - id * group, ids = blockDim.x / group, lane = threadIdx.x & 31;
   const int cols = static_cast<int>(a.cols), ng = static_cast<int>(held_groups(a.cols));
@@ -120,12 +124,26 @@ __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int
   std::int64_t row = static_cast<std::int64_t>(blockIdx.x) * ids + id;
   FwdRow<X, S, kAligned, kParts> in;
   if (row < a.rows) in.load(a, row, group, t);
-  float2 w[kParts][4], b[kParts][4] = {};
+  // Weights (0) and biases (1) of a thread's columns: one part's in registers, two
+  // parts' in shared memory (in two halves), so that twice as many rows are under way.
+  float2 kept[2][4];
+  auto at = [&](int which, int n, int half) { return params + ((which * kParts + n) * 2 + half) * group + t; };
 #pragma unroll
   for (int n = 0; n < kParts; ++n) {
-    load_any<kAligned>(a.w, a.wt, (n * group + t) * 8, cols, w[n]);
-    if (a.b != nullptr) load_any<kAligned>(a.b, a.wt, (n * group + t) * 8, cols, b[n]);
+    float2 w[4], b[4] = {};
+    load_any<kAligned>(a.w, a.wt, (n * group + t) * 8, cols, w);
+    if (a.b != nullptr) load_any<kAligned>(a.b, a.wt, (n * group + t) * 8, cols, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (kParts == 1) {
+        kept[0][i] = w[i], kept[1][i] = b[i];
+      } else if (id == 0 && i % 2 == 0) {
+        *at(0, n, i / 2) = float4{w[i].x, w[i].y, w[i + 1].x, w[i + 1].y};
+        *at(1, n, i / 2) = float4{b[i].x, b[i].y, b[i + 1].x, b[i + 1].y};
+      }
+    }
   }
+  if (kParts > 1) __syncthreads();
   for (; row < a.rows; row += stride) {
     float2 v[kParts][4];
 #pragma unroll
@@ -183,7 +201,17 @@ __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[n][i] = fma2(v[n][i], w[n][i], b[n][i]);
+      for (int half = 0; half < 2; ++half) {
+        float2* to = v[n] + 2 * half;
+        if constexpr (kParts == 1) {
+          to[0] = fma2(to[0], kept[0][2 * half], kept[1][2 * half]);
+          to[1] = fma2(to[1], kept[0][2 * half + 1], kept[1][2 * half + 1]);
+        } else {
+          const float4 w = *at(0, n, half), b = *at(1, n, half);
+          to[0] = fma2(to[0], float2{w.x, w.y}, float2{b.x, b.y});
+          to[1] = fma2(to[1], float2{w.z, w.w}, float2{b.z, b.w});
+        }
+      }
       Part<Y, kAligned>::store(static_cast<Y*>(a.y) + row * a.cols, c, cols, v[n], joined, last);
     }
   }
@@ -463,28 +491,33 @@ struct Walk {
   int parts, group, ids;  // parts 0: the row is too long, or its types are rare
 };
 
-Walk walk_of(std::int64_t cols, bool aligned, bool types, int ones) {
+// Two parts a thread halve the cost of a row's sums, where `two` says that their
+// registers allow it, unless a row then leaves much more of its last warp idle (768
+// columns are 96 threads of one part, or 48 of 64 of two).
+Walk walk_of(std::int64_t cols, bool aligned, bool types, bool two) {
   Walk p{};
   p.aligned = aligned;
-  // Two parts a thread halve the cost of a row's sums; up to `ones` columns one
-  // part fits a row better (768 columns are 96 threads of one, or 64 with 16
-  // idle), or the registers of two would spill.
-  p.parts = !types || cols > 16 * kMaxGroup ? 0 : cols <= ones ? 1 : 2;
-  if (p.parts == 0) return p;
-  p.group = static_cast<int>((cols + 8 * p.parts * 32 - 1) / (8 * p.parts * 32)) * 32;
+  if (!types || cols > 16 * kMaxGroup) return p;
+  const int warps1 = static_cast<int>((cols + 255) / 256), warps2 = static_cast<int>((cols + 511) / 512);
+  p.parts = cols > 8 * kMaxGroup || (two && 2 * warps2 * 4 <= warps1 * 5) ? 2 : 1;
+  p.group = 32 * (p.parts == 1 ? warps1 : warps2);
   p.ids = p.group < kBlock ? kBlock / p.group : 1;
   return p;
 }
 
 // Blocks that fill the GPU, or fewer where a group would have under `least` rows.
+// No more than run at once: the rest would walk over their rows after the others.
 template <auto kKernel>
-int blocks_of(const Walk& p, std::int64_t rows, int least) {
-  static const int registers = [] {
-    cudaFuncAttributes at;
-    return cudaFuncGetAttributes(&at, kKernel) == cudaSuccess ? (at.numRegs + 7) / 8 * 8 : 128;
-  }();
-  const int threads = p.group * p.ids, fit = 65536 / (registers * threads);
-  const std::int64_t most = static_cast<std::int64_t>(sm_count()) * (fit < 1 ? 1 : fit);
+int blocks_of(const Walk& p, std::int64_t rows, int least, int shared) {
+  static std::atomic<int> known[kMaxGroup / 32 + 1];  // blocks of an SM, by the warps of one
+  const int threads = p.group * p.ids;
+  int fit = known[threads / 32].load(std::memory_order_relaxed);
+  if (fit == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kKernel, threads, shared) != cudaSuccess || fit < 1)
+      fit = 1;
+    known[threads / 32].store(fit, std::memory_order_relaxed);
+  }
+  const std::int64_t most = static_cast<std::int64_t>(sm_count()) * fit;
   const std::int64_t each = static_cast<std::int64_t>(least) * p.ids, want = (rows + each - 1) / each;
   return static_cast<int>(want < most ? want : most);
 }
@@ -492,8 +525,12 @@ int blocks_of(const Walk& p, std::int64_t rows, int least) {
 Walk walk_of(const NormBwd& a) {
   const bool all = aligned(a.dy.p, a.dy.ld, a.cols) && aligned(a.ds.p, a.ds.ld, a.cols) &&
                    aligned(a.s.p, a.s.ld, a.cols) && aligned(a.w, a.cols, a.cols);
-  return walk_of(a.cols, all, paired(a.xt, a.dy.t) && (a.dr == nullptr || a.rt == a.dy.t),
-                 a.ds.p != nullptr ? 8 * kMaxGroup : 4 * kMaxGroup);
+  // One part or two: 97 or 87 us for 65536 rows of 1024 bf16, 110 or 85 from the 8-bit
+  // form. With a gradient of the stream as well two spill (185 or 253 us for 16384 rows
+  // of 4096 fp32), and unaligned rows have registers for two from the 8-bit form only
+  // (255 or 349 us for 32768 rows of 3001 bf16, 314 or 296).
+  const bool two = a.ds.p == nullptr && (all || a.q != nullptr);
+  return walk_of(a.cols, all, paired(a.xt, a.dy.t) && (a.dr == nullptr || a.rt == a.dy.t), two);
 }
 
 // Shares of the rows of a sweep over the columns.
@@ -505,25 +542,35 @@ int sweep_shares(const NormBwd& a) {
 
 constexpr int kMostPartials = 16;  // blocks an SM: 2 * 16 * 148 sums of a column at most
 
+constexpr int kParamBytes = 2 * 16 * static_cast<int>(sizeof(float));  // of a thread's two parts
+
 template <auto kKernel>
-void go_fwd(const NormFwd& a, const Walk& p, cudaStream_t stream) {
-  kKernel<<<blocks_of<kKernel>(p, a.rows, 1), p.group * p.ids, 0, stream>>>(a, p.group);
+cudaError_t go_fwd(const NormFwd& a, const Walk& p, cudaStream_t stream) {
+  const int shared = p.parts == 1 ? 0 : kParamBytes * p.group;
+  if (shared > 0) {
+    const cudaError_t rc = allow_shared<kKernel>(kParamBytes * kMaxGroup);
+    if (rc != cudaSuccess) return rc;
+  }
+  kKernel<<<blocks_of<kKernel>(p, a.rows, 1, shared), p.group * p.ids, shared, stream>>>(a, p.group);
+  return cudaSuccess;
 }
 
 template <typename X, typename Y, typename S>
-void launch_fwd(const NormFwd& a, const Walk& p, cudaStream_t stream) {
+cudaError_t launch_fwd(const NormFwd& a, const Walk& p, cudaStream_t stream) {
   if (p.aligned)
-    p.parts == 1 ? go_fwd<norm_fwd<X, Y, S, true, 1>>(a, p, stream) : go_fwd<norm_fwd<X, Y, S, true, 2>>(a, p, stream);
-  else
-    p.parts == 1 ? go_fwd<norm_fwd<X, Y, S, false, 1>>(a, p, stream)
-                 : go_fwd<norm_fwd<X, Y, S, false, 2>>(a, p, stream);
+    return p.parts == 1 ? go_fwd<norm_fwd<X, Y, S, true, 1>>(a, p, stream)
+                        : go_fwd<norm_fwd<X, Y, S, true, 2>>(a, p, stream);
+  return p.parts == 1 ? go_fwd<norm_fwd<X, Y, S, false, 1>>(a, p, stream)
+                      : go_fwd<norm_fwd<X, Y, S, false, 2>>(a, p, stream);
 }
 
 template <auto kKernel>
 int go_bwd(const NormBwd& a, const Walk& p, float* part, cudaStream_t stream) {
-  int blocks = blocks_of<kKernel>(p, a.rows, 4);
+  // a group's columns, or fewer; known by the threads of a block too
+  const int shared = p.ids > 1 ? 2 * 8 * static_cast<int>(sizeof(float)) * p.parts * p.group : 0;
+  int blocks = blocks_of<kKernel>(p, a.rows, 4, shared);
   if (blocks > kMostPartials * sm_count()) blocks = kMostPartials * sm_count();
-  kKernel<<<blocks, p.group * p.ids, p.ids > 1 ? 2 * sizeof(float) * a.cols : 0, stream>>>(a, p.group, part);
+  kKernel<<<blocks, p.group * p.ids, shared, stream>>>(a, p.group, part);
   return blocks;
 }
 
@@ -538,8 +585,11 @@ int launch_bwd(const NormBwd& a, const Walk& p, float* part, cudaStream_t stream
 cudaError_t norm_forward(const NormFwd& a, cudaStream_t stream) {
   const bool all = aligned(a.x.p, a.x.ld, a.cols) && aligned(a.r.p, a.r.ld, a.cols) && aligned(a.w, a.cols, a.cols) &&
                    aligned(a.b, a.cols, a.cols);
+  // One part or two: 131 or 107 us for 32768 rows of 4096 bf16; unaligned rows, 119 or
+  // 135 us for 65536 of 1001 bf16, but 162 or 107 us for 32768 of fp32 with a residual.
   const Walk p = walk_of(a.cols, all, paired(a.x.t, a.yt) && (a.r.p == nullptr || a.r.t == a.x.t || a.r.t == a.yt),
-                         8 * kMaxGroup);
+                         all || a.x.t == Type::f32);
+  cudaError_t rc = cudaSuccess;
   if (p.parts == 0) {
     const std::int64_t most = 32ll * sm_count();
     norm_fwd_sweep<<<static_cast<unsigned>(a.rows < most ? a.rows : most), kSweep, 0, stream>>>(a);
@@ -548,13 +598,14 @@ cudaError_t norm_forward(const NormFwd& a, cudaStream_t stream) {
       using X = decltype(x);
       using Y = decltype(y);
       if (a.r.p == nullptr)
-        launch_fwd<X, Y, None>(a, p, stream);
+        rc = launch_fwd<X, Y, None>(a, p, stream);
       else if (a.r.t == a.x.t)
-        launch_fwd<X, Y, X>(a, p, stream);
+        rc = launch_fwd<X, Y, X>(a, p, stream);
       else
-        launch_fwd<X, Y, Y>(a, p, stream);
+        rc = launch_fwd<X, Y, Y>(a, p, stream);
     });
   }
+  if (rc != cudaSuccess) return rc;
   commux_ops::g_launches++;
   return cudaGetLastError();
 }

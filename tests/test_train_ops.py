@@ -578,6 +578,55 @@ def test_cross_entropy_many_rows(rows, cols, dtype):
     assert dx[7].eq(0).all()
 
 
+@gpu
+@pytest.mark.parametrize("rows,cols", [(80, 5003), (80, 9001), (80, 16385), (160, 32001), (150, 32004), (75, 64001),
+                                       (75, 128257), (75, 9000)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_cross_entropy_targets_at_ends(rows, cols, dtype):
+    # the first and last elements of a row, and of what each of 2, 4 or 8 blocks has of it
+    g = gen(rows + 2 * cols)
+    x = randn(g, rows, cols, dtype=dtype, scale=2.0).requires_grad_()
+    places = [*range(9), *range(cols - 9, cols)]
+    for n in (2, 4, 8):
+        for k in range(1, n):
+            at = (-(-cols // n) + 7) // 8 * 8 * k
+            places += [at - 1, at]
+    places = [q for q in places if q < cols]
+    target = torch.tensor([places[i % len(places)] for i in range(rows)], device="cuda")
+    target[3::13] = -100
+    loss = ops.cross_entropy(x, target)
+    (dx,) = torch.autograd.grad(loss, x)
+    each, grad, mag, valid = xent64(x.detach().double(), target, -100)
+    n = valid.sum()
+    size = x.detach().double().abs().amax(1) + 16
+    close(loss.detach(), each.sum() / n, (size * valid).sum() / n, 32 + rows / 32, "loss")
+    close(dx, grad / n, mag / n, 16, "dx")
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(9000, 512), (6000, 768), (6000, 1024), (5000, 1001), (3000, 3000), (2500, 4096),
+                                       (1500, 6001)])
+@pytest.mark.parametrize("pack,residual", [(False, False), (True, False), (True, True)])
+def test_layer_norm_rows_alone(rows, cols, pack, residual):
+    # a row's results do not depend on which rows are there besides it
+    g = gen(rows + cols)
+    x, dy = randn(g, rows, cols, dtype=BF16), randn(g, rows, cols, dtype=BF16)
+    r = randn(g, rows, cols, dtype=BF16) if residual else None
+    w, b = randn(g, cols, dtype=BF16), randn(g, cols, dtype=BF16)
+
+    def run(part):
+        xs = x[part].clone().requires_grad_()
+        y, *rest = ops.layer_norm(xs, w, b, residual=r[part] if residual else None, pack=True) if pack else (
+            ops.layer_norm(xs, w, b),)
+        return [y.detach(), torch.autograd.grad(y, xs, dy[part])[0]] + ([rest[-1].q] if pack else [])
+
+    whole = run(slice(0, rows))
+    for first in (0, rows // 2, rows - 40):
+        part = slice(first, first + 40)
+        for got, want in zip(whole, run(part)):
+            assert torch.equal(got[part], want)
+
+
 # --- gradients against differences -------------------------------------------
 
 def _differences(f, xs, seed, step=2.0 ** -7):

@@ -2,8 +2,10 @@
 //   s = x + r,  h = (s - mean) / sqrt(var + eps),  y = w h + b
 //   dx = rstd (g - mean(g) - h mean(g h)) + ds with g = w dy,
 //   dw = sum over rows of dy h,  db = sum over rows of dy.
-// The variance is the mean square of s - mean (a second pass over the row),
-// not a difference of moments, so a large mean costs no accuracy.
+// The mean is the sum's quotient, off by its roundings, and what s - mean sums up
+// to (a second pass over the row) corrects it. The variance is the mean square of
+// s - mean, less that correction's, and not a difference of moments. So a large
+// mean costs no accuracy, and a constant row has no variance.
 // HBM-bound: about 10 operations an element.
 
 #include <atomic>
@@ -115,7 +117,7 @@ struct FwdRow<X, None, kAligned, kParts> {
 template <typename X, typename Y, typename S, bool kAligned, int kParts>
 __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int group) {
   extern __shared__ float4 params[];
-  __shared__ float slots[2][kMaxGroup / 32];
+  __shared__ float slots[kMaxGroup / 32], slots2[32 * (kMaxGroup / 64)];  // a group of one warp uses none
   const int id = threadIdx.x / group, t = threadIdx.x - id * group, ids = blockDim.x / group, lane = threadIdx.x & 31;
   const int cols = static_cast<int>(a.cols), ng = static_cast<int>(held_groups(a.cols));
   const float inv = 1.0f / static_cast<float>(cols);
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int
       }
     }
     if (row + stride < a.rows) in.load(a, row + stride, group, t);
-    float2 sum = {0.0f, 0.0f}, sq = {0.0f, 0.0f};
+    float2 sum = {0.0f, 0.0f}, rest = {0.0f, 0.0f}, sq = {0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < kParts; ++n) {
       if constexpr (!std::is_same<S, None>::value)
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum = add2(sum, v[n][i]);  // 0 past the row's end
     }
-    const float mean = group_sum(sum.x + sum.y, group, id, slots[0] + id * (group >> 5)) * inv;
+    const float mean = group_sum(sum.x + sum.y, group, id, slots + id * (group >> 5)) * inv;
 #pragma unroll
     for (int n = 0; n < kParts; ++n) {
       const int left = cols - (n * group + t) * 8;
@@ -179,20 +181,31 @@ __global__ void __launch_bounds__(kMaxGroup) norm_fwd(const NormFwd a, const int
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sq = fma2(v[n][i], v[n][i], sq);
+      for (int i = 0; i < 4; ++i) {
+        rest = add2(rest, v[n][i]);
+        sq = fma2(v[n][i], v[n][i], sq);
+      }
     }
-    const float var = group_sum(sq.x + sq.y, group, id, slots[1] + id * (group >> 5)) * inv;
+    const float2 joined2 = group_sum2(float2{rest.x + rest.y, sq.x + sq.y}, group, id, slots2 + id * 32);
+    const float off = joined2.x * inv, var = larger(joined2.y * inv - off * off, 0.0f);
     const float rstd = rsqrtf(var + a.eps);
     if (t == 0 && a.rstd != nullptr) {
       a.rstd[row] = rstd;
-      if (a.mean != nullptr) a.mean[row] = mean;
+      if (a.mean != nullptr) a.mean[row] = mean + off;
     }
 #pragma unroll
     for (int n = 0; n < kParts; ++n) {
       const int c = (n * group + t) * 8;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[n][i] = mul2(v[n][i], both(rstd));
+      for (int i = 0; i < 4; ++i) v[n][i] = fma2(v[n][i], both(rstd), both(-off * rstd));
       if (a.q != nullptr) {
+        if (cols - c < 8) {  // zeros past the row's end
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (c + 2 * i >= cols) v[n][i].x = 0.0f;
+            if (c + 2 * i + 1 >= cols) v[n][i].y = 0.0f;
+          }
+        }
         uint2 q;
         const unsigned e = pack_eight(v[n], q);
         if (c < ng * kGroup) {
@@ -384,20 +397,23 @@ __global__ void __launch_bounds__(kSweep) norm_fwd_sweep(const NormFwd a) {
       sum += v;
     }
     const float mean = block_sum(sum, slots) / static_cast<float>(a.cols);
-    float sq = 0.0f;
+    float rest = 0.0f, sq = 0.0f;
     for (std::int64_t i = threadIdx.x; i < a.cols; i += kSweep) {
       const float d = stream(i) - mean;
+      rest += d;
       sq += d * d;
     }
-    const float rstd = rsqrtf(block_sum(sq, slots) / static_cast<float>(a.cols) + a.eps);
+    const float off = block_sum(rest, slots) / static_cast<float>(a.cols);
+    const float var = larger(block_sum(sq, slots) / static_cast<float>(a.cols) - off * off, 0.0f);
+    const float rstd = rsqrtf(var + a.eps);
     if (threadIdx.x == 0) {
-      if (a.mean != nullptr) a.mean[row] = mean;
+      if (a.mean != nullptr) a.mean[row] = mean + off;
       if (a.rstd != nullptr) a.rstd[row] = rstd;
     }
     for (std::int64_t i = threadIdx.x; i < ng * kGroup; i += kSweep) {  // whole warps
       float h = 0.0f;
       if (i < a.cols) {
-        h = (stream(i) - mean) * rstd;
+        h = (stream(i) - mean - off) * rstd;
         const float y = h * load(a.w, a.wt, i) + (a.b != nullptr ? load(a.b, a.wt, i) : 0.0f);
         store(a.y, a.yt, oo + i, y);
       }

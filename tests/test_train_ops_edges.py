@@ -1,0 +1,52 @@
+"""The training operators (commux_b200.ops.train) at the edges of their ranges:
+long sums, constant and far rows, orders that are copied, devices' waits that
+give up, rows of more than 2^31 elements, and the ways through the kernels that
+common sizes do not take."""
+
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from commux_b200 import ops
+
+gpu = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def gen(seed=0):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32, scale=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+# --- layer norm of rows whose mean is far from their deviation ------------------
+
+@gpu
+@pytest.mark.parametrize("cols", [7, 41, 96, 768, 1000, 3001, 4100, 8192, 10007])
+@pytest.mark.parametrize("value", [1000.0, 1000.1, -0.3, 12345.678])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_layer_norm_constant_rows(cols, value, dtype):
+    # A constant row is its own mean. The mean of its sum (25 roundings one after the
+    # other at most) is off by 2^-19 of it, what corrects the mean by 2^-19 of that, and
+    # the normalised values are the rest times rstd = eps^-1/2 = 316. Its 8-bit form too.
+    x = torch.full((3, cols), value, dtype=dtype, device="cuda").requires_grad_()
+    w, b = torch.full((cols,), 2.0, device="cuda"), torch.full((cols,), 0.5, device="cuda")
+    far = 2.0 ** -38 * abs(value) * 317
+    y, kept = ops.layer_norm(x, w, b, pack=True)
+    assert ((y.detach().float() - 0.5).abs() <= 2 * far + 2.0 ** -24).all(), float((y.float() - 0.5).abs().max())
+    assert (ops.Act8(kept.q, kept.scale, kept.shape, F32).unpack().abs() <= 1.01 * far).all()
+    y = ops.layer_norm(x, w, b)
+    dy = randn(gen(cols), 3, cols, dtype=dtype)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    # the mean that the backward pass keeps is the value itself: h = 0
+    g = dy.double() * 2
+    want = (g - g.mean(1, keepdim=True)) / math.sqrt(1e-5)
+    tol = 2.0 ** {F32: -20, BF16: -8, F16: -10}[dtype] * 317 * (g.abs() + g.abs().mean(1, keepdim=True))
+    assert ((dx.double() - want).abs() <= tol).all()

@@ -271,14 +271,16 @@ struct BwdRow {
     }
   }
 
-  // past the row's end 0 (packed) or -mean * rstd, which meets a dy of 0
+  // 0 past the row's end: -mean * rstd there would meet a dy of 0, but it can be
+  // infinite where no normalised value of the row is
   __device__ __forceinline__ void normalised(int n, float2 (&h)[4]) const {
     if constexpr (kHeld) {
       unpack_eight(q[n], e[n], h);
     } else {
-      s[n].get(h);
+      s[n].get(h, mean);
+      const float m = kAligned && s[n].left <= 0 ? 0.0f : mean;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = mul2(add2(h[i], both(-mean)), both(rstd));
+      for (int i = 0; i < 4; ++i) h[i] = mul2(add2(h[i], both(-m)), both(rstd));
     }
   }
 };

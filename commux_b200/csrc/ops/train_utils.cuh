@@ -107,7 +107,7 @@ struct Elem<__half> {
 
 // A thread's part of a row: the 8 elements from column c, a multiple of 8, as
 // four pairs; a warp's lanes hold parts that follow each other. Columns past
-// the row's end read as 0 and are not written.
+// the row's end read as 0 (or as get()'s fill) and are not written.
 //
 // kAligned: rows are whole numbers of parts on 16-byte boundaries. Otherwise a
 // row begins `shift` elements after such a boundary, a part lies across two
@@ -141,7 +141,8 @@ struct Part {
     }
   }
 
-  __device__ __forceinline__ void get(float2 (&v)[4]) const {
+  // `fill`: what columns past the end of an unaligned row become
+  __device__ __forceinline__ void get(float2 (&v)[4], float fill = 0.0f) const {
     unsigned u[4 * kVectors];
 #pragma unroll
     for (int i = 0; i < 4 * kVectors; ++i) u[i] = w[i];
@@ -169,8 +170,8 @@ struct Part {
     if (!kAligned && left < 8) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (2 * i >= left) v[i].x = 0.0f;
-        if (2 * i + 1 >= left) v[i].y = 0.0f;
+        if (2 * i >= left) v[i].x = fill;
+        if (2 * i + 1 >= left) v[i].y = fill;
       }
     }
   }

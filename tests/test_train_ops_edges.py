@@ -50,3 +50,18 @@ def test_layer_norm_constant_rows(cols, value, dtype):
     want = (g - g.mean(1, keepdim=True)) / math.sqrt(1e-5)
     tol = 2.0 ** {F32: -20, BF16: -8, F16: -10}[dtype] * 317 * (g.abs() + g.abs().mean(1, keepdim=True))
     assert ((dx.double() - want).abs() <= tol).all()
+
+
+@gpu
+@pytest.mark.parametrize("cols", [7, 33, 77, 100])
+def test_layer_norm_backward_of_huge_rows(cols):
+    # 2^120 / sqrt(eps) is no fp32 number, and no element of the row has it: a constant
+    # row's normalised values are zero, and so is all that the columns beyond it add
+    x = torch.full((3, cols), 2.0 ** 120, device="cuda").requires_grad_()
+    w = torch.ones(cols, device="cuda").requires_grad_()
+    dy = randn(gen(1), 3, cols)
+    dx, dw = torch.autograd.grad(ops.layer_norm(x, w), (x, w), dy)
+    g = dy.double()
+    want = (g - g.mean(1, keepdim=True)) / math.sqrt(1e-5)
+    assert ((dx.double() - want).abs() <= 2.0 ** -20 * 317 * (g.abs() + g.abs().mean(1, keepdim=True))).all()
+    assert dw.eq(0).all()

@@ -8,7 +8,8 @@
 // sums. q s is exact in bf16 (see act8.cu), so the 8-bit form is widened on its
 // way into shared memory, and only 33/32 bytes an element are read. dy enters
 // as 1, 2 or 3 bf16 terms (bf16, fp16, fp32: 8, 11, 24 significant bits, each
-// term the next 8 of them), so the products are exact for every type.
+// term the next 8 of them), so the products are exact for every type. The terms
+// are further tokens of the same sums, the smallest terms first.
 //
 // 16384 tokens, 4096 x 4096: 451 us for the tiles (1.22 PFLOP/s) and 28 us to join
 // partial tiles; 8192 tokens, 768 x 3072, fp32 results: 51 and 7 us.
@@ -52,15 +53,20 @@ constexpr int kSlot = kM * kN + kM;           // floats of a partial tile: sums,
 // may begin and end inside a tile. A tile that one pair holds whole is written
 // at once, the others' parts go to slots that wgrad_join adds up in order.
 //
-// Tensor memory's fp32 sums are cut off, not rounded, at every 16 tokens, so a
-// sum shrinks with its length: by 4e-7, 9e-7 and 2.4e-6 of itself over 1024, 2048
-// and 4096 tokens. fp32 results are therefore summed over `cut` steps at most in
-// there, and a part's sums of those are added up, rounded, in its slot. For 16-bit
-// results, rounded by 2^-9 or more in the end, no part is cut.
+// Tensor memory's fp32 sums are cut off, not rounded, at every 16 tokens, so a sum
+// of products of one sign shrinks with its length: by 1.8e-6, 5.5e-5 and 1.2e-3 of
+// itself over 1536, 16384 and 200000 tokens. Results are therefore summed over `cut`
+// steps of dy's leading term at most in there, and a part's sums of those are added
+// up, rounded, in its slot: 1536 tokens for fp32 results, 8 and 32 times as many for
+// fp16 and bf16, whose sums then shrink by less than a tenth of half their unit. The
+// lower terms come first: what cuts off sums of theirs is 2^-8 of that, where between the leading
+// terms' products each of them would cut off the whole sum once more (1.7e-5 over
+// 1536 tokens of fp32, 2.1e-3 over 200000 of fp16).
 constexpr int kCut = 1536 / kK;
 struct Plan {
   std::int64_t rows, cols, outs, groups;
-  int tiles_n, tiles, steps, pairs, planes, cut, slots;  // slots of a pair
+  int tiles_n, tiles, pairs, cut, slots;  // slots of a pair
+  int span, lower, steps;                 // steps of one term of dy, of all but the leading one, of all
   __host__ __device__ std::int64_t begin(int pair) const {
     return static_cast<std::int64_t>(tiles) * steps * pair / pairs;
   }
@@ -180,6 +186,18 @@ __device__ __forceinline__ void load_sums(float (&v)[32], std::uint32_t at) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// Where a step's tokens and their term of dy are.
+struct Step {
+  int tile, term;
+  __device__ __forceinline__ Step(const Plan& p, int k) : tile(k % p.span), term(p.lower / p.span - k / p.span) {}
+  __device__ __forceinline__ void next(const Plan& p) {
+    if (++tile == p.span) {
+      tile = 0;
+      --term;
+    }
+  }
+};
+
 struct Segment {  // what a pair sums up in one go: (a cut of) its part of a tile
   int tile, first, last;  // steps [first, last)
   bool whole;             // the part is all of the tile
@@ -195,9 +213,11 @@ __device__ __forceinline__ Segment segment(const Plan& p, std::int64_t at, std::
   const int now = static_cast<int>(at - tile0);
   const int part0 = begin > tile0 ? static_cast<int>(begin - tile0) : 0;
   const int part1 = end < tile0 + p.steps ? static_cast<int>(end - tile0) : p.steps;
-  const int cuts = (part1 - part0 + p.cut - 1) / p.cut, size = (part1 - part0 + cuts - 1) / cuts;
+  // steps of the leading term are cut; what comes before them belongs to the first cut
+  const int lead = part0 > p.lower ? part0 : p.lower, cuts = part1 > lead ? (part1 - lead + p.cut - 1) / p.cut : 1;
+  const int size = (part1 - lead + cuts - 1) / cuts, last = (now > lead ? now : lead) + size;
   s.first = now;
-  s.last = now + size < part1 ? now + size : part1;
+  s.last = last < part1 ? last : part1;
   s.whole = part0 == 0 && part1 == p.steps;
   s.begins = now == part0;
   s.ends = s.last == part1;
@@ -213,31 +233,26 @@ __device__ __forceinline__ Segment segment(const Plan& p, std::int64_t at, std::
 // Row of the tile of a CTA's local row (0 to 255): 128 of each half
 __device__ __forceinline__ int tile_row(int local, int rank) { return (local >> 7) * 256 + rank * 128 + (local & 127); }
 
-// kOne: dy is one bf16 term. Then a step has one dy tile, and one barrier tells
-// the products that everything of a step is there and another that it was read:
-// the thread that issues the products is the narrowest place of the kernel (it
-// cost twice the products' time with a wait for each tile).
-template <bool kOne>
+// One barrier tells the products that everything of a step is there and another
+// that it was read: the thread that issues the products is the narrowest place of
+// the kernel (it cost twice the products' time with a wait for each tile).
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     wgrad_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_q, const Plan p,
                 const Out out, const std::uint8_t* scale, unsigned* status, std::uint64_t limit_ns) {
   extern __shared__ unsigned char raw[];
   unsigned char* smem = raw + ((1024u - (async::smem_u32(raw) & 1023u)) & 1023u);
-  // Barriers, by their addresses. In both CTAs: tiles of its own, widened tiles
-  // that were read, results. Used in CTA 0, which issues the products: peer_a (the
-  // other CTA's dy tiles are there), full_b (both have widened), sums_empty (both
-  // have the results). With kOne, done replaces empty_b and the products' part of
-  // empty_a, and full_b includes dy's tiles.
+  // Barriers, by their addresses. In both CTAs: tiles of its own, steps whose tiles
+  // were read (done), results. Used in CTA 0, which issues the products: full_b (both
+  // have widened, and have their dy tiles), sums_empty (both have the results).
   const std::uint32_t base = async::smem_u32(smem), bars = base + kOffBars;
   const std::uint32_t full_a = bars, empty_a = full_a + 8 * kStages, full_q = empty_a + 8 * kStages,
-                      empty_q = full_q + 8 * kStages, peer_a = empty_q + 8 * kStages, full_b = peer_a + 8 * kStages,
-                      empty_b = full_b + 8 * kWide, sums_full = empty_b + 8 * kWide, sums_empty = sums_full + 8,
-                      turned = sums_full + 16, column_full = sums_full + 24, drained = sums_full + 32,
-                      done = sums_full + 40;
-  constexpr int kAfter = kOffBars + 8 * (5 * kStages + 2 * kWide + 5 + kDone);
+                      empty_q = full_q + 8 * kStages, full_b = empty_q + 8 * kStages, sums_full = full_b + 8 * kWide,
+                      sums_empty = sums_full + 8, turned = sums_full + 16, column_full = sums_full + 24,
+                      drained = sums_full + 32, done = sums_full + 40;
+  constexpr int kAfter = kOffBars + 8 * (4 * kStages + kWide + 5 + kDone);
   std::uint32_t* tmem_at = reinterpret_cast<std::uint32_t*>(smem + kAfter);
   volatile int* gave_up = reinterpret_cast<volatile int*>(smem + kAfter + 8);
-  static_assert((5 * kStages + 2 * kWide + 7 + kDone) * 8 <= kBarBytes, "barriers");
+  static_assert((4 * kStages + kWide + 7 + kDone) * 8 <= kBarBytes, "barriers");
   static_assert(kConvert * 32 * 32 * 4 <= kWide * kBytesB, "the results are turned round in the widened tiles");
   __shared__ float column[kM / 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -247,15 +262,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       async::init(full_a + 8 * s, 1);
-      async::init(empty_a + 8 * s, (kOne ? 0 : 1) + kColumn);
+      async::init(empty_a + 8 * s, kColumn);
       async::init(full_q + 8 * s, 1 + kScale);
       async::init(empty_q + 8 * s, kConvert);
-      async::init(peer_a + 8 * s, 1);
     }
-    for (int s = 0; s < kWide; ++s) {
-      async::init(full_b + 8 * s, 2 * kConvert);
-      async::init(empty_b + 8 * s, 1);
-    }
+    for (int s = 0; s < kWide; ++s) async::init(full_b + 8 * s, 2 * kConvert);
     async::init(sums_full, 1);
     async::init(sums_empty, 2 * kConvert);
     async::init(turned, kConvert);
@@ -285,7 +296,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // All lanes go through the loop and one issues, here and for the products: the
     // addresses then stay in the warp's uniform registers.
     const bool chosen = async::elect();
-    async::Place ia, iq, freed;  // freed: the step whose read frees this one's dy tile
+    async::Place place, freed;  // freed: the step whose read frees this one's dy tile
     std::int64_t loaded_a = 0, loaded_q = 0;
     bool ok = true;
     for (std::int64_t at = begin; ok && at < end;) {
@@ -298,33 +309,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         m[b] = s.m0 + tile_row(64 * b, rank);
         boxes += m[b] < p.outs;
       }
-      for (int k = s.first; ok && k < s.last; ++k) {
-        ok = __all_sync(0xffffffffu, async::wait(empty_q + 8 * iq.slot, iq.round ^ 1u, bound));
+      Step step(p, s.first);
+      for (int k = s.first; k < s.last; ++k) {
+        ok = __all_sync(0xffffffffu, async::wait(empty_q + 8 * place.slot, place.round ^ 1u, bound));
         if (!ok) break;
         if (chosen) {
-          async::expect_tx(full_q + 8 * iq.slot, kBytesQ);
-          async::load_2d(base + kOffQ + iq.slot * kBytesQ, &map_q, n0, k * kK, full_q + 8 * iq.slot);
+          async::expect_tx(full_q + 8 * place.slot, kBytesQ);
+          async::load_2d(base + kOffQ + place.slot * kBytesQ, &map_q, n0, step.tile * kK, full_q + 8 * place.slot);
         }
-        iq.next(kStages);
         ++loaded_q;
-        for (int pl = 0; pl < (kOne ? 1 : p.planes); ++pl) {
-          ok = async::wait(empty_a + 8 * ia.slot, ia.round ^ 1u, bound);
-          if (kOne && loaded_a >= kStages) {
-            ok = ok && async::wait(done + 8 * freed.slot, freed.round, bound);
-            freed.next(kDone);
-          }
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (chosen) {
-            async::expect_tx(full_a + 8 * ia.slot, boxes * kBox);
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-              if (m[b] < p.outs)
-                async::load_3d(base + ia.slot * kBytesA + b * kBox, &map_a, m[b], k * kK, pl, full_a + 8 * ia.slot);
-          }
-          ia.next(kStages);
-          ++loaded_a;
+        ok = async::wait(empty_a + 8 * place.slot, place.round ^ 1u, bound);
+        if (loaded_a >= kStages) {
+          ok = ok && async::wait(done + 8 * freed.slot, freed.round, bound);
+          freed.next(kDone);
         }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (chosen) {
+          async::expect_tx(full_a + 8 * place.slot, boxes * kBox);
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (m[b] < p.outs)
+              async::load_3d(base + place.slot * kBytesA + b * kBox, &map_a, m[b], step.tile * kK, step.term,
+                             full_a + 8 * place.slot);
+        }
+        ++loaded_a;
+        place.next(kStages);
+        step.next(p);
       }
       at += s.last - s.first;
     }
@@ -333,16 +344,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       async::settle(full_a + 8 * static_cast<unsigned>(i % kStages), static_cast<unsigned>(i / kStages) & 1u, limit_ns);
     for (std::int64_t i = loaded_q > kStages ? loaded_q - kStages : 0; !ok && i < loaded_q; ++i)
       async::settle(full_q + 8 * static_cast<unsigned>(i % kStages), static_cast<unsigned>(i / kStages) & 1u, limit_ns);
-  } else if (warp == 1 && rank == 1) {  // --- tells CTA 0 of this CTA's dy tiles
-    if (!kOne && lane == 0) {
-      const std::uint32_t there = leaders(peer_a);
-      async::Place ia;
-      for (std::int64_t n = (end - begin) * p.planes; n > 0; --n) {
-        if (!async::wait(full_a + 8 * ia.slot, ia.round, bound)) break;
-        arrive_there(there + 8 * ia.slot);
-        ia.next(kStages);
-      }
-    }
+  } else if (warp == 1 && rank == 1) {  // CTA 0 issues the products of both
   } else if (warp == 1) {  // --- products
     const bool chosen = async::elect();
     async::Place ia, ib, steps;
@@ -356,25 +358,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       unsigned add = 0;
       for (int k = s.first; ok && k < s.last; ++k) {
         ok = __all_sync(0xffffffffu, async::wait<true>(full_b + 8 * ib.slot, ib.round, bound));
-        const unsigned b = b0 + ib.slot * (kBytesB >> 4);
-        for (int pl = 0; ok && pl < (kOne ? 1 : p.planes); ++pl) {
-          if (!kOne) {
-            ok = async::wait(full_a + 8 * ia.slot, ia.round, bound) &&
-                 async::wait<true>(peer_a + 8 * ia.slot, ia.round, bound);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const unsigned a = a0 + ia.slot * (kBytesA >> 4);
-          if (chosen) {
-            mma_step(tmem, a, b, form, add);
-            if (s.halves == 2) mma_step(tmem + kN, a + (2 * kBox >> 4), b, form, add);
-            if (!kOne) commit(empty_a + 8 * ia.slot);
-          }
-          add = 1;
-          ia.next(kStages);
+        if (!ok) break;
+        const unsigned a = a0 + ia.slot * (kBytesA >> 4), b = b0 + ib.slot * (kBytesB >> 4);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (chosen) {
+          mma_step(tmem, a, b, form, add);
+          if (s.halves == 2) mma_step(tmem + kN, a + (2 * kBox >> 4), b, form, add);
+          commit(done + 8 * steps.slot);
         }
-        if (ok && chosen) commit(kOne ? done + 8 * steps.slot : empty_b + 8 * ib.slot);
+        add = 1;
+        ia.next(kStages);
         ib.next(kWide);
         steps.next(kDone);
       }
@@ -398,9 +391,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool busy = in * 8 < s.n / 2;
       for (int k = s.first; k < s.last; ++k) {
         ok = async::wait(full_q + 8 * iq.slot, iq.round, bound);
-        if (!kOne) {
-          ok = ok && async::wait(empty_b + 8 * ib.slot, ib.round ^ 1u, bound);
-        } else if (widened < kWide) {
+        if (widened < kWide) {
           ++widened;
         } else {
           ok = ok && async::wait(done + 8 * freed.slot, freed.round, bound);
@@ -436,10 +427,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           async::arrive(empty_q + 8 * iq.slot);
           // one warp's arrival stands for dy's tile too; its places are the 8-bit
           // tile's. The others have arrived long before.
-          if (kOne && cw == 0) ok = async::wait(full_a + 8 * iq.slot, iq.round, bound);
+          if (cw == 0) ok = async::wait(full_a + 8 * iq.slot, iq.round, bound);
           if (ok) arrive_there(leaders_b + 8 * ib.slot);
         }
-        if (kOne) ok = __all_sync(0xffffffffu, ok);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         iq.next(kStages);
         ib.next(kWide);
@@ -523,8 +514,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const std::int64_t group = (s.n0 + rank * (s.n / 2)) / kGroup, left = p.groups - group;
       const int some = static_cast<int>(left < kEach ? left : kEach);
       unsigned ahead[2][kEach];
+      Step step(p, s.first);  // what is fetched next
       auto fetch = [&](int k, unsigned (&e)[kEach]) {
-        const std::int64_t t = static_cast<std::int64_t>(k) * kK + token;
+        const std::int64_t t = static_cast<std::int64_t>(step.tile) * kK + token;
+        step.next(p);
         const std::uint8_t* from = scale + t * p.groups + group;
         const bool in = k < s.last && t < p.rows;
 #pragma unroll
@@ -563,7 +556,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Segment s = segment(p, at, begin, end);
       const bool busy = sums_columns(s) && s.m0 + tile_row(64 * block, rank) < p.outs;
       if (s.begins) v0 = v1 = 0.0f;  // a part's cuts go on
-      for (std::int64_t k = static_cast<std::int64_t>(s.last - s.first) * p.planes; k > 0; --k) {
+      for (int k = s.first; k < s.last; ++k) {
         ok = __all_sync(0xffffffffu, async::wait(full_a + 8 * ia.slot, ia.round, bound));
         if (!ok) break;
         if (busy) {
@@ -658,15 +651,15 @@ __global__ void __launch_bounds__(kJoinThreads) wgrad_join(const Plan p, const O
   }
 }
 
-// dy as `planes` bf16 terms, [planes][rows][ld]: each term the leading 8 bits of
+// dy as `terms` bf16 terms, [terms][rows][ld]: each term the leading 8 bits of
 // what the terms before it left (cut off, not rounded, so no term overflows).
-__global__ void __launch_bounds__(256) wgrad_terms(Rows dy, __nv_bfloat16* to, int planes, std::int64_t rows,
+__global__ void __launch_bounds__(256) wgrad_terms(Rows dy, __nv_bfloat16* to, int terms, std::int64_t rows,
                                                    std::int64_t outs, std::int64_t ld) {
   const std::int64_t n = rows * ld;
   for (std::int64_t at = blockIdx.x * 256ll + threadIdx.x; at < n; at += gridDim.x * 256ll) {
     const std::int64_t t = at / ld, o = at - t * ld;
     float v = o < outs ? load(dy.p, dy.t, t * dy.ld + o) : 0.0f;
-    for (int p = 0; p < planes; ++p) {
+    for (int p = 0; p < terms; ++p) {
       const bool finite = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
       // a NaN whose bits are all in the lower half stays one
       const unsigned bits = v != v ? 0x7fc00000u : __float_as_uint(v) & 0xffff0000u;
@@ -698,7 +691,7 @@ bool as_it_is(const Wgrad8& a) {
          a.dy.ld >= a.outs;
 }
 
-int planes_of(Type t) { return t == Type::bf16 ? 1 : t == Type::f16 ? 2 : 3; }
+int terms_of(Type t) { return t == Type::bf16 ? 1 : t == Type::f16 ? 2 : 3; }
 
 Plan plan_of(const Wgrad8& a) {
   Plan p;
@@ -706,10 +699,11 @@ Plan plan_of(const Wgrad8& a) {
   p.cols = a.cols;
   p.outs = a.outs;
   p.groups = groups(a.cols);
-  p.planes = planes_of(a.dy.t);
   p.tiles_n = static_cast<int>((a.cols + kN - 1) / kN);
   p.tiles = static_cast<int>((a.outs + kM - 1) / kM) * p.tiles_n;
-  p.steps = static_cast<int>((a.rows + kK - 1) / kK);
+  p.span = static_cast<int>((a.rows + kK - 1) / kK);
+  p.lower = (terms_of(a.dy.t) - 1) * p.span;
+  p.steps = p.lower + p.span;
   // One CTA an SM. Where whole shares of the tiles fill nearly all of them,
   // every pair has one part of one tile; otherwise parts may cross tiles. No
   // tile is cut into parts under 4 steps, which cost about what a pair's start
@@ -722,8 +716,8 @@ Plan plan_of(const Wgrad8& a) {
   const std::int64_t most = (total + 3) / 4 > p.tiles ? (total + 3) / 4 : p.tiles;
   if (n > most) n = most;
   p.pairs = static_cast<int>(n);
-  p.cut = a.dwt == Type::f32 && p.steps > kCut ? kCut : p.steps;
-  p.slots = p.cut < p.steps ? 3 : 2;
+  p.cut = kCut << (a.dwt == Type::f32 ? 0 : a.dwt == Type::f16 ? 3 : 5);
+  p.slots = p.cut < p.span ? 3 : 2;
   return p;
 }
 
@@ -736,20 +730,21 @@ std::int64_t terms_ld(const Wgrad8& a) { return (a.outs + 7) / 8 * 8; }
 
 std::int64_t wgrad8_work(const Wgrad8& a) {
   const Plan p = plan_of(a);
-  return slots_bytes(p) + (as_it_is(a) ? 0 : 2ll * p.planes * a.rows * terms_ld(a));
+  return slots_bytes(p) + (as_it_is(a) ? 0 : 2ll * terms_of(a.dy.t) * a.rows * terms_ld(a));
 }
 
 cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
   const EncodeTiledFn encode = encode_tiled();
   if (encode == nullptr) return cudaErrorNotSupported;
   const Plan p = plan_of(a);
+  const int count = terms_of(a.dy.t);
   const void* dy = a.dy.p;
   std::int64_t ld = a.dy.ld;
   if (!as_it_is(a)) {
     auto* terms = reinterpret_cast<__nv_bfloat16*>(static_cast<char*>(a.work) + slots_bytes(p));
     ld = terms_ld(a);
     const std::int64_t want = (a.rows * ld + 255) / 256, most = 32ll * sm_count();
-    wgrad_terms<<<static_cast<unsigned>(want < most ? want : most), 256, 0, stream>>>(a.dy, terms, p.planes, a.rows,
+    wgrad_terms<<<static_cast<unsigned>(want < most ? want : most), 256, 0, stream>>>(a.dy, terms, count, a.rows,
                                                                                      a.outs, ld);
     commux_ops::g_launches++;
     dy = terms;
@@ -757,7 +752,7 @@ cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
   CUtensorMap map_a, map_q;
   const cuuint32_t one[3] = {1, 1, 1};
   const cuuint64_t dim_a[3] = {static_cast<cuuint64_t>(a.outs), static_cast<cuuint64_t>(a.rows),
-                               static_cast<cuuint64_t>(p.planes)};
+                               static_cast<cuuint64_t>(count)};
   const cuuint64_t stride_a[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(ld) * 2 * a.rows};
   const cuuint32_t box_a[3] = {64, kK, 1};
   const cuuint64_t dim_q[2] = {static_cast<cuuint64_t>(p.groups) * kGroup, static_cast<cuuint64_t>(a.rows)};
@@ -770,14 +765,13 @@ cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
-  const auto kernel = p.planes == 1 ? wgrad_tiles<true> : wgrad_tiles<false>;
-  const cudaError_t set =
-      p.planes == 1 ? allow_shared<wgrad_tiles<true>>(kSmem) : allow_shared<wgrad_tiles<false>>(kSmem);
+  const cudaError_t set = allow_shared<wgrad_tiles>(kSmem);
   if (set != cudaSuccess) return set;
   const Out out{a.dw, a.db, a.dwt, a.w, a.b, a.wt, static_cast<float*>(a.work)};
   unsigned* status = nullptr;
   commux_ops::status_word(&status);
-  kernel<<<2 * p.pairs, kThreads, kSmem, stream>>>(map_a, map_q, p, out, a.scale, status, commux_ops::wait_limit_ns());
+  wgrad_tiles<<<2 * p.pairs, kThreads, kSmem, stream>>>(map_a, map_q, p, out, a.scale, status,
+                                                        commux_ops::wait_limit_ns());
   commux_ops::g_launches++;
   bool joined = false;
   for (int c = 1; c < p.pairs && !joined; ++c) joined = p.begin(c) % p.steps != 0;

@@ -65,3 +65,46 @@ def test_layer_norm_backward_of_huge_rows(cols):
     want = (g - g.mean(1, keepdim=True)) / math.sqrt(1e-5)
     assert ((dx.double() - want).abs() <= 2.0 ** -20 * 317 * (g.abs() + g.abs().mean(1, keepdim=True))).all()
     assert dw.eq(0).all()
+
+
+# --- long sums of the weight gradient -------------------------------------------
+
+def _one_sign(rows, dtype, out):
+    """weight_grad8 of products of one sign, whose losses add up, and its values in 64 bits
+    (some columns). So many columns that every pair of blocks has sums over all tokens."""
+    cols, outs = 74 * 256, 512
+    g = gen(rows)
+    q = torch.randint(1, 128, (rows, cols), generator=g, device="cuda", dtype=torch.int8)
+    scale = torch.full((rows, cols // 32), 120, dtype=torch.uint8, device="cuda")
+    spread = 1 + torch.rand(outs, generator=g, device="cuda")  # results all over a binade
+    dy = (torch.rand(rows, outs, generator=g, device="cuda") * spread / 16).to(dtype)
+    dw = ops.weight_grad8(dy, ops.Act8(q, scale, (rows, cols), dtype), out_dtype=out)
+    some = torch.arange(0, cols, 37, device="cuda")
+    want = torch.zeros(outs, len(some), dtype=torch.float64, device="cuda")
+    for k in range(0, rows, 50_000):
+        want += dy[k:k + 50_000].double().t() @ (q[k:k + 50_000][:, some].double() / 128)
+    return dw[:, some].double(), want
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows", [1536, 5000])
+def test_weight_grad8_sums_do_not_shrink(rows, dtype):
+    # What tensor memory cuts off is half a unit on average at each of 96 additions of
+    # a sum, which is half its final size on average, and 2^-24 of that size is half a
+    # unit at most. It does not depend on the number of terms that dy comes in.
+    dw, want = _one_sign(rows, dtype, F32)
+    off = float((dw - want).norm() / want.norm())
+    assert off <= 96 * 2.0 ** -25, off
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_weight_grad8_long_sums_in_16_bits(dtype):
+    # Rounded to nearest, results are off to both sides alike: the mean of 262144 relative
+    # errors (over 512 different sizes) is u / 50 by chance. Cut-off sums stay under a
+    # tenth of u, half a unit of the type.
+    u = {F16: 2.0 ** -11, BF16: 2.0 ** -8}[dtype]
+    dw, want = _one_sign(200_000, dtype, dtype)
+    off = float(((dw - want) / want).mean())
+    assert dw.isfinite().all() and abs(off) <= u * (0.1 + 0.02), off / u

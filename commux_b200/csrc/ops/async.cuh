@@ -95,12 +95,11 @@ template <bool kCluster>
 __device__ __forceinline__ bool wait_here(std::uint32_t bar, unsigned parity, volatile int* gave_up, unsigned* status,
                                           std::uint64_t limit_ns) {
   std::uint64_t since = 0;
-  for (unsigned tries = 1; !try_wait<kCluster>(bar, parity); ++tries) {
-    if (tries % 64 != 0) continue;  // the timer and the flag in one of many tries
+  while (!try_wait<kCluster>(bar, parity)) {  // which itself blocks for up to 4 us
     if (*gave_up != 0) return false;
     const std::uint64_t now = gtimer();
     if (since == 0) since = now;
-    if (now - since > limit_ns) {
+    if (now - since >= limit_ns) {
       *gave_up = 1;
       if (status != nullptr) atomicExch(status, 1u);
       return false;
@@ -158,9 +157,12 @@ __device__ __forceinline__ void load_3d(std::uint32_t dst, const CUtensorMap* ma
       : "memory");
 }
 
-// A last wait, for what is in flight after another wait gave up.
-__device__ __forceinline__ void settle(std::uint32_t bar, unsigned parity, std::uint64_t limit_ns) {
-  for (const std::uint64_t t0 = gtimer(); !try_wait<false>(bar, parity) && gtimer() - t0 <= limit_ns;) {
+// A last wait, for a CTA's copies in flight before it ends. Copies arrive within
+// microseconds; the bound, which no setting changes, is for a barrier that also
+// counts arrivals of threads that gave up.
+constexpr std::uint64_t kSettleNs = 20'000'000;
+__device__ __forceinline__ void settle(std::uint32_t bar, unsigned parity) {
+  for (const std::uint64_t t0 = gtimer(); !try_wait<false>(bar, parity) && gtimer() - t0 <= kSettleNs;) {
   }
 }
 

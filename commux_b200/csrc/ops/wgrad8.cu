@@ -233,6 +233,31 @@ __device__ __forceinline__ Segment segment(const Plan& p, std::int64_t at, std::
 // Row of the tile of a CTA's local row (0 to 255): 128 of each half
 __device__ __forceinline__ int tile_row(int local, int rank) { return (local >> 7) * 256 + rank * 128 + (local & 127); }
 
+// NaN in a CTA's rows of its pair's tiles, or parts of tiles, of which some were not summed up.
+__device__ __noinline__ void poison(const Plan& p, const Out& out, std::int64_t begin, std::int64_t end, int pair,
+                                    int rank) {
+  const float nan = __int_as_float(0x7fffffff);
+  for (std::int64_t at = begin; at < end;) {
+    const Segment s = segment(p, at, begin, end);
+    float* slot = out.slots + (static_cast<std::int64_t>(p.slots) * pair + s.slot) * kSlot;
+    for (int k = threadIdx.x; k < kM / 2 * kN; k += kThreads) {
+      const int row = tile_row(k / kN, rank), col = k % kN;
+      const std::int64_t o = s.m0 + row, i = s.n0 + col;
+      if (!s.whole)
+        slot[row * kN + col] = nan;
+      else if (o < p.outs && i < p.cols)
+        store(out.dw, out.dwt, o * p.cols + i, nan);
+      if (col > 0) continue;
+      if (!s.whole)
+        slot[kM * kN + row] = nan;
+      else if (o < p.outs && s.n0 == 0 && out.db != nullptr)
+        store(out.db, out.dwt, o, nan);
+    }
+    const std::int64_t tile_end = static_cast<std::int64_t>(s.tile + 1) * p.steps;
+    at = tile_end < end ? tile_end : end;
+  }
+}
+
 // One barrier tells the products that everything of a step is there and another
 // that it was read: the thread that issues the products is the narrowest place of
 // the kernel (it cost twice the products' time with a wait for each tile).
@@ -255,6 +280,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   static_assert((4 * kStages + kWide + 7 + kDone) * 8 <= kBarBytes, "barriers");
   static_assert(kConvert * 32 * 32 * 4 <= kWide * kBytesB, "the results are turned round in the widened tiles");
   __shared__ float column[kM / 2];
+  __shared__ int others_gave_up;  // in the other CTA
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pair = static_cast<int>(blockIdx.x >> 1), rank = static_cast<int>(blockIdx.x & 1);
   const async::Bound bound{gave_up, status, limit_ns};
@@ -273,7 +299,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     async::init(column_full, kColumn);
     async::init(drained, 1);
     for (int s = 0; s < kDone; ++s) async::init(done + 8 * s, 1);
-    *gave_up = 0;
+    *gave_up = others_gave_up = 0;
     async::fence_async();
   }
   if (warp == 1) {
@@ -339,11 +365,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       at += s.last - s.first;
     }
-    // the CTA's shared memory outlives the copies also where a wait gave up
-    for (std::int64_t i = loaded_a > kStages ? loaded_a - kStages : 0; !ok && i < loaded_a; ++i)
-      async::settle(full_a + 8 * static_cast<unsigned>(i % kStages), static_cast<unsigned>(i / kStages) & 1u, limit_ns);
-    for (std::int64_t i = loaded_q > kStages ? loaded_q - kStages : 0; !ok && i < loaded_q; ++i)
-      async::settle(full_q + 8 * static_cast<unsigned>(i % kStages), static_cast<unsigned>(i / kStages) & 1u, limit_ns);
+    // the CTA's shared memory outlives the copies, also where a wait gave up, here or elsewhere
+    for (std::int64_t i = loaded_a > kStages ? loaded_a - kStages : 0; i < loaded_a; ++i)
+      async::settle(full_a + 8 * static_cast<unsigned>(i % kStages), static_cast<unsigned>(i / kStages) & 1u);
+    for (std::int64_t i = loaded_q > kStages ? loaded_q - kStages : 0; i < loaded_q; ++i)
+      async::settle(full_q + 8 * static_cast<unsigned>(i % kStages), static_cast<unsigned>(i / kStages) & 1u);
   } else if (warp == 1 && rank == 1) {  // CTA 0 issues the products of both
   } else if (warp == 1) {  // --- products
     const bool chosen = async::elect();
@@ -354,7 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (std::int64_t at = begin; ok && at < end; ++seg) {
       const Segment s = segment(p, at, begin, end);
       const unsigned form = mma_form(s.n);
-      ok = async::wait<true>(sums_empty, seg & 1u ^ 1u, bound);
+      ok = __all_sync(0xffffffffu, async::wait<true>(sums_empty, seg & 1u ^ 1u, bound));
       unsigned add = 0;
       for (int k = s.first; ok && k < s.last; ++k) {
         ok = __all_sync(0xffffffffu, async::wait<true>(full_b + 8 * ib.slot, ib.round, bound));
@@ -373,10 +399,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (ok && chosen) commit(sums_full);
       at += s.last - s.first;
-    }
-    if (!ok) {  // products in flight read shared memory and write tensor memory
-      if (chosen) commit(drained);
-      async::settle(drained, 0, limit_ns);
     }
   } else if (warp < 2 + kConvert) {  // --- widening, and the results
     // A warp takes two tokens' 128 columns at a time, a lane 8 of them: 8 bytes
@@ -590,7 +612,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  sync_pair();  // neither CTA's memory is in use by the other
+  if (threadIdx.x == 0 && *gave_up != 0) {
+    std::uint32_t there;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(async::smem_u32(&others_gave_up)), "r"(rank ^ 1));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(1) : "memory");
+  }
+  sync_pair();  // neither CTA's memory is in use by the other, unless a wait gave up
+  if (*gave_up != 0 || *const_cast<volatile int*>(&others_gave_up) != 0) {
+    // products in flight read shared memory and write tensor memory of both CTAs
+    if (warp == 1) {
+      if (rank == 0 && async::elect()) commit(drained);  // the thread that issued them
+      __syncwarp();
+      async::settle(drained, 0);
+    }
+    poison(p, out, begin, end, pair, rank);
+    sync_pair();
+  }
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }

@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
   // shared memory outlives the copies, and what other blocks send, also where a wait gave up
   if (t == 0 && gave_up != 0)
     for (unsigned i = 0; i < kBuffers; ++i)
-      async::settle(async::smem_u32(&full[i]), i < asked.slot ? asked.round : asked.round ^ 1u, limit_ns);
+      async::settle(async::smem_u32(&full[i]), i < asked.slot ? asked.round : asked.round ^ 1u);
   if constexpr (kC > 1) cg::this_cluster().sync();
 }
 

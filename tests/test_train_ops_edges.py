@@ -7,6 +7,9 @@ import math
 import os
 import subprocess
 import sys
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -108,3 +111,17 @@ def test_weight_grad8_long_sums_in_16_bits(dtype):
     dw, want = _one_sign(200_000, dtype, dtype)
     off = float(((dw - want) / want).mean())
     assert dw.isfinite().all() and abs(off) <= u * (0.1 + 0.02), off / u
+
+
+# --- waits that run out -------------------------------------------------------------
+
+def _wait_worker(what, limit_ms):
+    worker = os.path.join(ROOT, "tests", "workers", "train_waits.py")
+    env = dict(os.environ, COMMUX_KERNEL_WAIT_MS=limit_ms, PYTHONPATH=ROOT)
+    r = subprocess.run([sys.executable, worker, what], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and "PASS" in r.stdout, r.stdout[-3000:] + r.stderr[-3000:]
+
+
+@gpu
+def test_weight_grad8_waits_that_run_out():
+    _wait_worker("weight_grad8", "0")

@@ -1,0 +1,59 @@
+"""Bounded waits of the training operators' kernels that run out: run with
+COMMUX_KERNEL_WAIT_MS=0, where a wait gives up at its first look that finds
+nothing. No result may look like one that is not: each is right or NaN, the
+status says so, and the device stays usable."""
+
+import sys
+
+import torch
+
+from commux_b200 import _ops, ops
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+U = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+g = torch.Generator(device="cuda").manual_seed(1)
+
+
+def randn(*shape, dtype=F32):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def right_or_nan(got, want, tol, what):
+    torch.cuda.synchronize()
+    status = _ops.kernel_status(True)
+    bad = ~(got.isnan() | ((got.double() - want).abs() <= tol))
+    assert not bad.any(), (what, int(bad.sum()), bad.numel())
+    assert status != 0 or not got.isnan().any(), what
+    return status != 0, float(got.isnan().double().mean())
+
+
+def weight_grad8():
+    nans = []
+    for rows, cols, outs, dtype, out, norm in [(8192, 768, 3072, BF16, F32, False),
+                                               (4096, 74 * 256, 512, BF16, BF16, True),
+                                               (4096, 700, 500, F32, F32, True), (3000, 1000, 90, F16, F16, False)]:
+        x, dy = randn(rows, cols, dtype=BF16), randn(rows, outs, dtype=dtype)
+        w, b = (1 + 0.2 * randn(cols), randn(cols)) if norm else (None, None)
+        kept = ops.layer_norm(x, w, b, pack=True)[1] if norm else ops.pack8(x)
+        v = ops.Act8(kept.q, kept.scale, kept.shape, F32).unpack()
+        mag = v.abs()
+        if norm:
+            v, mag = v * w + b, mag * w.abs() + b.abs()
+        d = dy.double()
+        want, size = d.t() @ v.double(), d.abs().t() @ mag.double()
+        dw, db = ops.weight_grad8(dy, kept, bias=True, out_dtype=out)
+        ran_out, some = right_or_nan(dw, want, 1.01 * U[out] * want.abs() + (rows + 64) * 2.0 ** -24 * size, "dw")
+        want = d.sum(0)
+        assert (db.isnan() | ((db.double() - want).abs() <= 1.01 * U[out] * want.abs()
+                              + (rows + 64) * 2.0 ** -24 * d.abs().sum(0))).all()
+        print(f"weight_grad8 {rows} {cols} {outs}: {100 * some:.1f} % NaN", flush=True)
+        nans.append(ran_out and some)
+    # in a short sum nothing takes longer than one look, which itself waits for 4 us
+    assert max(nans) > 0
+
+
+if __name__ == "__main__":
+    globals()[sys.argv[1]]()
+    x = torch.arange(1000, device="cuda")
+    assert int(x.sum()) == 499500
+    print("PASS")

@@ -128,6 +128,13 @@ __device__ __forceinline__ bool wait_inline(std::uint32_t bar, unsigned parity, 
   return wait_here<false>(bar, parity, b.gave_up, b.status, b.limit_ns);
 }
 
+// For blocks of a cluster whose last stores to each other's shared memory nobody
+// waited for.
+__device__ __forceinline__ void pause() {
+  for (const std::uint64_t t0 = gtimer(); gtimer() - t0 < 1'000'000;) {
+  }
+}
+
 __device__ __forceinline__ void arrive(std::uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }

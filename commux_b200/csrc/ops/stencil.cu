@@ -46,7 +46,7 @@ unsigned* status_word(unsigned** dev) {
 std::uint64_t wait_limit_ns() {
   static const std::uint64_t v = [] {
     const char* e = std::getenv("COMMUX_KERNEL_WAIT_MS");
-    return static_cast<std::uint64_t>(e ? std::atoll(e) : 2000) * 1000000ull;
+    return static_cast<std::uint64_t>((e ? std::max(std::atof(e), 0.0) : 2000.0) * 1e6);
   }();
   return v;
 }

@@ -325,6 +325,31 @@ __device__ __forceinline__ void send(float2* to, std::uint64_t* bar, int rank, f
                : "memory");
 }
 
+// A block's part of every row: parts begin on whole vectors of the columns.
+template <int E, int kC>
+struct Share {
+  int first, cols;
+  __device__ __forceinline__ Share(std::int64_t all, int rank) {
+    const std::int64_t share = ((all + kC - 1) / kC + E - 1) / E * E;
+    first = static_cast<int>(share * rank);
+    cols = static_cast<int>(all - first < share ? (all > first ? all - first : 0) : share);
+  }
+};
+
+// Rows that a block did not finish, since a wait gave up in its turn `left` (from 1):
+// NaN in its part of their gradients, in their losses and in what a later pass reads.
+// The turn before that one's row was not finished either.
+template <typename T, int kC>
+__device__ __forceinline__ void poison(const Xent& a, int left) {
+  const Share<16 / sizeof(T), kC> part(a.cols, blockIdx.x % kC);
+  const int clusters = gridDim.x / kC;
+  for (std::int64_t row = blockIdx.x / kC + (left > 1 ? left - 2ll : 0) * clusters; row < a.rows; row += clusters) {
+    T* dx = static_cast<T*>(a.dx) + row * a.cols + part.first;
+    for (int i = threadIdx.x; a.dx != nullptr && i < part.cols; i += blockDim.x) dx[i] = Elem<T>::put(nan_value());
+    if (threadIdx.x == 0) finish_row(a, row, false, nan_value(), nan_value(), nan_value());
+  }
+}
+
 // kWhole: every row lies in whole vectors. Where one does not, its buffer holds
 // other rows' elements before and after its own. The warp that owns such a vector
 // overwrites them with -inf, so that all threads may take all vectors as they are
@@ -340,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
   __shared__ float2 slots[2][kWarps], ranks[2][8];  // (sum of a row, maximum of the next)
   __shared__ float factors[2];                      // of a row's gradient
   __shared__ uint4 ends[2];                         // a gradient's first and last vector
-  __shared__ int gave_up;
+  __shared__ int gave_up, left_at;  // left_at: the turn, from 1, in which a wait gave up
   // What single warps keep from row to row is in shared memory too: registers
   // would hold it in every thread, and the exponentials need them.
   __shared__ struct {
@@ -364,10 +389,8 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
   int rank = 0;
   if constexpr (kC > 1) rank = cg::this_cluster().block_rank();
   const int clusters = gridDim.x / kC;
-  // this block's part of every row; parts begin on whole vectors of the columns
-  const std::int64_t share = ((a.cols + kC - 1) / kC + E - 1) / E * E;
-  const int first = static_cast<int>(share * rank);
-  const int cols = static_cast<int>(a.cols - first < share ? (a.cols > first ? a.cols - first : 0) : share);
+  const Share<E, kC> part(a.cols, rank);
+  const int first = part.first, cols = part.cols;
   const int vectors = cols == 0 ? 0 : kWhole ? cols / E : (cols + 2 * E - 2) / E;  // that a part may touch
   // vectors of this warp's threads
   const int mine = (vectors - warp * 32 + kThreads - 1) / kThreads;
@@ -375,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
     for (int i = 0; i < kBuffers; ++i) async::mbar_init(&full[i], 1);
     if constexpr (kC > 1)
       for (int i = 0; i < 2; ++i) async::mbar_init(&joined[i], 1);
-    gave_up = 0;
+    gave_up = left_at = 0;
   }
   // what no row fills, up to a whole warp's vectors
   for (int i = 0; i < kBuffers; ++i)
@@ -388,12 +411,16 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
   // The long way of a wait is a call, for which every thread keeps values in local
   // memory, or inlined, which is more code in the loop. 192 or 204 us for 8192 rows of
   // 32000 bf16, but 213 or 208 of 32001, 127 or 124 for 1024 rows of 128000.
-  auto wait = [&](std::uint64_t& bar, unsigned parity) {
-    if constexpr (kWhole && kC == 1)
-      async::wait(async::smem_u32(&bar), parity, bound);
-    else
-      async::wait_inline(async::smem_u32(&bar), parity, bound);
+  auto wait = [&](std::uint64_t& bar, unsigned parity, int turn) {
+    if constexpr (kWhole && kC == 1) {
+      if (!async::wait(async::smem_u32(&bar), parity, bound)) left_at = turn + 1;
+    } else {
+      if (!async::wait_inline(async::smem_u32(&bar), parity, bound)) left_at = turn + 1;
+    }
   };
+  // Whether the block leaves in this turn. Asked after a barrier behind the turn's
+  // waits, so that all threads leave: one that is a turn ahead may have given up there.
+  auto leaves = [&](int turn) { return left_at != 0 && left_at <= turn + 1; };
 
   // a row's part: of the logits, and of dx, whose rows lie alike to their vectors
   const int row0 = blockIdx.x / kC;
@@ -450,9 +477,10 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
     if constexpr (kC > 1) {
       // slots and barriers come in two sets: a block that is a row ahead writes to
       // the other one, and it cannot be two ahead
+      if (leaves(turn)) v = float2{nan_value(), nan_value()};  // the other blocks' rows are not what they should be
       if (t == 0) async::mbar_expect_tx(&joined[set], kC * 8);
       if (t < kC) send(&ranks[set][rank], &joined[set], t, v);
-      if (t == 0) wait(joined[set], turn >> 1 & 1);
+      if (t == 0) wait(joined[set], turn >> 1 & 1, turn);
       __syncthreads();
       v = ranks[set][lane & (kC - 1)];
       v = float2{warp_sum(lane < kC ? v.x : 0.0f), largest(v.y)};
@@ -496,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
     float top = -INFINITY;
     if (more) {
       // one lane of a warp asks: a thousand threads at a barrier are served one by one
-      if (lane == 0) wait(full[slot], third & 1u);
+      if (lane == 0) wait(full[slot], third & 1u, turn);
       __syncwarp();
       if (heads || tails) {
         // what is not the part's in its first vector, and from its end to the last one
@@ -513,6 +541,7 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
     if (notes && lane == 0)
       factors[set] = note.target == a.ignore ? 0.0f : bad_target(a, note.target) ? nan_value() : note.f;
     const float2 v = join(turn, sum, top);
+    if (leaves(turn)) break;
     if (asks && turn > 0) {
       async::fence_async();
       request();
@@ -601,10 +630,18 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
   __syncthreads();
   if (notes) late();
   // shared memory outlives the copies, and what other blocks send, also where a wait gave up
-  if (t == 0 && gave_up != 0)
-    for (unsigned i = 0; i < kBuffers; ++i)
-      async::settle(async::smem_u32(&full[i]), i < asked.slot ? asked.round : asked.round ^ 1u);
+  if (left_at != 0) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (t == 0) {
+      for (unsigned i = 0; i < kBuffers; ++i)
+        async::settle(async::smem_u32(&full[i]), i < asked.slot ? asked.round : asked.round ^ 1u);
+      if constexpr (kC > 1) async::pause();
+    }
+    __syncthreads();
+  }
   if constexpr (kC > 1) cg::this_cluster().sync();
+  // after whatever the row's other blocks wrote
+  if (left_at != 0) poison<T, kC>(a, left_at);
 }
 
 // --- rows longer than a cluster's registers, and gradients formed again ---

@@ -125,3 +125,9 @@ def _wait_worker(what, limit_ms):
 @gpu
 def test_weight_grad8_waits_that_run_out():
     _wait_worker("weight_grad8", "0")
+
+
+@gpu
+@pytest.mark.parametrize("limit_ms", ["0", "0.004"])
+def test_cross_entropy_waits_that_run_out(limit_ms):
+    _wait_worker("cross_entropy", limit_ms)

@@ -1,8 +1,9 @@
 """Bounded waits of the training operators' kernels that run out: run with
-COMMUX_KERNEL_WAIT_MS=0, where a wait gives up at its first look that finds
-nothing. No result may look like one that is not: each is right or NaN, the
+COMMUX_KERNEL_WAIT_MS=0, where a wait gives up after its first looks (a look
+blocks for 4 us), or a few microseconds. No result may look like one that is not: each is right or NaN, the
 status says so, and the device stays usable."""
 
+import os
 import sys
 
 import torch
@@ -50,6 +51,42 @@ def weight_grad8():
         nans.append(ran_out and some)
     # in a short sum nothing takes longer than one look, which itself waits for 4 us
     assert max(nans) > 0
+
+
+def cross_entropy():
+    given_up = 0
+    for rows, cols, dtype in [(700, 9001, BF16), (600, 32000, BF16), (500, 32001, F32), (300, 20000, F32),
+                              (160, 120001, BF16), (150, 128256, BF16), (20, 32000, F32), (9, 140001, F16)]:
+        x = randn(rows, cols, dtype=dtype).requires_grad_()
+        target = torch.randint(0, cols, (rows,), generator=g, device="cuda")
+        target[::7] = -100
+        z = x.detach().double()
+        ls = torch.log_softmax(z, 1)
+        valid = target != -100
+        at = torch.where(valid, target, 0)[:, None]
+        each = torch.where(valid, -ls.gather(1, at)[:, 0], 0)
+        p = torch.exp(ls)
+        grad = (p - torch.zeros_like(p).scatter_(1, at, 1.0)) * valid[:, None]
+        # its rounding, a dozen roundings of an exponent's argument under 30, and float16's least
+        tol, least = (1.01 * U[dtype] + 512 * 2.0 ** -24) * grad.abs(), 2.0 ** -24 * (dtype == F16) + 2.0 ** -133
+        for reduction in ("none", "mean"):
+            loss = ops.cross_entropy(x, target, reduction=reduction)
+            torch.cuda.synchronize()
+            first = _ops.kernel_status(True)
+            want = each if reduction == "none" else each.sum() / valid.sum()
+            assert (loss.isnan() | ((loss.double() - want).abs() <= 1e-4)).all(), (rows, cols, reduction)
+            assert first != 0 or not loss.isnan().any()
+            (dx,) = torch.autograd.grad(loss.sum(), x)
+            n = 1 if reduction == "none" else valid.sum()
+            torch.cuda.synchronize()
+            bad = ~(dx.isnan() | ((dx.double() - grad / n).abs() <= tol / n + least))
+            assert not bad.any(), (rows, cols, reduction, int(bad.sum()))
+            assert first != 0 or not dx.isnan().any()
+            given_up += first != 0
+            print(f"cross_entropy {rows} {cols} {reduction}: {100 * float(dx.isnan().double().mean()):.2f} % NaN",
+                  flush=True)
+    # the GPU's memory does not fill every block's shared memory within a look
+    assert given_up > 0 or os.environ["COMMUX_KERNEL_WAIT_MS"] != "0"
 
 
 if __name__ == "__main__":

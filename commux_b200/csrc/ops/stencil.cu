@@ -27,6 +27,8 @@ namespace commux_ops {
 
 std::atomic<std::int64_t> g_launches{0};
 
+static std::atomic<unsigned*> g_status{nullptr};  // on the host, once there is one
+
 // host-mapped status word of the kernels with bounded waits (nonzero: one gave up)
 unsigned* status_word(unsigned** dev) {
   struct Word {
@@ -37,10 +39,16 @@ unsigned* status_word(unsigned** dev) {
     C10_CUDA_CHECK(cudaHostAlloc(reinterpret_cast<void**>(&v.host), 64, cudaHostAllocMapped | cudaHostAllocPortable));
     *v.host = 0;
     C10_CUDA_CHECK(cudaHostGetDevicePointer(reinterpret_cast<void**>(&v.device), v.host, 0));
+    g_status.store(v.host);
     return v;
   }();
   *dev = w.device;
   return w.host;
+}
+
+bool wait_gave_up() {
+  const unsigned* host = g_status.load(std::memory_order_relaxed);
+  return host != nullptr && *const_cast<volatile const unsigned*>(host) != 0;
 }
 
 std::uint64_t wait_limit_ns() {

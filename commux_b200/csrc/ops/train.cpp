@@ -119,6 +119,14 @@ void check_held(const Tensor& q, const Tensor& scale, std::int64_t rows, std::in
 std::int8_t* q_ptr(const Tensor& q) { return q.defined() ? q.data_ptr<std::int8_t>() : nullptr; }
 std::uint8_t* s_ptr(const Tensor& s) { return s.defined() ? s.data_ptr<std::uint8_t>() : nullptr; }
 
+// A kernel whose wait ran out has left NaN. Its call has returned long before, so
+// the next one says it; the word is in host memory and nothing waits for the GPU.
+void check_waits(const char* who) {
+  TORCH_CHECK(!commux_ops::wait_gave_up(), who,
+              ": a kernel's wait has run out (COMMUX_KERNEL_WAIT_MS), and results since then may "
+              "be NaN; commux_b200.ops.kernel_status(reset=True) clears this");
+}
+
 void no_second_order(const char* who) {
   TORCH_CHECK(!at::GradMode::is_enabled(), who, ": the backward pass has no derivative (create_graph=True)");
 }
@@ -136,6 +144,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                                const Tensor& weight, const optional<Tensor>& bias, double eps, at::ScalarType out,
                                bool pack, bool train) {
     const char* who = "layer_norm";
+    check_waits(who);
     const Mat m = matrix(x, who, "x");
     check_dtype(out, who, "out_dtype");
     c10::cuda::CUDAGuard guard(x.device());
@@ -198,6 +207,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* who = "layer_norm";
+    check_waits(who);
     no_second_order(who);
     const auto saved = ctx->get_saved_variables();
     const Tensor &kept = saved[0], &q = saved[1], &scale = saved[2], &stats = saved[3], &weight = saved[4];
@@ -275,6 +285,7 @@ variable_list layer_norm(const Tensor& x, const optional<Tensor>& residual, cons
 // --- 8-bit form ------------------------------------------------------------------
 
 std::tuple<Tensor, Tensor> pack8(const Tensor& x) {
+  check_waits("pack8");
   const Mat m = matrix(x, "pack8", "x");
   c10::cuda::CUDAGuard guard(x.device());
   const Held h = new_held(x, m.n, m.cols);
@@ -286,6 +297,7 @@ std::tuple<Tensor, Tensor> pack8(const Tensor& x) {
 Tensor unpack8(const Tensor& q, const Tensor& scale, std::vector<int64_t> sizes, at::ScalarType dtype,
                const optional<Tensor>& weight, const optional<Tensor>& bias) {
   const char* who = "unpack8";
+  check_waits(who);
   check_dtype(dtype, who, "dtype");
   TORCH_CHECK(!sizes.empty() && sizes.back() >= 1, who, ": shape needs rows of one element at least");
   const int64_t cols = sizes.back(), rows = c10::multiply_integers(sizes) / cols;
@@ -311,6 +323,7 @@ struct Gelu8 : torch::autograd::Function<Gelu8<kTanh>> {
   // returns y, then its 8-bit form (if packed)
   static variable_list forward(AutogradContext* ctx, const Tensor& x, bool pack, bool train) {
     const char* who = "gelu8";
+    check_waits(who);
     const Mat m = matrix(x, who, "x");
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor y = at::empty(x.sizes(), x.options());
@@ -343,6 +356,7 @@ struct Gelu8 : torch::autograd::Function<Gelu8<kTanh>> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* who = "gelu8";
+    check_waits(who);
     no_second_order(who);
     variable_list out(3);
     if (!grads[0].defined()) return out;
@@ -376,6 +390,7 @@ std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& q, const
                                         const optional<Tensor>& weight, const optional<Tensor>& bias, bool need_db,
                                         at::ScalarType out) {
   const char* who = "weight_grad8";
+  check_waits(who);
   check_dtype(out, who, "out_dtype");
   const Mat m = matrix(dy, who, "dy");
   same_device(dy, q, who, "the 8-bit form");
@@ -418,6 +433,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
                         const optional<Tensor>& q, const optional<Tensor>& scale, const optional<Tensor>& nw,
                         const optional<Tensor>& nb, bool keep) {
     const char* who = "linear8";
+    check_waits(who);
     const Mat m = matrix(x, who, "x");
     c10::cuda::CUDAGuard guard(x.device());
     same_device(x, weight, who, "weight");
@@ -451,6 +467,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_waits("linear8");
     no_second_order("linear8");
     variable_list out(8);
     const Tensor& dy = grads[0];
@@ -497,6 +514,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& target, int64_t ignore,
                         int64_t reduction, bool train) {
     const char* who = "cross_entropy";
+    check_waits(who);
     const Mat m = matrix(logits, who, "logits");
     same_device(logits, target, who, "targets");
     TORCH_CHECK(target.scalar_type() == at::kLong, who, ": targets must be int64, got ", target.scalar_type());
@@ -525,6 +543,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* who = "cross_entropy";
+    check_waits(who);
     no_second_order(who);
     const auto saved = ctx->get_saved_variables();
     const int64_t reduction = ctx->saved_data["reduction"].toInt();

@@ -151,6 +151,7 @@ extern std::atomic<std::int64_t> g_launches;  // kernels this extension launched
 // Host-mapped status word (nonzero after a bounded wait in a kernel gave up)
 // and its device address.
 unsigned* status_word(unsigned** dev);
+bool wait_gave_up();             // whether the status word says so, without one made for it
 std::uint64_t wait_limit_ns();  // bound of every wait in a kernel (COMMUX_KERNEL_WAIT_MS)
 
 }  // namespace commux_ops

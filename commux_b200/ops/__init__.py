@@ -42,6 +42,13 @@ def launches() -> int:
     return _need_native().launches() if _native is not None else 0
 
 
+def kernel_status(reset: bool = False) -> int:
+    """0, or 1 once a bounded wait in a kernel of this process has run out
+    (``COMMUX_KERNEL_WAIT_MS``). Work on the GPU that has not finished may still
+    set it. ``reset`` clears it; until then the training operators raise."""
+    return _need_native().kernel_status(reset)
+
+
 def jacobi7_reference(u: torch.Tensor, v: torch.Tensor, halo: int) -> float:
     """fp64 PyTorch reference of jacobi7 (writes v's interior, returns the residual)."""
     h = halo
@@ -57,5 +64,5 @@ def jacobi7_reference(u: torch.Tensor, v: torch.Tensor, halo: int) -> float:
 from .train import (Act8, cross_entropy, gelu8, layer_norm, linear8, pack8,  # noqa: E402
                     weight_grad8)
 
-__all__ = ["jacobi7", "jacobi7_reference", "launches", "Act8", "cross_entropy", "gelu8", "layer_norm", "linear8",
-           "pack8", "weight_grad8"]
+__all__ = ["jacobi7", "jacobi7_reference", "kernel_status", "launches", "Act8", "cross_entropy", "gelu8", "layer_norm",
+           "linear8", "pack8", "weight_grad8"]

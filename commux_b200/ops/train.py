@@ -14,6 +14,11 @@ the group's largest magnitude, a value x is held as rint(x / s), so it is off
 by at most s / 2, which is under 1/127 of that magnitude. A finite value stays
 finite (63 s and 65504 in the places of 2^128 and float16's 2^16). A group with
 an infinity or NaN stands for NaN throughout, so an overflow stays visible.
+
+Waits inside the kernels of ``cross_entropy`` and the weight gradient are
+bounded (``COMMUX_KERNEL_WAIT_MS``, 2000 by default). One that runs out leaves
+NaN in the results that were not finished, and every operator raises from then
+on until ``commux_b200.ops.kernel_status(reset=True)``.
 """
 
 from __future__ import annotations

@@ -131,3 +131,8 @@ def test_weight_grad8_waits_that_run_out():
 @pytest.mark.parametrize("limit_ms", ["0", "0.004"])
 def test_cross_entropy_waits_that_run_out(limit_ms):
     _wait_worker("cross_entropy", limit_ms)
+
+
+@gpu
+def test_the_call_after_a_wait_that_ran_out_raises():
+    _wait_worker("raises", "0")

@@ -53,6 +53,29 @@ def weight_grad8():
     assert max(nans) > 0
 
 
+def raises():
+    """The call after one whose wait ran out says so, in both directions; then all is as before."""
+    x, w, t = randn(500, 32001).requires_grad_(), torch.ones(32001, device="cuda"), torch.zeros(500, dtype=torch.int64,
+                                                                                                device="cuda")
+    y, kept = ops.layer_norm(x, w, pack=True)
+    z, u = ops.gelu8(x), ops.linear8(x, w[None].requires_grad_(), act8=kept)
+    assert ops.kernel_status() == 0
+    loss = ops.cross_entropy(x, t)
+    torch.cuda.synchronize()
+    assert loss.isnan() and ops.kernel_status() == 1
+    for f in (lambda: ops.layer_norm(x, w), lambda: ops.gelu8(x), lambda: ops.pack8(x), kept.unpack,
+              lambda: ops.linear8(x, w[None]), lambda: ops.weight_grad8(u.detach(), kept),
+              lambda: ops.cross_entropy(x, t), *(lambda y=y: torch.autograd.grad(y.sum(), x) for y in (loss, y, z, u))):
+        try:
+            f()
+        except RuntimeError as e:
+            assert "wait has run out" in str(e) and "kernel_status(reset=True)" in str(e), e
+        else:
+            raise AssertionError("no error")
+    assert ops.kernel_status(reset=True) == 1 and ops.kernel_status() == 0
+    assert torch.equal(ops.layer_norm(x, w), ops.layer_norm(x, w)) and ops.kernel_status() == 0
+
+
 def cross_entropy():
     given_up = 0
     for rows, cols, dtype in [(700, 9001, BF16), (600, 32000, BF16), (500, 32001, F32), (300, 20000, F32),

@@ -136,3 +136,32 @@ def test_cross_entropy_waits_that_run_out(limit_ms):
 @gpu
 def test_the_call_after_a_wait_that_ran_out_raises():
     _wait_worker("raises", "0")
+
+
+# --- the exact GELU ---------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_gelu8_exact_form_keeps_its_relative_accuracy(dtype):
+    # Phi(x) of a negative x is small, and the product keeps its relative accuracy: half
+    # a unit of the type, and 32 bits' in the exponential's argument z = x^2 / 2 log2(e)
+    # (four roundings of z <= 18 for x >= -5, times ln 2) and about ten beside it.
+    x = -torch.linspace(0.001, 5, 40_000, device="cuda").to(dtype).view(40, 1000)
+    y = ops.gelu8(x, approximate="none").double()
+    x64 = x.double()
+    want = x64 * 0.5 * torch.erfc(-x64 / math.sqrt(2))
+    u, least = {F32: (2.0 ** -24, 2.0 ** -149), BF16: (2.0 ** -8, 2.0 ** -133), F16: (2.0 ** -11, 2.0 ** -24)}[dtype]
+    tol = want.abs() * (u + (4 * 18 * 0.7 + 10) * 2.0 ** -24) + least
+    worst = float(((y - want).abs() / tol).max())
+    assert worst <= 1, worst
+
+
+@gpu
+def test_gelu8_exact_form_against_torch():
+    # no further from 64 bits, in norm, than one and a half times torch's own 32-bit form
+    g = gen(3)
+    x = randn(g, 500, 1000) * torch.where(torch.rand(1000, generator=g, device="cuda") < 0.01, 6.0, 1.0)
+    want = x.double() * 0.5 * torch.erfc(-x.double() / math.sqrt(2))
+    plain = 0.5 * x * (1 + torch.erf(x * math.sqrt(0.5)))
+    off = [float((y.double() - want).norm() / want.norm()) for y in (ops.gelu8(x, approximate="none"), plain)]
+    assert off[0] <= 1.5 * off[1], off

@@ -196,7 +196,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
     if (train) {
       // the packed form replaces the stream itself in what is kept
-      ctx->save_for_backward({pack ? Tensor() : s.defined() ? s : x, held.q, held.scale, stats, weight});
+      ctx->save_for_backward({pack ? Tensor() : s.defined() ? s : m.t, held.q, held.scale, stats, weight});
       // dtypes of x and of the residual, and whether there is a bias, in one number: every entry costs host time
       ctx->saved_data["kinds"] = static_cast<int64_t>(x.scalar_type()) |
                                  (r.t.defined() ? static_cast<int64_t>(residual->scalar_type()) : int64_t{0xff}) << 8 |
@@ -532,7 +532,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
     a.dx = out_ptr(dx);
     C10_CUDA_CHECK(train::xent_forward(a, stream_of(logits)));
     if (train) {
-      ctx->save_for_backward({logits, t, stats, work});
+      ctx->save_for_backward({m.t, t, stats, work});  // a copy that was made serves both passes
       // the gradient for an upstream gradient of one, handed out by the first backward pass
       if (now) ctx->saved_data["unit"] = dx;
       ctx->saved_data["ignore"] = ignore;

@@ -165,3 +165,52 @@ def test_gelu8_exact_form_against_torch():
     plain = 0.5 * x * (1 + torch.erf(x * math.sqrt(0.5)))
     off = [float((y.double() - want).norm() / want.norm()) for y in (ops.gelu8(x, approximate="none"), plain)]
     assert off[0] <= 1.5 * off[1], off
+
+
+# --- orders that are copied -------------------------------------------------------
+
+def _peak_of(f):
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = f()
+    torch.cuda.synchronize()
+    return got, torch.cuda.max_memory_allocated() - before
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_cross_entropy_of_a_shifted_slice_copies_once(reduction):
+    # logits[:, :-1] has outer dimensions that do not merge: the forward pass's copy
+    # serves the backward pass too
+    g = gen(1)
+    x = randn(g, 6, 65, 2000).requires_grad_()
+    target = torch.randint(0, 2000, (6, 64), generator=g, device="cuda")
+    part = x[:, :-1]
+    loss = ops.cross_entropy(part, target, reduction=reduction)
+    up = torch.rand_like(loss)
+    size = 6 * 64 * 2000 * 4
+    (dx,), peak = _peak_of(lambda: torch.autograd.grad(loss, part, up, retain_graph=True))
+    made = size if reduction == "none" else 0  # the mean's is there since the forward pass
+    assert peak <= made + size // 4, (peak, size)
+    ref = part.detach().double().requires_grad_()
+    want = torch.nn.functional.cross_entropy(ref.flatten(0, 1), target.flatten(), reduction=reduction)
+    (wx,) = torch.autograd.grad(want, ref, up.flatten().double() if reduction == "none" else up.double())
+    assert torch.allclose(dx.double(), wx, rtol=1e-5, atol=1e-8)
+    (again,) = torch.autograd.grad(loss, part, up)
+    assert torch.allclose(again, dx, rtol=1e-6, atol=1e-9)
+
+
+@gpu
+def test_layer_norm_of_a_shifted_slice_copies_once():
+    g = gen(2)
+    x, w = randn(g, 6, 129, 1000).requires_grad_(), randn(g, 1000)
+    part = x[:, :-1]
+    y = ops.layer_norm(part, w)
+    dy = randn(g, 6, 128, 1000)
+    size = dy.numel() * 4
+    (dx,), peak = _peak_of(lambda: torch.autograd.grad(y, part, dy))
+    assert peak <= size + size // 4, (peak, size)
+    ref = part.detach().double().requires_grad_()
+    (want,) = torch.autograd.grad(torch.nn.functional.layer_norm(ref, (1000,), w.double()), ref, dy.double())
+    assert torch.allclose(dx.double(), want, rtol=1e-4, atol=1e-5)

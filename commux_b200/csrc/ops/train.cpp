@@ -387,8 +387,8 @@ variable_list gelu8(const Tensor& x, bool tanh_form, bool pack) {
 // --- linear ----------------------------------------------------------------------
 
 std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& q, const Tensor& scale, int64_t cols,
-                                        const optional<Tensor>& weight, const optional<Tensor>& bias, bool need_db,
-                                        at::ScalarType out) {
+                                        const optional<Tensor>& weight, const optional<Tensor>& bias,
+                                        optional<at::ScalarType> db_out, at::ScalarType out) {
   const char* who = "weight_grad8";
   check_waits(who);
   check_dtype(out, who, "out_dtype");
@@ -402,7 +402,7 @@ std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& q, const
   TORCH_CHECK(!b.defined() || (w.defined() && w.scalar_type() == b.scalar_type()), who,
               ": a bias comes with a weight of its dtype");
   const Tensor dw = at::empty({m.cols, cols}, dy.options().dtype(out));
-  const Tensor db = need_db ? at::empty({m.cols}, dy.options().dtype(out)) : Tensor();
+  const Tensor db = db_out.has_value() ? at::empty({m.cols}, dy.options().dtype(*db_out)) : Tensor();
   train::Wgrad8 a{};
   a.dy = m.rows;
   a.q = q_ptr(q);
@@ -413,6 +413,7 @@ std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& q, const
   a.dw = dw.data_ptr();
   a.db = out_ptr(db);
   a.dwt = type_of(dw, who, "out_dtype");
+  a.dbt = db.defined() ? type_of(db, who, "bias") : a.dwt;
   a.rows = m.n;
   a.cols = cols;
   a.outs = m.cols;
@@ -479,9 +480,10 @@ struct Linear8 : torch::autograd::Function<Linear8> {
     if (ctx->needs_input_grad(0)) out[0] = at::matmul(dy, saved[2]);
     if (ctx->needs_input_grad(1)) {
       const auto opt = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); };
-      const auto g = weight_grad8(dy, saved[0], saved[1], saved[2].size(1), opt(saved[3]), opt(saved[4]), need_b, wt);
+      const auto g = weight_grad8(dy, saved[0], saved[1], saved[2].size(1), opt(saved[3]), opt(saved[4]),
+                                  need_b ? optional<at::ScalarType>(static_cast<at::ScalarType>(bt)) : c10::nullopt, wt);
       out[1] = std::get<0>(g);
-      if (need_b) out[2] = std::get<1>(g).to(static_cast<at::ScalarType>(bt));
+      if (need_b) out[2] = std::get<1>(g);
     } else if (need_b) {
       out[2] = dy.reshape({-1, dy.size(-1)}).sum(0, false, static_cast<at::ScalarType>(bt));
     }
@@ -584,7 +586,8 @@ void bind_train(py::module& m) {
   m.def("weight_grad8", [](const Tensor& dy, const Tensor& q, const Tensor& scale, int64_t cols,
                            const optional<Tensor>& weight, const optional<Tensor>& bias, bool need_db,
                            const py::object& out) {
-    return weight_grad8(dy, q, scale, cols, weight, bias, need_db, dtype_of(out));
+    const at::ScalarType t = dtype_of(out);
+    return weight_grad8(dy, q, scale, cols, weight, bias, need_db ? optional<at::ScalarType>(t) : c10::nullopt, t);
   });
   m.def("linear8", &linear8);
   m.def("cross_entropy", &cross_entropy);

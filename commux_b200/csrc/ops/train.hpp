@@ -108,7 +108,7 @@ struct Wgrad8 {
   const void *w, *b;
   Type wt;
   void *dw, *db;  // db may be null
-  Type dwt;
+  Type dwt, dbt;
   void* work;  // wgrad8_work() bytes, 16-byte aligned
   std::int64_t rows, cols, outs;
 };

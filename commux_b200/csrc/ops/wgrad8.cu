@@ -74,7 +74,7 @@ struct Plan {
 
 struct Out {
   void *dw, *db;
-  Type dwt;
+  Type dwt, dbt;
   const void *w, *b;
   Type wt;
   float* slots;
@@ -251,7 +251,7 @@ __device__ __noinline__ void poison(const Plan& p, const Out& out, std::int64_t 
       if (!s.whole)
         slot[kM * kN + row] = nan;
       else if (o < p.outs && s.n0 == 0 && out.db != nullptr)
-        store(out.db, out.dwt, o, nan);
+        store(out.db, out.dbt, o, nan);
     }
     const std::int64_t tile_end = static_cast<std::int64_t>(s.tile + 1) * p.steps;
     at = tile_end < end ? tile_end : end;
@@ -511,7 +511,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (!s.whole)
             slot[kM * kN + rows0 + lane] = column[local0 + lane];
           else if (o < p.outs && out.db != nullptr)
-            store(out.db, out.dwt, o, column[local0 + lane]);
+            store(out.db, out.dbt, o, column[local0 + lane]);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(kJoinThreads) wgrad_join(const Plan p, const O
       float db = 0.0f;
       for (int k = 0; k < n; ++k) db += slot(k)[kM * kN + r];
       column[threadIdx.x] = db;
-      if (n0 == 0 && out.db != nullptr && m0 + r < p.outs) store(out.db, out.dwt, m0 + r, db);
+      if (n0 == 0 && out.db != nullptr && m0 + r < p.outs) store(out.db, out.dbt, m0 + r, db);
     }
     __syncthreads();
   }
@@ -804,7 +804,7 @@ cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   const cudaError_t set = allow_shared<wgrad_tiles>(kSmem);
   if (set != cudaSuccess) return set;
-  const Out out{a.dw, a.db, a.dwt, a.w, a.b, a.wt, static_cast<float*>(a.work)};
+  const Out out{a.dw, a.db, a.dwt, a.dbt, a.w, a.b, a.wt, static_cast<float*>(a.work)};
   unsigned* status = nullptr;
   commux_ops::status_word(&status);
   wgrad_tiles<<<2 * p.pairs, kThreads, kSmem, stream>>>(map_a, map_q, p, out, a.scale, status,

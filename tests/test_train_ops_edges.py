@@ -214,3 +214,20 @@ def test_layer_norm_of_a_shifted_slice_copies_once():
     ref = part.detach().double().requires_grad_()
     (want,) = torch.autograd.grad(torch.nn.functional.layer_norm(ref, (1000,), w.double()), ref, dy.double())
     assert torch.allclose(dx.double(), want, rtol=1e-4, atol=1e-5)
+
+
+# --- linear8 whose bias has another type than its weight ---------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype,wt,bt", [(BF16, BF16, F32), (F16, F16, F32), (F32, BF16, F32), (BF16, F32, BF16)])
+def test_linear8_bias_gradient_in_its_own_type(dtype, wt, bt):
+    # the sum over 150 tokens in 32 bits, rounded once, to the bias's type
+    g = gen(8)
+    x = randn(g, 150, 96, dtype=dtype)
+    w, b = randn(g, 40, 96, dtype=wt).requires_grad_(), randn(g, 40, dtype=bt).requires_grad_()
+    dy = randn(g, 150, 40, dtype=dtype)
+    dw, db = torch.autograd.grad(ops.linear8(x, w, b), (w, b), dy)
+    assert dw.dtype == wt and db.dtype == bt
+    u = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}[bt]
+    want = dy.double().sum(0)
+    assert ((db.double() - want).abs() <= 1.01 * u * want.abs() + 160 * 2.0 ** -24 * dy.double().abs().sum(0)).all()

@@ -10,7 +10,9 @@ With ``GPTConfig(act8=True)`` the same weights run through ``commux_b200.ops``
 (CUDA only): the residual sums inside the norms, every linear layer's input
 but the attention's (which flash SDPA keeps anyway) held in 8 bits for its
 weight's gradient, the norms' and GELU's backward passes from those same
-checkpoints, and the loss with its gradient in one pass over the logits.
+checkpoints, and the loss with its gradient in one pass over the logits. Blocks
+and layers are the same modules with the same parameters, called as modules, so
+hooks and wrappers on them run. Without a gradient nothing is held in 8 bits.
 """
 
 from __future__ import annotations
@@ -36,29 +38,48 @@ class GPTConfig:
     act8: bool = False  # training operators with 8-bit activation checkpoints
 
 
+class Norm8(nn.LayerNorm):
+    def forward(self, x, r=None):
+        """(s, y, y's checkpoint) of ``s = x + r`` (s is x when r is None)."""
+        pack = torch.is_grad_enabled()
+        got = ops.layer_norm(x, self.weight, self.bias, self.eps, residual=r, pack=pack)
+        got = got if isinstance(got, tuple) else (got,)
+        return x if r is None else got[1], got[0], got[-1] if pack else None
+
+
+class Linear8(nn.Linear):
+    def forward(self, x, act8=None):
+        return ops.linear8(x, self.weight, self.bias, act8=act8)
+
+
 class Block(nn.Module):
     def __init__(self, c: GPTConfig):
         super().__init__()
-        self.ln1 = nn.LayerNorm(c.d_model)
-        self.qkv = nn.Linear(c.d_model, 3 * c.d_model)
+        norm, linear = (Norm8, Linear8) if c.act8 else (nn.LayerNorm, nn.Linear)
+        self.ln1 = norm(c.d_model)
+        self.qkv = linear(c.d_model, 3 * c.d_model)
         self.proj = nn.Linear(c.d_model, c.d_model)
-        self.ln2 = nn.LayerNorm(c.d_model)
-        self.fc = nn.Linear(c.d_model, c.d_ff)
-        self.out = nn.Linear(c.d_ff, c.d_model)
+        self.ln2 = norm(c.d_model)
+        self.fc = linear(c.d_model, c.d_ff)
+        self.out = linear(c.d_ff, c.d_model)
         self.n_head = c.n_head
+        self.act8 = c.act8
 
-    def forward(self, x):
+    def forward(self, x, r=None):
+        """With ``act8``, the block on the stream ``x`` and what is still to be added
+        to it (None before the first block); returns the same pair."""
+        if self.act8:
+            return self._forward8(x, r)
         x = x + self.proj(self._attend(self.qkv(self.ln1(x))))
         return x + self.out(F.gelu(self.fc(self.ln2(x)), approximate="tanh"))
 
-    def forward8(self, x, r):
-        """The block on the stream ``x`` and what is still to be added to it
-        (None before the first block); returns the same pair."""
-        x, y, kept = _norm8(self.ln1, x, r)
-        r = self.proj(self._attend(ops.linear8(y, self.qkv.weight, self.qkv.bias, act8=kept)))
-        x, y, kept = _norm8(self.ln2, x, r)
-        a, kept = ops.gelu8(ops.linear8(y, self.fc.weight, self.fc.bias, act8=kept), pack=True)
-        return x, ops.linear8(a, self.out.weight, self.out.bias, act8=kept)
+    def _forward8(self, x, r):
+        x, y, kept = self.ln1(x, r)
+        r = self.proj(self._attend(self.qkv(y, kept)))
+        x, y, kept = self.ln2(x, r)
+        h = self.fc(y, kept)
+        a, kept = ops.gelu8(h, pack=True) if torch.is_grad_enabled() else (ops.gelu8(h), None)
+        return x, self.out(a, kept)
 
     def _attend(self, qkv):
         B, T, C = qkv.shape[0], qkv.shape[1], qkv.shape[2] // 3
@@ -71,15 +92,6 @@ class Block(nn.Module):
         return y.transpose(1, 2).reshape(B, T, C)
 
 
-def _norm8(ln, x, r):
-    """(s, y, y's checkpoint) of ``s = x + r`` (s is x when r is None)."""
-    if r is None:
-        y, kept = ops.layer_norm(x, ln.weight, ln.bias, ln.eps, pack=True)
-        return x, y, kept
-    y, s, kept = ops.layer_norm(x, ln.weight, ln.bias, ln.eps, residual=r, pack=True)
-    return s, y, kept
-
-
 class GPT(nn.Module):
     def __init__(self, c: GPTConfig):
         super().__init__()
@@ -87,8 +99,8 @@ class GPT(nn.Module):
         self.tok = nn.Embedding(c.vocab, c.d_model)
         self.pos = nn.Embedding(c.seq_len, c.d_model)
         self.blocks = nn.ModuleList(Block(c) for _ in range(c.n_layer))
-        self.ln = nn.LayerNorm(c.d_model)
-        self.head = nn.Linear(c.d_model, c.vocab, bias=False)
+        self.ln = (Norm8 if c.act8 else nn.LayerNorm)(c.d_model)
+        self.head = (Linear8 if c.act8 else nn.Linear)(c.d_model, c.vocab, bias=False)
         self.head.weight = self.tok.weight  # tied
         self.apply(self._init)
         for n, p in self.named_parameters():
@@ -119,9 +131,9 @@ class GPT(nn.Module):
     def _forward8(self, x, targets):
         r = None
         for b in self.blocks:
-            x, r = b.forward8(x, r)
-        _, y, kept = _norm8(self.ln, x, r)
-        logits = ops.linear8(y, self.head.weight, act8=kept)
+            x, r = b(x, r)
+        _, y, kept = self.ln(x, r)
+        logits = self.head(y, kept)
         if targets is None:
             return logits
         return ops.cross_entropy(logits, targets)

@@ -231,3 +231,57 @@ def test_linear8_bias_gradient_in_its_own_type(dtype, wt, bt):
     u = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}[bt]
     want = dy.double().sum(0)
     assert ((db.double() - want).abs() <= 1.01 * u * want.abs() + 160 * 2.0 ** -24 * dy.double().abs().sum(0)).all()
+
+
+# --- the model that uses them -------------------------------------------------------
+
+def _small_gpt(**more):
+    from commux_b200.models.gpt import GPT, GPTConfig
+
+    torch.manual_seed(3)
+    return GPT(GPTConfig(n_layer=2, n_head=4, d_model=160, d_ff=448, vocab=1003, seq_len=96, **more))
+
+
+def test_gpt_has_the_same_parameters_with_and_without():
+    plain, held = _small_gpt(), _small_gpt(act8=True)
+    assert {k: v.shape for k, v in plain.state_dict().items()} == {k: v.shape for k, v in held.state_dict().items()}
+    assert all(torch.equal(a, b) for a, b in zip(plain.state_dict().values(), held.state_dict().values()))
+
+
+@gpu
+def test_gpt_without_a_gradient_holds_no_checkpoints(monkeypatch):
+    made = []
+    init = ops.Act8.__init__
+    monkeypatch.setattr(ops.Act8, "__init__", lambda self, *a, **k: (made.append(1), init(self, *a, **k))[1])
+    m = _small_gpt(act8=True).cuda()
+    idx = torch.randint(0, 1003, (2, 96), device="cuda")
+    with torch.no_grad():
+        a = m(idx)
+    assert not made
+    b = m(idx)
+    assert made and torch.equal(a, b)
+
+
+@gpu
+def test_gpt_hooks_and_checkpointing_see_every_layer():
+    m = _small_gpt(act8=True).cuda()
+    idx, target = (torch.randint(0, 1003, (2, 96), device="cuda") for _ in range(2))
+    seen = set()
+    handles = [sub.register_forward_hook(lambda mod, i, o, name=name: seen.add(name))
+               for name, sub in m.named_modules() if name and not isinstance(sub, torch.nn.ModuleList)]
+    loss = m(idx, target)
+    loss.backward()
+    for h in handles:
+        h.remove()
+    assert seen == {name for name, sub in m.named_modules() if name and not isinstance(sub, torch.nn.ModuleList)}
+    want = [p.grad.clone() for p in m.parameters()]
+    # blocks that are run again in the backward pass
+    from torch.utils.checkpoint import checkpoint
+
+    for b in m.blocks:
+        run = b.forward
+        b.forward = lambda *a, run=run: checkpoint(run, *a, use_reentrant=False)
+    m.zero_grad()
+    m(idx, target).backward()
+    for p, g in zip(m.parameters(), want):
+        assert torch.allclose(p.grad, g, rtol=1e-5, atol=1e-8)

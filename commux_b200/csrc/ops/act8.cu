@@ -10,6 +10,8 @@
 // tensor core multiplies it without a second rounding. Against the best step
 // that costs at most one bit of the eight.
 
+#include <type_traits>
+
 #include "train_utils.cuh"
 
 namespace train {
@@ -96,22 +98,22 @@ struct Args {
 
 struct Pack {
   static constexpr bool kReads = true, kHeld = false, kWrites = false;
-  template <typename T>
-  static __device__ __forceinline__ void apply(const Args&, int, const float2 (&)[4], const float2 (&)[4],
+  template <typename T, typename Col>
+  static __device__ __forceinline__ void apply(const Args&, Col, const float2 (&)[4], const float2 (&)[4],
                                                float2 (&)[4]) {}
 };
 
 template <bool kAffine>
 struct Unpack {
   static constexpr bool kReads = false, kHeld = true, kWrites = true;
-  template <typename T>
-  static __device__ __forceinline__ void apply(const Args& a, int c, const float2 (&)[4], const float2 (&h)[4],
+  template <typename T, typename Col>
+  static __device__ __forceinline__ void apply(const Args& a, Col c, const float2 (&)[4], const float2 (&h)[4],
                                                float2 (&y)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       y[i] = h[i];
       if constexpr (kAffine) {
-        const int at = c + 2 * i;
+        const Col at = c + 2 * i;
         const bool one = at < a.cols, two = at + 1 < a.cols;
         y[i] = mul2(y[i], float2{one ? train::load(a.w, a.wt, at) : 0.0f, two ? train::load(a.w, a.wt, at + 1) : 0.0f});
         if (a.b != nullptr)
@@ -129,8 +131,8 @@ struct Unpack {
 template <bool kTanh>
 struct GeluForward {
   static constexpr bool kReads = true, kHeld = false, kWrites = true;
-  template <typename T>
-  static __device__ __forceinline__ void apply(const Args&, int, const float2 (&x)[4], const float2 (&)[4],
+  template <typename T, typename Col>
+  static __device__ __forceinline__ void apply(const Args&, Col, const float2 (&x)[4], const float2 (&)[4],
                                                float2 (&y)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = gelu<kTanh>(x[i]);  // 0 at 0, as past a row's end
@@ -140,8 +142,8 @@ struct GeluForward {
 template <bool kTanh>
 struct GeluBackward {
   static constexpr bool kReads = true, kHeld = true, kWrites = true;
-  template <typename T>
-  static __device__ __forceinline__ void apply(const Args&, int, const float2 (&x)[4], const float2 (&h)[4],
+  template <typename T, typename Col>
+  static __device__ __forceinline__ void apply(const Args&, Col, const float2 (&x)[4], const float2 (&h)[4],
                                                float2 (&y)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = mul2(x[i], gelu_slope<kTanh>(h[i]));
@@ -159,7 +161,8 @@ __device__ __forceinline__ void pack_part(const float2 (&v)[4], std::int8_t* q, 
 
 // A thread takes a few parts of 8 elements; four threads hold a group. kFlat:
 // the rows are whole groups without gaps, so the matrix is one long row (and
-// no index is divided); otherwise Index counts parts through the rows.
+// no index is divided); otherwise Index counts parts through the rows, and a
+// column has as many bits.
 constexpr int unroll_of(bool aligned) { return aligned ? 4 : 2; }  // independent loads, as the registers allow
 
 template <typename T, typename Pass, bool kFlat, bool kAligned, typename Index>
@@ -168,22 +171,27 @@ __global__ void __launch_bounds__(kThreads) eights(const Args a) {
   const Index per = static_cast<Index>((a.cols + kGroup - 1) / kGroup * 4);  // parts of a row
   const Index total = static_cast<Index>(a.rows) * per;
   const Index first = static_cast<Index>(blockIdx.x) * (kThreads * kUnroll) + threadIdx.x;
-  const int cols = kFlat ? 8 : static_cast<int>(a.cols);  // flat: a part is a row of its own
+  using Col = std::conditional_t<sizeof(Index) == 4, int, std::int64_t>;
+  const Col cols = kFlat ? 8 : static_cast<Col>(a.cols);  // flat: a part is a row of its own
   Part<T, kAligned> in[Pass::kReads ? kUnroll : 1];
   uint2 held[kUnroll];
   unsigned e[kUnroll];
   Index row[kUnroll];
-  int col[kUnroll];
+  Col col[kUnroll];
+  // a part's place in its row, for Part, whose columns are ints
+  auto near = [&](Col c) { return sizeof(Col) == 4 ? static_cast<int>(c) : 0; };
+  auto ends = [&](Col c) { return sizeof(Col) == 4 ? static_cast<int>(cols) : static_cast<int>(min(cols - c, Col{64})); };
+  auto skip = [&](Col c) { return sizeof(Col) == 4 ? Col{0} : c; };
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const Index part = first + u * kThreads;
     const bool some = part < total;
     row[u] = kFlat ? part : part / per;
-    col[u] = kFlat ? 0 : static_cast<int>(part - row[u] * per) * 8;
+    col[u] = kFlat ? 0 : static_cast<Col>(part - row[u] * per) * 8;
     if (!some) col[u] = cols;  // past the end: reads 0, writes nothing
     if (Pass::kReads) {
       const std::int64_t at = some ? (kFlat ? static_cast<std::int64_t>(part) * 8 : row[u] * a.x.ld) : 0;
-      in[u].load(static_cast<const T*>(a.x.p) + at, col[u], cols);
+      in[u].load(static_cast<const T*>(a.x.p) + at + skip(col[u]), near(col[u]), ends(col[u]));
     }
     if (Pass::kHeld) {
       held[u] = uint2{0, 0};
@@ -205,8 +213,8 @@ __global__ void __launch_bounds__(kThreads) eights(const Args a) {
       const bool some = part < total;
       T* to = static_cast<T*>(a.y) + (some ? (kFlat ? static_cast<std::int64_t>(part) * 8 : row[u] * a.cols) : 0);
       const int lane = threadIdx.x & 31;
-      Part<T, kAligned>::store(to, col[u], cols, y, lane > 0 && col[u] > 0 && some,
-                               some && (lane == 31 || part + 1 == total || col[u] + 8 >= static_cast<int>(per) * 8));
+      Part<T, kAligned>::store(to + skip(col[u]), near(col[u]), ends(col[u]), y, lane > 0 && col[u] > 0 && some,
+                               some && (lane == 31 || part + 1 == total || col[u] + 8 >= static_cast<Col>(per) * 8));
     }
     if (Pass::kReads && a.xq != nullptr) pack_part(x, a.xq, a.xscale, part, part < total);
     if (Pass::kReads && a.yq != nullptr) pack_part(y, a.yq, a.yscale, part, part < total);
@@ -216,10 +224,14 @@ __global__ void __launch_bounds__(kThreads) eights(const Args a) {
 template <typename T, typename Pass>
 cudaError_t launch(const Args& a, cudaStream_t stream) {
   const std::int64_t parts = a.rows * groups(a.cols) * 4;
-  const bool small = parts < (1ll << 30), aligned = aligned_rows(a.x.p, a.x.ld, a.cols) && small;
+  // 32 bits count the parts, and the columns of a row (a few past its end too)
+  const bool few = parts < (1ll << 30), small = few && a.cols < (1ll << 31) - 64;
+  const bool whole = few && aligned_rows(a.x.p, a.x.ld, a.cols);
+  const bool flat = whole && a.cols % kGroup == 0 && (a.x.ld == a.cols || a.rows == 1) && a.w == nullptr;
+  const bool aligned = flat || (whole && small);
   const std::int64_t each = kThreads * unroll_of(aligned);
   const unsigned blocks = static_cast<unsigned>((parts + each - 1) / each);
-  if (aligned && a.cols % kGroup == 0 && (a.x.ld == a.cols || a.rows == 1) && a.w == nullptr)
+  if (flat)
     eights<T, Pass, true, true, unsigned><<<blocks, kThreads, 0, stream>>>(a);
   else if (aligned)
     eights<T, Pass, false, true, unsigned><<<blocks, kThreads, 0, stream>>>(a);

@@ -386,6 +386,13 @@ variable_list gelu8(const Tensor& x, bool tanh_form, bool pack) {
 
 // --- linear ----------------------------------------------------------------------
 
+// Coordinates of the tiles' copies are 32-bit.
+void check_extent(std::int64_t rows, std::int64_t cols, std::int64_t outs, const char* who) {
+  constexpr std::int64_t most = (1ll << 31) - 1024;
+  TORCH_CHECK(rows <= most && cols <= most && outs <= most, who, ": at most ", most,
+              " rows, columns and outputs, got ", rows, ", ", cols, " and ", outs);
+}
+
 std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& q, const Tensor& scale, int64_t cols,
                                         const optional<Tensor>& weight, const optional<Tensor>& bias,
                                         optional<at::ScalarType> db_out, at::ScalarType out) {
@@ -395,6 +402,7 @@ std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& q, const
   const Mat m = matrix(dy, who, "dy");
   same_device(dy, q, who, "the 8-bit form");
   check_held(q, scale, m.n, cols, who);
+  check_extent(m.n, cols, m.cols, who);
   c10::cuda::CUDAGuard guard(dy.device());
   Tensor w = defined_or(weight), b = defined_or(bias);
   if (w.defined()) w = column_vector(w, dy, cols, who, "weight");
@@ -441,6 +449,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
     TORCH_CHECK(weight.dim() == 2 && weight.size(1) == m.cols, who, ": weight must have shape [outputs, ", m.cols,
                 "], got ", weight.sizes());
     check_dtype(weight.scalar_type(), who, "weight");
+    if (keep) check_extent(m.n, m.cols, weight.size(0), who);
     if (bias.has_value()) {
       same_device(x, *bias, who, "bias");
       TORCH_CHECK(bias->dim() == 1 && bias->size(0) == weight.size(0), who, ": bias must have shape [",

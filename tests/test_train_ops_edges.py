@@ -285,3 +285,50 @@ def test_gpt_hooks_and_checkpointing_see_every_layer():
     m(idx, target).backward()
     for p, g in zip(m.parameters(), want):
         assert torch.allclose(p.grad, g, rtol=1e-5, atol=1e-8)
+
+
+# --- rows of more than 2^31 elements ---------------------------------------------------
+
+def _room(n):
+    if torch.cuda.mem_get_info()[0] < n:
+        pytest.skip(f"needs {n / 1e9:.0f} GB of free device memory")
+
+
+@gpu
+@pytest.mark.parametrize("extra", [37, 64, 72])
+def test_packing_and_gelu_of_rows_past_31_bits(extra):
+    # a group's results do not depend on where in the row it lies
+    _room(60e9)
+    cols = 2 ** 31 + extra
+    x = torch.zeros(1, cols, dtype=BF16, device="cuda")
+    places = [(2 ** 31 - 4096, 4096 + extra), (2 ** 30 - 96, 4096), (0, 4096)]
+    g = gen(extra)
+    for at, n in places:
+        x[0, at:at + n] = randn(g, n, dtype=BF16)
+    kept = ops.pack8(x)
+    values = kept.unpack()
+    for at, n in places:
+        small = ops.pack8(x[:, at:at + n].clone())
+        assert torch.equal(kept.q[:, at:at + n], small.q[:, :n])
+        assert torch.equal(kept.scale[:, at // 32:-(-(at + n) // 32)], small.scale)
+        assert torch.equal(values[:, at:at + n], small.unpack())
+    assert not kept.q[:, cols:].any() and not values[0, 2 ** 31 - 8192:2 ** 31 - 4096].any()
+    del kept, values
+    x.requires_grad_()
+    y = ops.gelu8(x)
+    (dx,) = torch.autograd.grad(y, x, x.detach())
+    for at, n in places:
+        t = x.detach()[:, at:at + n].clone().requires_grad_()
+        z = ops.gelu8(t)
+        (dz,) = torch.autograd.grad(z, t, t.detach())
+        assert torch.equal(y[:, at:at + n], z) and torch.equal(dx[:, at:at + n], dz)
+
+
+@gpu
+def test_weight_grad8_refuses_sizes_past_31_bits():
+    _room(30e9)
+    dy = torch.zeros(1, 2 ** 31, dtype=BF16, device="cuda")
+    with pytest.raises(RuntimeError, match="weight_grad8: at most"):
+        ops.weight_grad8(dy, ops.pack8(torch.ones(1, 1, dtype=BF16, device="cuda")))
+    with pytest.raises(RuntimeError, match="weight_grad8: at most"):
+        ops.weight_grad8(torch.ones(1, 1, dtype=BF16, device="cuda"), ops.pack8(dy))

@@ -527,14 +527,12 @@ Walk walk_of(std::int64_t cols, bool aligned, bool types, bool two) {
 // No more than run at once: the rest would walk over their rows after the others.
 template <auto kKernel>
 int blocks_of(const Walk& p, std::int64_t rows, int least, int shared) {
-  static std::atomic<int> known[kMaxGroup / 32 + 1];  // blocks of an SM, by the warps of one
-  const int threads = p.group * p.ids;
-  int fit = known[threads / 32].load(std::memory_order_relaxed);
-  if (fit == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kKernel, threads, shared) != cudaSuccess || fit < 1)
-      fit = 1;
-    known[threads / 32].store(fit, std::memory_order_relaxed);
-  }
+  // blocks of an SM, by the warps of a group: for one kernel they give a block's threads and its shared memory
+  static Occupancy<kMaxGroup / 32 + 1> known;
+  const int found = known.get(p.group / 32, [&](int* n) {
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, kKernel, p.group * p.ids, shared);
+  });
+  const int fit = found > 0 ? found : 1;
   const std::int64_t most = static_cast<std::int64_t>(sm_count()) * fit;
   const std::int64_t each = static_cast<std::int64_t>(least) * p.ids, want = (rows + each - 1) / each;
   return static_cast<int>(want < most ? want : most);
@@ -584,7 +582,6 @@ cudaError_t launch_fwd(const NormFwd& a, const Walk& p, cudaStream_t stream) {
 
 template <auto kKernel>
 int go_bwd(const NormBwd& a, const Walk& p, float* part, cudaStream_t stream) {
-  // a group's columns, or fewer; known by the threads of a block too
   const int shared = p.ids > 1 ? 2 * 8 * static_cast<int>(sizeof(float)) * p.parts * p.group : 0;
   int blocks = blocks_of<kKernel>(p, a.rows, 4, shared);
   if (blocks > kMostPartials * sm_count()) blocks = kMostPartials * sm_count();

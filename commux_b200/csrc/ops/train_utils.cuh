@@ -264,6 +264,31 @@ cudaError_t allow_shared(int bytes) {
   return rc;
 }
 
+// What an occupancy query answered, by device and a small key; 0: not asked yet.
+// An answer that fails is not kept, and its error is not left to the next check.
+template <int kKeys>
+class Occupancy {
+ public:
+  template <typename F>
+  int get(int key, F query) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= kDevices) device = -1;
+    std::atomic<int>* at = device < 0 ? nullptr : &known_[device][key];
+    int n = at != nullptr ? at->load(std::memory_order_relaxed) : 0;
+    if (n > 0) return n;
+    if (query(&n) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      return 0;
+    }
+    if (at != nullptr) at->store(n, std::memory_order_relaxed);
+    return n;
+  }
+
+ private:
+  static constexpr int kDevices = 16;
+  std::atomic<int> known_[kDevices][kKeys]{};
+};
+
 // Calls f with a value of the element type that t names.
 template <typename F>
 void with_type(Type t, F f) {

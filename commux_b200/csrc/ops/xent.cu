@@ -714,13 +714,9 @@ cudaError_t launch_long(const Xent& a, cudaStream_t stream) {
   cfg.numAttrs = 1;
   // The clusters that run at once (an SM count of a GPU part need not be a
   // multiple of kC): one more would wait for another to finish all its rows.
-  static std::atomic<int> known{0};
-  int most = known.load(std::memory_order_relaxed);
-  if (most == 0) {
-    if (kC == 1 || cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1)
-      most = sm_count() * (kLong / kThreads) / kC;
-    known.store(most, std::memory_order_relaxed);
-  }
+  static Occupancy<1> known;
+  int most = kC == 1 ? 0 : known.get(0, [&](int* n) { return cudaOccupancyMaxActiveClusters(n, kernel, &cfg); });
+  if (most == 0) most = sm_count() * (kLong / kThreads) / kC;
   cfg.gridDim = dim3(static_cast<unsigned>((a.rows < most ? a.rows : most) * kC));
   unsigned* status = nullptr;
   commux_ops::status_word(&status);

@@ -124,8 +124,9 @@ __device__ __forceinline__ bool wait(std::uint32_t bar, unsigned parity, const B
 
 // For a kernel without registers to spare: the call that wait() may make has every
 // thread keep values in local memory, whether it is made or not.
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_inline(std::uint32_t bar, unsigned parity, const Bound& b) {
-  return wait_here<false>(bar, parity, b.gave_up, b.status, b.limit_ns);
+  return wait_here<kCluster>(bar, parity, b.gave_up, b.status, b.limit_ns);
 }
 
 // For blocks of a cluster whose last stores to each other's shared memory nobody

@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
     if constexpr (kWhole && kC == 1) {
       if (!async::wait(async::smem_u32(&bar), parity, bound)) left_at = turn + 1;
     } else {
-      if (!async::wait_inline(async::smem_u32(&bar), parity, bound)) left_at = turn + 1;
+      if (!async::wait_inline<>(async::smem_u32(&bar), parity, bound)) left_at = turn + 1;
     }
   };
   // Whether the block leaves in this turn. Asked after a barrier behind the turn's
@@ -480,7 +480,8 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
       if (leaves(turn)) v = float2{nan_value(), nan_value()};  // the other blocks' rows are not what they should be
       if (t == 0) async::mbar_expect_tx(&joined[set], kC * 8);
       if (t < kC) send(&ranks[set][rank], &joined[set], t, v);
-      if (t == 0) wait(joined[set], turn >> 1 & 1, turn);
+      // what the other blocks stored is acquired from the cluster, not from this block
+      if (t == 0 && !async::wait_inline<true>(async::smem_u32(&joined[set]), turn >> 1 & 1, bound)) left_at = turn + 1;
       __syncthreads();
       v = ranks[set][lane & (kC - 1)];
       v = float2{warp_sum(lane < kC ? v.x : 0.0f), largest(v.y)};

@@ -332,3 +332,93 @@ def test_weight_grad8_refuses_sizes_past_31_bits():
         ops.weight_grad8(dy, ops.pack8(torch.ones(1, 1, dtype=BF16, device="cuda")))
     with pytest.raises(RuntimeError, match="weight_grad8: at most"):
         ops.weight_grad8(torch.ones(1, 1, dtype=BF16, device="cuda"), ops.pack8(dy))
+
+
+# --- ways through the kernels that common sizes do not take ---------------------------
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(400, 9001), (200, 32000), (160, 32001), (60, 40000), (20, 128257)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("ahead,behind", [(0, 8), (0, 5), (8, 8), (3, 4)])
+def test_cross_entropy_of_a_slice(rows, cols, dtype, ahead, behind):
+    # rows apart, off 16-byte boundaries, and lying otherwise than dx's: the same results
+    g = gen(rows + cols)
+    wide = torch.full((rows, ahead + cols + behind), math.nan, dtype=dtype, device="cuda")
+    wide[:, ahead:ahead + cols] = randn(g, rows, cols, dtype=dtype, scale=2.0)
+    x = wide[:, ahead:ahead + cols]
+    target = torch.randint(0, cols, (rows,), generator=g, device="cuda")
+    target[::9] = -100
+    for reduction in ("mean", "none"):
+        got, want = [], []
+        for t, to in ((x.detach(), got), (x.detach().contiguous(), want)):
+            t.requires_grad_()
+            loss = ops.cross_entropy(t, target, reduction=reduction)
+            (dx,) = torch.autograd.grad(loss.sum(), t)
+            to += [loss.detach(), dx]
+        # sums in another order: 2^-20 of a loss of order 10; a probability's and its rounding
+        assert torch.allclose(got[0], want[0], rtol=1e-6, atol=1e-5)
+        assert torch.allclose(got[1].float(), want[1].float(), rtol=2.0 ** -7 if dtype == BF16 else 1e-5, atol=1e-12)
+
+
+@gpu
+@pytest.mark.parametrize("pack", [False, True])
+def test_layer_norm_rows_past_32_bits(pack):
+    # the kernels that hold a row in registers, with their gradients
+    rows, cols = 1_100_001, 2048  # 2.25e9 elements
+    if torch.cuda.mem_get_info()[0] < 60e9:
+        pytest.skip("needs 60 GB of free device memory")
+    g = gen(4)
+    x = torch.zeros(rows, cols, dtype=BF16, device="cuda")
+    tail, w, b = randn(g, 3, cols, dtype=BF16), randn(g, cols, dtype=BF16), randn(g, cols, dtype=BF16)
+    x[-3:] = tail
+    x.requires_grad_()
+    got = ops.layer_norm(x, w, b, pack=pack)
+    y = got[0] if pack else got
+    (dx,) = torch.autograd.grad(y, x, x.detach())
+    t = tail.clone().requires_grad_()
+    got3 = ops.layer_norm(t, w, b, pack=pack)
+    y3 = got3[0] if pack else got3
+    (dx3,) = torch.autograd.grad(y3, t, tail)
+    assert torch.equal(y[-3:], y3) and torch.equal(dx[-3:], dx3)
+    assert not dx[:1000].any() and not dx[rows // 2:rows // 2 + 1000].any()
+    assert torch.equal(y[rows // 2], b)
+    if pack:
+        assert torch.equal(got[-1].q[-3:], got3[-1].q)
+
+
+@gpu
+def test_operators_from_two_threads():
+    # each thread on a stream of its own, the same results as alone
+    import threading
+
+    g = gen(5)
+    xs = [randn(g, 300, 768, dtype=BF16) for _ in range(2)]
+    w, b, wl = randn(g, 768), randn(g, 768), randn(g, 9000, 768)
+    target = torch.randint(0, 9000, (300,), generator=g, device="cuda")
+    torch.cuda.synchronize()
+
+    def step(x):
+        x, ws = x.clone().requires_grad_(), wl.clone().requires_grad_()
+        y, kept = ops.layer_norm(x, w, b, pack=True)
+        loss = ops.cross_entropy(ops.linear8(ops.gelu8(y), ws, act8=None), target)
+        return [loss.detach(), *torch.autograd.grad(loss, [x, ws])]
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(8):
+                    got[k] = step(xs[k])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
+    for a, c in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, c))

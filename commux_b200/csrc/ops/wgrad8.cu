@@ -160,8 +160,9 @@ __device__ __forceinline__ void sync_pair() {
 
 // The address of CTA 0's copy of a barrier, and an arrival there. What this CTA's
 // threads wrote to its shared memory for the products has passed a proxy fence
-// before; a release over the cluster would also wait for every result on its way
-// to memory.
+// before: they are in the memory that the tensor core reads, and no other thread
+// reads them. A release over the cluster for each step would wait for more than
+// that (64 or 82 us for 8192 tokens, 768 -> 3072; 530 or 800 for 16384, 4096 -> 4096).
 __device__ __forceinline__ std::uint32_t leaders(std::uint32_t bar) {
   std::uint32_t there;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(bar));

@@ -408,15 +408,11 @@ __global__ void __launch_bounds__(kThreads, kLong / kThreads)
   __syncthreads();
   if constexpr (kC > 1) cg::this_cluster().sync();  // every block has started: its shared memory can be written
   const async::Bound bound{&gave_up, status, limit_ns};
-  // The long way of a wait is a call, for which every thread keeps values in local
-  // memory, or inlined, which is more code in the loop. 192 or 204 us for 8192 rows of
-  // 32000 bf16, but 213 or 208 of 32001, 127 or 124 for 1024 rows of 128000.
+  // Inlined: the long way of a wait as a call has every thread keep values in local
+  // memory (208 or 222 us for 8192 rows of 32001 bf16, 192 either way of 32000, 120 or
+  // 118 for 1024 rows of 128000).
   auto wait = [&](std::uint64_t& bar, unsigned parity, int turn) {
-    if constexpr (kWhole && kC == 1) {
-      if (!async::wait(async::smem_u32(&bar), parity, bound)) left_at = turn + 1;
-    } else {
-      if (!async::wait_inline<>(async::smem_u32(&bar), parity, bound)) left_at = turn + 1;
-    }
+    if (!async::wait_inline<>(async::smem_u32(&bar), parity, bound)) left_at = turn + 1;
   };
   // Whether the block leaves in this turn. Asked after a barrier behind the turn's
   // waits, so that all threads leave: one that is a turn ahead may have given up there.

@@ -2,8 +2,9 @@
 // input kept in that form. All are HBM-bound: an element costs its own bytes
 // plus 33/32 of a byte for each 8-bit copy. 8192 x 3072 bf16: GELU with two copies
 // 25.9 us (5.9 TB/s), its backward pass 21.9 us (5.8), unpacking 12.5 us (6.1);
-// 4099 x 10001 fp32, exact form, 68 us and 65 us (5.5). Two exponential-unit
-// operations an element keep that unit 50 to 60 % busy beside the memory.
+// 4099 x 10001 fp32, exact form, 73 us and 69 us (5.1; 68 and 65 with a shorter fit, of
+// absolute accuracy). Two exponential-unit operations an element keep that unit 50 to
+// 60 % busy beside the memory.
 //
 // A group's step is a power of two, so x / s and q s are exact, the packing is
 // the same on every path, and q s (7 significant bits) is exact in bf16: a
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) eights(const Args a) {
   Col col[kUnroll];
   // a part's place in its row, for Part, whose columns are ints
   auto near = [&](Col c) { return sizeof(Col) == 4 ? static_cast<int>(c) : 0; };
-  auto ends = [&](Col c) { return sizeof(Col) == 4 ? static_cast<int>(cols) : static_cast<int>(min(cols - c, Col{64})); };
+  auto ends = [&](Col c) { return static_cast<int>(sizeof(Col) == 4 ? cols : min(cols - c, Col{64})); };
   auto skip = [&](Col c) { return sizeof(Col) == 4 ? Col{0} : c; };
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {

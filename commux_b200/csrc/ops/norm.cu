@@ -24,8 +24,9 @@ namespace {
 // while one is worked on. Arithmetic is on pairs of elements. What bounds both next to
 // the memory is how many rows are under way (registers) and the instructions: converting
 // 16-bit values, the group's reductions and the 8-bit form cost as many as the norm
-// itself. 32768 rows of 4096 bf16 take 105 us forward (5.1 TB/s), 135 with the 8-bit
-// form (5.0 TB/s), and 146 backward from it (4.6 TB/s).
+// itself. 32768 rows of 4096 bf16 take 108 us forward (5.0 TB/s; 104 without the
+// correction of the mean), 139 with the 8-bit form (4.8 TB/s), and 157 backward from it
+// with the join of the columns' sums (4.3 TB/s).
 constexpr int kMaxGroup = 512;
 constexpr int kBlock = 256;  // threads of a block of several groups, about
 
@@ -541,10 +542,12 @@ int blocks_of(const Walk& p, std::int64_t rows, int least, int shared) {
 Walk walk_of(const NormBwd& a) {
   const bool all = aligned(a.dy.p, a.dy.ld, a.cols) && aligned(a.ds.p, a.ds.ld, a.cols) &&
                    aligned(a.s.p, a.s.ld, a.cols) && aligned(a.w, a.cols, a.cols);
-  // One part or two: 97 or 87 us for 65536 rows of 1024 bf16, 110 or 85 from the 8-bit
-  // form. With a gradient of the stream as well two spill (185 or 253 us for 16384 rows
+  // One part or two: 112 or 89 us for 65536 rows of 1024 bf16, 110 or 83 from the 8-bit
+  // form. With a gradient of the stream as well two spill (181 or 276 us for 16384 rows
   // of 4096 fp32), and unaligned rows have registers for two from the 8-bit form only
-  // (255 or 349 us for 32768 rows of 3001 bf16, 314 or 296).
+  // (253 or 359 us for 32768 rows of 3001 bf16, 312 or 294). Rows over 4096 take two
+  // all the same: sweeps are slower yet (16384 rows of 8192 fp32 with a gradient of the
+  // stream 591 or 2175 us, 8192 of 6001 476 or 749, 16384 of 6001 bf16 without 392 or 1435).
   const bool two = a.ds.p == nullptr && (all || a.q != nullptr);
   return walk_of(a.cols, all, paired(a.xt, a.dy.t) && (a.dr == nullptr || a.rt == a.dy.t), two);
 }
@@ -600,8 +603,8 @@ int launch_bwd(const NormBwd& a, const Walk& p, float* part, cudaStream_t stream
 cudaError_t norm_forward(const NormFwd& a, cudaStream_t stream) {
   const bool all = aligned(a.x.p, a.x.ld, a.cols) && aligned(a.r.p, a.r.ld, a.cols) && aligned(a.w, a.cols, a.cols) &&
                    aligned(a.b, a.cols, a.cols);
-  // One part or two: 131 or 107 us for 32768 rows of 4096 bf16; unaligned rows, 119 or
-  // 135 us for 65536 of 1001 bf16, but 162 or 107 us for 32768 of fp32 with a residual.
+  // One part or two: 133 or 109 us for 32768 rows of 4096 bf16; unaligned rows, 125 or
+  // 141 us for 65536 of 1001 bf16, but 162 or 115 us for 32768 of fp32 with a residual.
   const Walk p = walk_of(a.cols, all, paired(a.x.t, a.yt) && (a.r.p == nullptr || a.r.t == a.x.t || a.r.t == a.yt),
                          all || a.x.t == Type::f32);
   cudaError_t rc = cudaSuccess;

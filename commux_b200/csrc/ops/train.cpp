@@ -490,7 +490,8 @@ struct Linear8 : torch::autograd::Function<Linear8> {
     if (ctx->needs_input_grad(1)) {
       const auto opt = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); };
       const auto g = weight_grad8(dy, saved[0], saved[1], saved[2].size(1), opt(saved[3]), opt(saved[4]),
-                                  need_b ? optional<at::ScalarType>(static_cast<at::ScalarType>(bt)) : c10::nullopt, wt);
+                                  need_b ? optional<at::ScalarType>(static_cast<at::ScalarType>(bt)) : c10::nullopt,
+                                  wt);
       out[1] = std::get<0>(g);
       if (need_b) out[2] = std::get<1>(g);
     } else if (need_b) {

@@ -12,7 +12,8 @@
 // are further tokens of the same sums, the smallest terms first.
 //
 // 16384 tokens, 4096 x 4096: 451 us for the tiles (1.22 PFLOP/s) and 28 us to join
-// partial tiles; 8192 tokens, 768 x 3072, fp32 results: 51 and 7 us.
+// partial tiles; 8192 tokens, 768 x 3072, fp32 results: 51 and 7 us. 4096 tokens, 4096 x
+// 4096: 348 us in fp16 (two terms, 0.79 PFLOP/s of them) and 485 in fp32 (three, 0.85).
 
 #include <cuda.h>
 

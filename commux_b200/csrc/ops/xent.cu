@@ -295,8 +295,9 @@ __global__ void __launch_bounds__(kRowThreads) xent_rows(const Xent a, const int
 // shared memory until then, its maximum and its exponentials read it from there.
 //
 // A row's chain (wait, maximum, barrier, two reductions) and the instructions bound
-// it next to the memory: 8192 rows of 32000 bf16 with their gradient take 184 us,
-// 5.7 TB/s; 208 us with 32001 columns; 1024 rows of 128001 in clusters of 4 take 146.
+// it next to the memory: 8192 rows of 32000 bf16 with their gradient take 192 us with the
+// small kernels before and after (5.5 TB/s); 208 us with 32001 columns; 1024 rows of
+// 128001 in clusters of 4 take 151.
 
 constexpr int kLong = 1024;    // threads of an SM
 constexpr int kVectors = 4;    // 16-byte vectors of a thread

@@ -3,10 +3,15 @@ a residual stream, activation checkpoints in 8 bits with the backward passes
 that read them, and the softmax cross entropy with its gradient.
 
 Everything here takes CUDA tensors of float32, bfloat16 or float16, works on
-the current stream, computes in 32 bits and rounds once at the end. The last
+the current stream, computes in 32 bits and rounds once at the end. (Inside the
+tensor cores, 32-bit sums are cut off rather than rounded; the weight gradient
+keeps what that costs under 3e-6 of a sum of one sign for float32 results, and
+under a tenth of their own rounding for 16-bit ones.) The last
 dimension is a row; rows may lie apart (a slice of a wider tensor), other
-orders are copied first. Gradients come through autograd; a second derivative
-is refused.
+orders are copied first, once for both passes. Gradients come through autograd; a
+second derivative is refused. What the 8-bit form itself is made of or gives
+(``pack8``, ``Act8.unpack``, ``weight_grad8``) carries no gradient: its results
+are detached, whether or not its arguments require one.
 
 An 8-bit checkpoint holds a row's groups of 32 neighbours with one power-of-two
 step each (33/32 bytes an element): the step s is the smallest with 127 s >=
@@ -39,7 +44,8 @@ class Act8:
     ``scale`` (uint8, [rows, groups of 32]; 2^(scale - 127) is a group's step),
     the tensor's ``shape`` and ``dtype``. A packed :func:`layer_norm` holds the
     normalised input, before ``weight`` and ``bias``, which then belong to the
-    form: the values it stands for are ``held * weight + bias``."""
+    form: the values it stands for are ``held * weight + bias``, with the
+    parameters themselves, so an optimizer's step changes them."""
 
     __slots__ = ("q", "scale", "shape", "dtype", "weight", "bias")
 
@@ -53,7 +59,7 @@ class Act8:
         return self.q.numel() + self.scale.numel()
 
     def unpack(self, dtype: torch.dtype | None = None) -> torch.Tensor:
-        """The values as a tensor (of the held tensor's dtype by default)."""
+        """The values as a tensor (of the held tensor's dtype by default), without a gradient."""
         det = [t.detach() if t is not None else None for t in (self.weight, self.bias)]
         return _native().unpack8(self.q, self.scale, list(self.shape), dtype or self.dtype, *det)
 
@@ -81,7 +87,7 @@ def layer_norm(x, weight, bias=None, eps=1e-5, *, residual=None, out_dtype=None,
 
 
 def pack8(x) -> Act8:
-    """``x`` held in 8 bits."""
+    """``x`` held in 8 bits, without a gradient."""
     q, scale = _native().pack8(x.detach())
     return Act8(q, scale, x.shape, x.dtype)
 
@@ -103,8 +109,8 @@ def linear8(x, weight, bias=None, *, act8=None):
 
     ``act8`` is x's 8-bit form where it is there already (from
     :func:`layer_norm` or :func:`gelu8`); x is packed otherwise. Under autocast
-    x is cast to its dtype; the weight may be of another dtype than x, and its
-    gradient is formed in the weight's dtype directly.
+    x is cast to its dtype; the weight and the bias may be of other dtypes than
+    x, and their gradients are formed in their own.
     """
     if torch.is_autocast_enabled("cuda"):
         x = x.to(torch.get_autocast_dtype("cuda"))
@@ -120,7 +126,7 @@ def weight_grad8(dy, act8, *, bias=False, out_dtype=None):
     """Gradient of a linear layer's weight from its output's gradient ``dy``
     ([..., outputs]) and its input's 8-bit form: ``dy.T @ values``, [outputs,
     columns]. With ``bias``, ``(that, dy summed over the rows)``. ``out_dtype``
-    is dy's dtype by default."""
+    is dy's dtype by default. The result carries no gradient."""
     if dy.shape[:-1] != act8.shape[:-1]:
         raise ValueError(f"weight_grad8: dy is {tuple(dy.shape)}, act8 holds {tuple(act8.shape)}")
     det = [t.detach() if t is not None else None for t in (act8.weight, act8.bias)]

@@ -113,6 +113,23 @@ def test_weight_grad8_long_sums_in_16_bits(dtype):
     assert dw.isfinite().all() and abs(off) <= u * (0.1 + 0.02), off / u
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("rows,cols,outs", [(3000, 2050, 9000), (700, 2100, 9000), (5000, 700, 1500)])
+def test_weight_grad8_terms_in_shared_tiles(rows, cols, outs, dtype):
+    # pairs' parts that begin and end among the lower terms, with and without cuts; each
+    # addition of a sum in tensor memory is off by a unit, 2^-23 of what has been added up
+    g = gen(rows)
+    x, dy = randn(g, rows, cols, dtype=BF16), randn(g, rows, outs, dtype=dtype)
+    kept = ops.pack8(x)
+    dw, db = ops.weight_grad8(dy, kept, bias=True, out_dtype=F32)
+    v, d = kept.unpack(F32).double(), dy.double()
+    want = d.t() @ v
+    assert ((dw.double() - want).abs() <= (rows / 8 + 64) * 2.0 ** -24 * (d.abs().t() @ v.abs())).all()
+    assert float((dw.double() - want).norm() / want.norm()) <= 2 * 96 * 2.0 ** -24.5
+    assert ((db.double() - d.sum(0)).abs() <= (rows / 8 + 64) * 2.0 ** -24 * d.abs().sum(0)).all()
+
+
 # --- waits that run out -------------------------------------------------------------
 
 def _wait_worker(what, limit_ms):

@@ -20,45 +20,6 @@ __device__ __forceinline__ std::uint64_t gtimer() {
   return t;
 }
 
-__device__ __forceinline__ void mbar_init(std::uint64_t* bar, unsigned count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(std::uint64_t* bar, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-               : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(std::uint64_t* bar, unsigned parity) {
-  unsigned done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      " selp.b32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
-// Bounded wait; false if it gave up.
-__device__ __forceinline__ bool mbar_wait(std::uint64_t* bar, unsigned parity, std::uint64_t limit_ns) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const std::uint64_t t0 = gtimer();
-  while (!mbar_try_wait(bar, parity)) {
-    if (gtimer() - t0 > limit_ns) return false;
-  }
-  return true;
-}
-
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
-                                            std::uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<std::uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
-
 // Writes of this thread to shared memory become visible to TMA and the tensor core.
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -163,6 +124,24 @@ __device__ __forceinline__ void load_3d(std::uint32_t dst, const CUtensorMap* ma
       " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(reinterpret_cast<std::uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
+}
+
+// The same by pointers.
+__device__ __forceinline__ void mbar_init(std::uint64_t* bar, unsigned count) { init(smem_u32(bar), count); }
+__device__ __forceinline__ void mbar_expect_tx(std::uint64_t* bar, unsigned bytes) { expect_tx(smem_u32(bar), bytes); }
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
+                                            std::uint64_t* bar) {
+  load_3d(smem_u32(dst), map, x, y, z, smem_u32(bar));
+}
+
+// Bounded wait without a status; false if it gave up.
+__device__ __forceinline__ bool mbar_wait(std::uint64_t* bar, unsigned parity, std::uint64_t limit_ns) {
+  if (try_wait<false>(smem_u32(bar), parity)) return true;
+  const std::uint64_t t0 = gtimer();
+  while (!try_wait<false>(smem_u32(bar), parity)) {
+    if (gtimer() - t0 > limit_ns) return false;
+  }
+  return true;
 }
 
 // A last wait, for a CTA's copies in flight before it ends. Copies arrive within

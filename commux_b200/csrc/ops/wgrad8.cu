@@ -18,6 +18,7 @@
 #include <cuda.h>
 
 #include "async.cuh"
+#include "tensor_map.hpp"
 #include "train_utils.cuh"
 
 namespace train {
@@ -708,22 +709,6 @@ __global__ void __launch_bounds__(256) wgrad_terms(Rows dy, __nv_bfloat16* to, i
   }
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-  static const EncodeTiledFn fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<EncodeTiledFn>(f);
-  }();
-  return fn;
-}
-
 // TMA reads dy itself where it is bf16 with rows on 16-byte boundaries.
 bool as_it_is(const Wgrad8& a) {
   return a.dy.t == Type::bf16 && reinterpret_cast<std::uintptr_t>(a.dy.p) % 16 == 0 && a.dy.ld % 8 == 0 &&
@@ -773,7 +758,7 @@ std::int64_t wgrad8_work(const Wgrad8& a) {
 }
 
 cudaError_t wgrad8(const Wgrad8& a, cudaStream_t stream) {
-  const EncodeTiledFn encode = encode_tiled();
+  const auto encode = commux_ops::encode_tiled();
   if (encode == nullptr) return cudaErrorNotSupported;
   const Plan p = plan_of(a);
   const int count = terms_of(a.dy.t);
